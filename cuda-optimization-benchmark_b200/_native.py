@@ -10,6 +10,7 @@ from pathlib import Path
 from . import _build
 
 c_f = ctypes.c_float
+c_d = ctypes.c_double
 c_i32 = ctypes.c_int32
 c_i64 = ctypes.c_int64
 c_sz = ctypes.c_size_t
@@ -80,6 +81,25 @@ SIGNATURES = {
     "b200_leaky_backward_workspace_bytes": (c_i64, [c_i32, c_i32]),
     "b200_leaky_backward_async": (c_int, [c_p, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_p, c_p, c_f, c_p, c_p, c_p,
                                           c_p, c_p, c_i64, c_p]),
+    # gated linear recurrence
+    "b200_linear_recurrence_checkpoint_bytes": (c_i64, [c_i32, c_i32, c_i32]),
+    "b200_linear_recurrence_workspace_bytes": (c_i64, [c_i32, c_i32, c_i32]),
+    "b200_linear_recurrence_async": (c_int, [c_p, c_p, c_int, c_int, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_p, c_p,
+                                             c_p, c_p, c_i64, c_p]),
+    "b200_linear_recurrence_backward_async": (c_int, [c_p, c_p, c_int, c_int, c_p, c_p, c_p, c_p, c_p, c_i32, c_i32,
+                                                      c_i32, c_p, c_p, c_p, c_p, c_i64, c_p]),
+    "b200_linear_recurrence_step_async": (c_int, [c_p, c_p, c_int, c_int, c_p, c_p, c_p, c_p, c_i32, c_i32, c_i32,
+                                                  c_p, c_p]),
+    # token log-probs, policy and preference losses
+    "b200_token_logprob_async": (c_int, [c_p, c_int, c_p, c_p, c_i32, c_i32, c_i32, c_d, c_p, c_p, c_p, c_p]),
+    "b200_token_logprob_backward_async": (c_int, [c_p, c_int, c_p, c_p, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_d,
+                                                  c_p, c_p]),
+    "b200_policy_loss_workspace_bytes": (c_i64, [c_i32, c_i32]),
+    "b200_policy_loss_async": (c_int, [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i32, c_i32, c_d, c_d, c_d, c_d, c_int,
+                                       c_d, c_int, c_d, c_p, c_p, c_p, c_p, c_i64, c_p]),
+    "b200_preference_loss_workspace_bytes": (c_i64, [c_i32]),
+    "b200_preference_loss_async": (c_int, [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_d, c_int, c_d,
+                                           c_d, c_int, c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_p]),
     # KAN
     "b200_efficient_kan": (None, [c_p, c_p, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_i32, c_i32, c_p]),
     "b200_efficient_kan_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32]),

@@ -17,8 +17,12 @@
 #include "ops/gae.cuh"
 #include "ops/kan_backward.cuh"
 #include "ops/lif_backward.cuh"
+#include "ops/linear_recurrence.cuh"
+#include "ops/policy_loss.cuh"
+#include "ops/preference_loss.cuh"
 #include "ops/rl_step.cuh"
 #include "ops/rtg_chunked.cuh"
+#include "ops/token_logprob.cuh"
 
 namespace {
 thread_local int g_last_status = 0;
@@ -279,6 +283,87 @@ int b200_leaky_backward_async(const float* input_current, const float* checkpoin
   return b200::lif::backward(input_current, checkpoints, beta, threshold, T, B, H, grad_spikes, grad_final_mem, alpha,
                              grad_input, grad_mem0, grad_beta, grad_threshold, workspace, workspace_bytes,
                              as_stream(stream));
+}
+
+// ------------------------------------------------------------------- gated linear recurrence
+int64_t b200_linear_recurrence_checkpoint_bytes(int32_t B, int32_t T, int32_t H) {
+  if (B < 0 || T < 0 || H < 0) return -1;
+  return b200::linrec::checkpoint_count(B, T, H) * int64_t(sizeof(float));
+}
+
+int64_t b200_linear_recurrence_workspace_bytes(int32_t B, int32_t T, int32_t H) {
+  if (B < 0 || T < 0 || H < 0) return -1;
+  return b200::linrec::workspace_bytes(B, T, H);
+}
+
+int b200_linear_recurrence_async(const void* gate, const void* x, int dtype, int form, const int64_t* strides,
+                                 const float* state, const uint8_t* reset, int32_t B, int32_t T, int32_t H, void* h,
+                                 float* final_state, float* checkpoints, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+  return b200::linrec::forward(gate, x, dtype, form, strides, state, reset, B, T, H, h, final_state, checkpoints,
+                               workspace, workspace_bytes, as_stream(stream));
+}
+
+int b200_linear_recurrence_backward_async(const void* gate, const void* x, int dtype, int form,
+                                          const int64_t* strides, const float* checkpoints, const uint8_t* reset,
+                                          const void* grad_h, const float* grad_final, int32_t B, int32_t T, int32_t H,
+                                          void* grad_gate, void* grad_x, float* grad_state, void* workspace,
+                                          int64_t workspace_bytes, void* stream) {
+  return b200::linrec::backward(gate, x, dtype, form, strides, checkpoints, reset, grad_h, grad_final, B, T, H,
+                                grad_gate, grad_x, grad_state, workspace, workspace_bytes, as_stream(stream));
+}
+
+int b200_linear_recurrence_step_async(const void* gate, const void* x, int dtype, int form, const int64_t* strides,
+                                      const float* state, float* state_out, const int32_t* slots, int32_t n_slots,
+                                      int32_t B, int32_t H, void* h, void* stream) {
+  return b200::linrec::step(gate, x, dtype, form, strides, state, state_out, slots, n_slots, B, H, h,
+                            as_stream(stream));
+}
+
+// ------------------------------------------------------------------------- token log-probs
+int b200_token_logprob_async(const void* logits, int dtype, const int64_t* strides, const int64_t* token, int32_t B,
+                             int32_t T, int32_t V, double temperature, float* log_prob, float* entropy, float* stats,
+                             void* stream) {
+  return b200::lp::forward(logits, dtype, strides, token, B, T, V, temperature, log_prob, entropy, stats,
+                           as_stream(stream));
+}
+
+int b200_token_logprob_backward_async(const void* logits, int dtype, const int64_t* strides, const int64_t* token,
+                                      const float* stats, const float* grad_log_prob, const float* grad_entropy,
+                                      int32_t B, int32_t T, int32_t V, double temperature, void* grad_logits,
+                                      void* stream) {
+  return b200::lp::backward(logits, dtype, strides, token, stats, grad_log_prob, grad_entropy, B, T, V, temperature,
+                            grad_logits, as_stream(stream));
+}
+
+// ----------------------------------------------------------------- policy and preference losses
+int64_t b200_policy_loss_workspace_bytes(int32_t B, int32_t T) {
+  if (B < 0 || T < 0) return -1;
+  return b200::policy::workspace_bytes(B, T);
+}
+
+int b200_policy_loss_async(const float* log_prob, const float* old_log_prob, const float* advantage,
+                           const float* ref_log_prob, const float* entropy, const uint8_t* mask,
+                           const int64_t* strides, int32_t B, int32_t T, double clip_low, double clip_high,
+                           double dual_clip, double kl_coef, int kl_form, double entropy_coef, int reduction,
+                           double scale, float* output, float* grad_log_prob, float* grad_entropy, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+  return b200::policy::run(log_prob, old_log_prob, advantage, ref_log_prob, entropy, mask, strides, B, T, clip_low,
+                           clip_high, dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale, output,
+                           grad_log_prob, grad_entropy, workspace, workspace_bytes, as_stream(stream));
+}
+
+int64_t b200_preference_loss_workspace_bytes(int32_t B) { return B < 0 ? -1 : b200::pref::workspace_bytes(B); }
+
+int b200_preference_loss_async(const float* chosen, const float* rejected, const float* ref_chosen,
+                               const float* ref_rejected, const uint8_t* chosen_mask, const uint8_t* rejected_mask,
+                               const int64_t* strides, int32_t B, int32_t Tc, int32_t Tr, double beta, int form,
+                               double label_smoothing, double margin, int average, float* output,
+                               float* reward_chosen, float* reward_rejected, float* grad_chosen,
+                               float* grad_rejected, void* workspace, int64_t workspace_bytes, void* stream) {
+  return b200::pref::run(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, strides, B, Tc, Tr,
+                         beta, form, label_smoothing, margin, average, output, reward_chosen, reward_rejected,
+                         grad_chosen, grad_rejected, workspace, workspace_bytes, as_stream(stream));
 }
 
 // --------------------------------------------------------------------------------- FP8 linear

@@ -10,6 +10,7 @@ non-zero native status; there is no CPU fallback.
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -589,6 +590,574 @@ class LeakyFunction(torch.autograd.Function):
         need = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
         gx, gm, gb, gt = leaky_backward(x, ckpt, beta, threshold, gs, gf, ctx.alpha, need_params=need)
         return gx, gm, gb, gt, None
+
+
+# --------------------------------------------------------------- gated linear recurrence
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # B200_F32, B200_BF16, B200_F16
+RECURRENCE_FORMS = {"decay": 0, "sigmoid": 1}
+_I32_MAX = 2**31 - 1
+
+
+def _strides(*values):
+    """A host array of element strides for the C ABI."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _needs(ctx, k):
+    """Whether apply()'s argument k (which may have been left out) requires a gradient."""
+    return k < len(ctx.needs_input_grad) and ctx.needs_input_grad[k]
+
+
+def _on_device(device):
+    """Context in which `device` is the current one (a launch goes to the current device)."""
+    return torch.cuda.device(device)
+
+
+def _scratch(op, nbytes, device):
+    """workspace(), except that a call being captured into a CUDA graph gets scratch of its own (its
+    zero-fill is captured with it): graphs may be replayed at the same time as one another and as
+    calls outside them."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+    return workspace(op, nbytes, device)
+
+
+def _float_tensor(t, name, device=None, dtype=None, dims=None):
+    """A CUDA tensor of a model (fp32, bf16 or fp16, or `dtype`) whose last axis is contiguous."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor (no CPU path)")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name}: on {t.device}, expected {device}")
+    if dtype is None:
+        if t.dtype not in DTYPE_CODES:
+            raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    elif t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    if dims is not None and t.dim() != dims:
+        raise ValueError(f"{name}: expected {dims} dimensions, got {t.dim()}")
+    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: expected a contiguous last dimension")
+    if any(n > _I32_MAX for n in t.shape):
+        raise ValueError(f"{name}: a dimension is larger than 2^31 - 1")
+    return t
+
+
+def _bth(gate, x, form):
+    """Checks gate and x [B, T, H] of a recurrence: (device, dtype code, form code, B, T, H)."""
+    if form not in RECURRENCE_FORMS:
+        raise ValueError(f"form must be one of {sorted(RECURRENCE_FORMS)}, got {form!r}")
+    _float_tensor(x, "x", dims=3)
+    _float_tensor(gate, "gate", x.device, x.dtype, 3)
+    if gate.shape != x.shape:
+        raise ValueError("gate and x must have the same shape (B, T, H)")
+    B, T, H = x.shape
+    return x.device, DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form], B, T, H
+
+
+def _like_bth(x):
+    """An output of x's shape and dtype: dense, time first in memory when x is."""
+    B, T, H = x.shape
+    if B > 1 and T > 1 and x.stride(0) < x.stride(1):
+        return torch.empty((T, B, H), dtype=x.dtype, device=x.device).transpose(0, 1)
+    return torch.empty((B, T, H), dtype=x.dtype, device=x.device)
+
+
+def _writable(t, like, name):
+    """A caller's output for `like`'s shape: own memory per element."""
+    _float_tensor(t, name, like.device, like.dtype, like.dim())
+    if t.shape != like.shape:
+        raise ValueError(f"{name}: expected shape {tuple(like.shape)}, got {tuple(t.shape)}")
+    if t.numel():
+        dims = sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1)
+        reach = 1
+        for s, n in dims:
+            if s < reach:
+                raise ValueError(f"{name}: elements share memory")
+            reach = s * (n - 1) + reach
+    return t
+
+
+def _state_arg(state, name, B, H, device):
+    if state is None:
+        return None
+    _need(state, name, torch.float32, device)
+    if state.shape != (B, H):
+        raise ValueError(f"{name} must be ({B}, {H})")
+    return state
+
+
+def _reset_arg(reset, B, T, device):
+    if reset is None:
+        return None
+    if not isinstance(reset, torch.Tensor) or not reset.is_cuda or reset.dtype != torch.bool:
+        raise ValueError("reset: expected a CUDA bool tensor")
+    if reset.device != device or reset.shape != (B, T):
+        raise ValueError(f"reset must be ({B}, {T}) on {device}")
+    return reset
+
+
+def _bt_strides(*tensors):
+    out = []
+    for t in tensors:
+        out += [0, 0] if t is None else [t.stride(0), t.stride(1)]
+    return _strides(*out)
+
+
+def _recurrence_forward(gate, x, state, reset, form, out, train):
+    dev, dt, fm, B, T, H = _bth(gate, x, form)
+    state = _state_arg(state, "state", B, H, dev)
+    reset = _reset_arg(reset, B, T, dev)
+    h = _like_bth(x) if out is None else _writable(out, x, "out")
+    lib = _lib()
+    with _on_device(dev):
+        final = torch.empty((B, H), dtype=torch.float32, device=dev)
+        ckpt = None
+        if train:
+            n = lib.b200_linear_recurrence_checkpoint_bytes(B, T, H) // 4
+            ckpt = torch.empty(n, dtype=torch.float32, device=dev)
+        ws = _scratch("linear_recurrence", lib.b200_linear_recurrence_workspace_bytes(B, T, H), dev)
+        _native.check(lib.b200_linear_recurrence_async(
+            _ptr(gate), _ptr(x), dt, fm, _bt_strides(gate, x, h, reset), _ptr(state), _ptr(reset), B, T, H, _ptr(h),
+            _ptr(final), _ptr(ckpt), _ptr(ws), ws.numel(), _stream(dev)), "linear_recurrence")
+    return h, final, ckpt
+
+
+def linear_recurrence(gate, x, state=None, reset=None, form="decay", out=None):
+    """Gated linear recurrence over x [B, T, H]: h[t] = a[t] h[t-1] + v[t] per channel, with a = gate,
+    v = x ("decay", |gate| <= 1 expected) or a = sigmoid(gate), v = (1 - a) x ("sigmoid").
+
+    gate and x: fp32, bf16 or fp16 with a contiguous channel axis and any other strides (halves of one
+    projection, time-first layouts).  state: fp32 [B, H] before the first step (None: 0).  reset: bool
+    [B, T], True where a step starts a new document (the state before it is dropped).  Returns (h of x's
+    dtype, the fp32 state [B, H] after the last step)."""
+    h, final, _ = _recurrence_forward(gate, x, state, reset, form, out, False)
+    return h, final
+
+
+def linear_recurrence_train(gate, x, state=None, reset=None, form="decay"):
+    """linear_recurrence for training: (h, final state, checkpoints); the checkpoints (fp32 states at
+    fixed steps) are what linear_recurrence_backward recomputes h from."""
+    return _recurrence_forward(gate, x, state, reset, form, None, True)
+
+
+def linear_recurrence_backward(gate, x, checkpoints, grad_h, grad_final=None, reset=None, form="decay"):
+    """Gradients of linear_recurrence: (grad_gate, grad_x, grad_state) for grad_h [B, T, H] (x's dtype) and
+    grad_final (fp32 [B, H] or None)."""
+    dev, dt, fm, B, T, H = _bth(gate, x, form)
+    _float_tensor(grad_h, "grad_h", dev, x.dtype, 3)
+    if grad_h.shape != x.shape:
+        raise ValueError("grad_h must have x's shape")
+    grad_final = _state_arg(grad_final, "grad_final", B, H, dev)
+    reset = _reset_arg(reset, B, T, dev)
+    lib = _lib()
+    _need(checkpoints, "checkpoints", torch.float32, dev)
+    if checkpoints.numel() * 4 != lib.b200_linear_recurrence_checkpoint_bytes(B, T, H):
+        raise ValueError("checkpoints do not belong to inputs of this shape")
+    with _on_device(dev):
+        gg, gx = _like_bth(gate), _like_bth(x)
+        gs = torch.empty((B, H), dtype=torch.float32, device=dev)
+        ws = _scratch("linear_recurrence", lib.b200_linear_recurrence_workspace_bytes(B, T, H), dev)
+        _native.check(lib.b200_linear_recurrence_backward_async(
+            _ptr(gate), _ptr(x), dt, fm, _bt_strides(gate, x, grad_h, gg, gx, reset), _ptr(checkpoints), _ptr(reset),
+            _ptr(grad_h), _ptr(grad_final), B, T, H, _ptr(gg), _ptr(gx), _ptr(gs), _ptr(ws), ws.numel(),
+            _stream(dev)), "linear_recurrence_backward")
+    return gg, gx, gs
+
+
+def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, state_out=None):
+    """One token per row: h [B, H] from gate and x [B, H] and a pool of states fp32 [S, H], updated in place
+    (or written to state_out).  slots (int32 [B]) names each row's state, row b its own without it.  Rows
+    with the same slot are consecutive tokens of one sequence, in row order; a row whose slot is outside
+    [0, S) is skipped (its h row is left as it was, so pass `out` to know what it holds)."""
+    if form not in RECURRENCE_FORMS:
+        raise ValueError(f"form must be one of {sorted(RECURRENCE_FORMS)}, got {form!r}")
+    _float_tensor(x, "x", dims=2)
+    dev = x.device
+    _float_tensor(gate, "gate", dev, x.dtype, 2)
+    if gate.shape != x.shape:
+        raise ValueError("gate and x must have the same shape (B, H)")
+    B, H = x.shape
+    _need(state, "state", torch.float32, dev)
+    if state.dim() != 2 or state.shape[1] != H:
+        raise ValueError(f"state must be (slots, {H})")
+    if state_out is None:
+        state_out = state
+    else:
+        _need(state_out, "state_out", torch.float32, dev)
+        if state_out.shape != state.shape:
+            raise ValueError("state_out must have state's shape")
+    if slots is None:
+        if state.shape[0] < B:
+            raise ValueError("state has fewer rows than x and no slots are given")
+    else:
+        _need(slots, "slots", torch.int32, dev)
+        if slots.shape != (B,):
+            raise ValueError(f"slots must be ({B},)")
+    h = torch.empty((B, H), dtype=x.dtype, device=dev) if out is None else _writable(out, x, "out")
+    with _on_device(dev):
+        _native.check(_lib().b200_linear_recurrence_step_async(
+            _ptr(gate), _ptr(x), DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form],
+            _strides(gate.stride(0), x.stride(0), h.stride(0)), _ptr(state), _ptr(state_out), _ptr(slots),
+            state.shape[0], B, H, _ptr(h), _stream(dev)), "linear_recurrence_step")
+    return h
+
+
+class LinearRecurrenceFunction(torch.autograd.Function):
+    """torch.autograd form of the recurrence: apply(gate, x, state, reset, form) -> (h, final state), forward
+    through linear_recurrence_train, backward through linear_recurrence_backward."""
+
+    @staticmethod
+    def forward(ctx, gate, x, state=None, reset=None, form="decay"):
+        h, final, ckpt = linear_recurrence_train(gate, x, state, reset, form)
+        ctx.save_for_backward(gate, x, ckpt, reset)
+        ctx.form = form
+        return h, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_h, grad_final):
+        gate, x, ckpt, reset = ctx.saved_tensors
+        if grad_h is None:
+            grad_h = torch.zeros_like(x)
+        elif grad_h.shape[-1] > 1 and grad_h.stride(-1) != 1:
+            grad_h = grad_h.contiguous()
+        gf = None if grad_final is None else grad_final.contiguous()
+        gg, gx, gs = linear_recurrence_backward(gate, x, ckpt, grad_h, gf, reset, ctx.form)
+        return gg, gx, gs if _needs(ctx, 2) else None, None, None
+
+
+# ------------------------------------------------------------------------------ token log-probs
+def _token_args(logits, token):
+    """(device, dtype code, B, T, V, strides) of logits [..., V] and token [...] with 1 or 2 leading axes."""
+    _float_tensor(logits, "logits")
+    if logits.dim() not in (2, 3):
+        raise ValueError("logits must be (N, V) or (B, T, V)")
+    if not isinstance(token, torch.Tensor) or token.dtype != torch.int64:
+        raise ValueError("token: expected an int64 tensor")
+    if token.device != logits.device:
+        raise ValueError(f"token: on {token.device}, expected {logits.device}")
+    if token.shape != logits.shape[:-1]:
+        raise ValueError("token must have the shape of logits without the last axis")
+    V = logits.shape[-1]
+    if V < 1:
+        raise ValueError("logits: the vocabulary is empty")
+    if logits.dim() == 2:
+        B, T = 1, logits.shape[0]
+        st = _strides(0, logits.stride(0), 0, token.stride(0))
+    else:
+        B, T = logits.shape[:2]
+        st = _strides(logits.stride(0), logits.stride(1), token.stride(0), token.stride(1))
+    if B * T > _I32_MAX:
+        raise ValueError("logits: more than 2^31 - 1 rows")
+    return logits.device, DTYPE_CODES[logits.dtype], B, T, V, st
+
+
+def _temperature(temperature):
+    temperature = float(temperature)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError("temperature must be positive and finite")
+    return temperature
+
+
+def _token_logprob(logits, token, temperature, entropy, train):
+    dev, dt, B, T, V, st = _token_args(logits, token)
+    temperature = _temperature(temperature)
+    with _on_device(dev):
+        lp = torch.empty(token.shape, dtype=torch.float32, device=dev)
+        ent = torch.empty(token.shape, dtype=torch.float32, device=dev) if entropy else None
+        stats = torch.empty((*token.shape, 3), dtype=torch.float32, device=dev) if train else None
+        _native.check(_lib().b200_token_logprob_async(_ptr(logits), dt, st, _ptr(token), B, T, V, temperature,
+                                                      _ptr(lp), _ptr(ent), _ptr(stats), _stream(dev)),
+                      "token_logprob")
+    return lp, ent, stats
+
+
+def token_logprob(logits, token, temperature=1.0, entropy=True):
+    """Log-probability (fp32) of each position's token under softmax(logits / temperature), and that
+    distribution's entropy (fp32, None unless `entropy`).
+
+    logits: fp32, bf16 or fp16 [N, V] or [B, T, V] with a contiguous vocabulary axis (views such as
+    logits[:, :-1] are taken as they are); token: int64 of the leading shape.  A negative token masks its
+    position (outputs 0); a token >= V gives NaN."""
+    lp, ent, _ = _token_logprob(logits, token, temperature, entropy, False)
+    return lp, ent
+
+
+def token_logprob_train(logits, token, temperature=1.0, entropy=True):
+    """token_logprob for training: (log_prob, entropy, stats), stats (fp32 [..., 3]) for
+    token_logprob_backward."""
+    return _token_logprob(logits, token, temperature, entropy, True)
+
+
+def token_logprob_backward(logits, token, stats, grad_log_prob, grad_entropy=None, temperature=1.0, out=None):
+    """grad_logits (contiguous, of logits' dtype) for the gradients of token_logprob's outputs (fp32).  out may
+    be the logits themselves when these are contiguous (they are overwritten)."""
+    dev, dt, B, T, V, st = _token_args(logits, token)
+    temperature = _temperature(temperature)
+    for t, nm, shape in ((stats, "stats", (*token.shape, 3)), (grad_log_prob, "grad_log_prob", token.shape),
+                         (grad_entropy, "grad_entropy", token.shape)):
+        if t is None and nm == "grad_entropy":
+            continue
+        _need(t, nm, torch.float32, dev)
+        if t.shape != shape:
+            raise ValueError(f"{nm} must be {tuple(shape)}")
+    with _on_device(dev):
+        if out is None:
+            out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        else:
+            _need(out, "out", logits.dtype, dev)
+            if out.shape != logits.shape:
+                raise ValueError("out must have logits' shape")
+        _native.check(_lib().b200_token_logprob_backward_async(
+            _ptr(logits), dt, st, _ptr(token), _ptr(stats), _ptr(grad_log_prob), _ptr(grad_entropy), B, T, V,
+            temperature, _ptr(out), _stream(dev)), "token_logprob_backward")
+    return out
+
+
+class TokenLogProbFunction(torch.autograd.Function):
+    """torch.autograd form: apply(logits, token, temperature) -> (log_prob, entropy)."""
+
+    @staticmethod
+    def forward(ctx, logits, token, temperature=1.0):
+        lp, ent, stats = token_logprob_train(logits, token, temperature)
+        ctx.save_for_backward(logits, token, stats)
+        ctx.temperature = float(temperature)
+        ctx.set_materialize_grads(False)
+        return lp, ent
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_lp, grad_ent):
+        logits, token, stats = ctx.saved_tensors
+        if grad_lp is None and grad_ent is None:
+            return None, None, None
+        gl = torch.zeros(token.shape, device=logits.device) if grad_lp is None else grad_lp.contiguous()
+        ge = None if grad_ent is None else grad_ent.contiguous()
+        return token_logprob_backward(logits, token, stats, gl, ge, ctx.temperature), None, None
+
+
+# ----------------------------------------------------------------- policy and preference losses
+KL_FORMS = {"k1": 0, "k2": 1, "k3": 2}
+LOSS_REDUCTIONS = {"token_mean": 0, "sequence_mean": 1, "sum": 2}
+PREFERENCE_FORMS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+POLICY_OUTPUTS = ("loss", "policy", "kl", "entropy", "clip_fraction", "approx_kl", "max_ratio", "mean_ratio")
+PREFERENCE_OUTPUTS = ("loss", "accuracy", "margin")
+
+
+def _token_stream(t, name, B, T, device, dtype=torch.float32):
+    """A [B, T] per-token tensor with a contiguous token axis."""
+    _float_tensor(t, name, device, dtype, 2)
+    if t.shape != (B, T):
+        raise ValueError(f"{name} must be ({B}, {T}), got {tuple(t.shape)}")
+    return t
+
+
+def _row_stride(t):
+    return 0 if t is None else t.stride(0)
+
+
+def _number(v, name):
+    v = float(v)
+    if v != v or v in (float("inf"), float("-inf")):
+        raise ValueError(f"{name} must be finite")
+    return v
+
+
+def _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy, clip_low, clip_high, dual_clip,
+                 kl_coef, kl_form, entropy_coef, reduction, scale, want_grad, want_grad_entropy):
+    _float_tensor(log_prob, "log_prob", dtype=torch.float32, dims=2)
+    dev = log_prob.device
+    B, T = log_prob.shape
+    old = log_prob if old_log_prob is None else _token_stream(old_log_prob, "old_log_prob", B, T, dev)
+    if isinstance(advantage, torch.Tensor) and advantage.dim() == 1:
+        _float_tensor(advantage.unsqueeze(1), "advantage", dev, torch.float32)
+        if advantage.shape != (B,):
+            raise ValueError(f"advantage must be ({B},) or ({B}, {T})")
+        adv_s, adv_e = advantage.stride(0), 0
+    else:
+        _token_stream(advantage, "advantage", B, T, dev)
+        adv_s, adv_e = advantage.stride(0), 1
+    if mask is not None:
+        _token_stream(mask, "mask", B, T, dev, torch.bool)
+    if ref_log_prob is not None:
+        _token_stream(ref_log_prob, "ref_log_prob", B, T, dev)
+    if entropy is not None:
+        _token_stream(entropy, "entropy", B, T, dev)
+    if kl_form not in KL_FORMS:
+        raise ValueError(f"kl_form must be one of {sorted(KL_FORMS)}, got {kl_form!r}")
+    if reduction not in LOSS_REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(LOSS_REDUCTIONS)}, got {reduction!r}")
+    clip_low, clip_high = _number(clip_low, "clip_low"), _number(clip_high, "clip_high")
+    if not 0.0 <= clip_low < 1.0 or clip_high < 0.0:
+        raise ValueError("clip_low must be in [0, 1) and clip_high >= 0")
+    dual = 0.0 if dual_clip is None else _number(dual_clip, "dual_clip")
+    if dual_clip is not None and dual <= 1.0:
+        raise ValueError("dual_clip must be larger than 1")
+    kl_coef, entropy_coef = _number(kl_coef, "kl_coef"), _number(entropy_coef, "entropy_coef")
+    if kl_coef != 0.0 and ref_log_prob is None:
+        raise ValueError("kl_coef needs ref_log_prob")
+    if entropy_coef != 0.0 and entropy is None:
+        raise ValueError("entropy_coef needs entropy")
+    lib = _lib()
+    with _on_device(dev):
+        out = torch.empty(8, dtype=torch.float32, device=dev)
+        grad = torch.empty((B, T), dtype=torch.float32, device=dev) if want_grad else None
+        ge = torch.empty((B, T), dtype=torch.float32, device=dev) if want_grad_entropy else None
+        ws = _scratch("policy_loss", lib.b200_policy_loss_workspace_bytes(B, T), dev)
+        st = _strides(log_prob.stride(0), old.stride(0), adv_s, adv_e, _row_stride(ref_log_prob),
+                      _row_stride(entropy), _row_stride(mask))
+        _native.check(lib.b200_policy_loss_async(
+            _ptr(log_prob), _ptr(old), _ptr(advantage), _ptr(ref_log_prob), _ptr(entropy), _ptr(mask), st, B, T,
+            clip_low, clip_high, dual, kl_coef, KL_FORMS[kl_form], entropy_coef, LOSS_REDUCTIONS[reduction],
+            _number(scale, "scale"), _ptr(out), _ptr(grad), _ptr(ge), _ptr(ws), ws.numel(), _stream(dev)),
+            "policy_loss")
+    return out, grad, ge
+
+
+def policy_loss(log_prob, old_log_prob, advantage, mask=None, ref_log_prob=None, entropy=None, clip_low=0.2,
+                clip_high=0.2, dual_clip=None, kl_coef=0.0, kl_form="k3", entropy_coef=0.0, reduction="token_mean",
+                scale=1.0):
+    """Clipped policy loss of token log-probs fp32 [B, T] with a KL term to ref_log_prob and an entropy
+    term: a tensor of POLICY_OUTPUTS.
+
+    old_log_prob: [B, T], or None for an update on the policy's own samples (ratio 1).  advantage: [B, T],
+    or [B] for one per sequence.  mask: bool [B, T], True where a token counts; what masked-out tokens
+    hold is never looked at.  The token axis of each is contiguous, rows may be strided.  kl_form: "k1", "k2" or "k3";
+    reduction: "token_mean", "sequence_mean" (mean over the non-empty sequences of their means) or
+    "sum"; scale multiplies the loss."""
+    return _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy, clip_low, clip_high,
+                        dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale, False, False)[0]
+
+
+def policy_loss_grad(log_prob, old_log_prob, advantage, mask=None, ref_log_prob=None, entropy=None, clip_low=0.2,
+                     clip_high=0.2, dual_clip=None, kl_coef=0.0, kl_form="k3", entropy_coef=0.0,
+                     reduction="token_mean", scale=1.0):
+    """policy_loss with its gradients: (outputs, d loss / d log_prob [B, T], d loss / d entropy [B, T] or None
+    without an entropy)."""
+    return _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy, clip_low, clip_high,
+                        dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale, True, entropy is not None)
+
+
+class PolicyLossFunction(torch.autograd.Function):
+    """torch.autograd form: apply(log_prob, entropy, old_log_prob, advantage, mask, ref_log_prob, options) ->
+    (loss, outputs), options a dict of policy_loss's other arguments.  The forward computes the gradients
+    with the loss; the backward scales them.  outputs (POLICY_OUTPUTS) carries no gradient."""
+
+    @staticmethod
+    def forward(ctx, log_prob, entropy, old_log_prob, advantage, mask=None, ref_log_prob=None, options=None):
+        if any(_needs(ctx, k) for k in (2, 3, 5)):
+            raise ValueError("PolicyLossFunction: old_log_prob, advantage and ref_log_prob are constants; detach them")
+        o = dict(clip_low=0.2, clip_high=0.2, dual_clip=None, kl_coef=0.0, kl_form="k3", entropy_coef=0.0,
+                 reduction="token_mean", scale=1.0)
+        unknown = set(options or {}) - set(o)
+        if unknown:
+            raise TypeError(f"PolicyLossFunction: unknown options {sorted(unknown)}")
+        o.update(options or {})
+        out, grad, ge = _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy, **o,
+                                     want_grad=ctx.needs_input_grad[0], want_grad_entropy=ctx.needs_input_grad[1])
+        ctx.save_for_backward(grad, ge)
+        ctx.mark_non_differentiable(out)
+        return out[0].clone(), out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss, _):
+        grad, ge = ctx.saved_tensors
+        return (None if grad is None else grad * grad_loss, None if ge is None else ge * grad_loss, None, None, None,
+                None, None)
+
+
+def _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, form,
+                     label_smoothing, margin, average, want_chosen, want_rejected):
+    _float_tensor(chosen, "chosen", dtype=torch.float32, dims=2)
+    dev = chosen.device
+    _float_tensor(rejected, "rejected", dev, torch.float32, 2)
+    (B, Tc), Tr = chosen.shape, rejected.shape[1]
+    if rejected.shape[0] != B:
+        raise ValueError("chosen and rejected must have the same number of rows")
+    if (ref_chosen is None) != (ref_rejected is None):
+        raise ValueError("ref_chosen and ref_rejected go together")
+    for t, nm, T, ty in ((ref_chosen, "ref_chosen", Tc, torch.float32),
+                         (ref_rejected, "ref_rejected", Tr, torch.float32),
+                         (chosen_mask, "chosen_mask", Tc, torch.bool), (rejected_mask, "rejected_mask", Tr, torch.bool)):
+        if t is not None:
+            _token_stream(t, nm, B, T, dev, ty)
+    if form not in PREFERENCE_FORMS:
+        raise ValueError(f"form must be one of {sorted(PREFERENCE_FORMS)}, got {form!r}")
+    beta, margin = _number(beta, "beta"), _number(margin, "margin")
+    label_smoothing = _number(label_smoothing, "label_smoothing")
+    if beta <= 0.0:
+        raise ValueError("beta must be positive")
+    if not 0.0 <= label_smoothing <= 0.5 or (label_smoothing and form != "sigmoid"):
+        raise ValueError("label_smoothing must be in [0, 0.5], and 0 unless form is 'sigmoid'")
+    lib = _lib()
+    with _on_device(dev):
+        out = torch.empty(3, dtype=torch.float32, device=dev)
+        rc, rr = (torch.empty(B, dtype=torch.float32, device=dev) for _ in range(2))
+        gc = torch.empty((B, Tc), dtype=torch.float32, device=dev) if want_chosen else None
+        gr = torch.empty((B, Tr), dtype=torch.float32, device=dev) if want_rejected else None
+        ws = _scratch("preference_loss", lib.b200_preference_loss_workspace_bytes(B), dev)
+        st = _strides(*(_row_stride(t) for t in (chosen, rejected, ref_chosen, ref_rejected, chosen_mask,
+                                                 rejected_mask)))
+        _native.check(lib.b200_preference_loss_async(
+            _ptr(chosen), _ptr(rejected), _ptr(ref_chosen), _ptr(ref_rejected), _ptr(chosen_mask),
+            _ptr(rejected_mask), st, B, Tc, Tr, beta, PREFERENCE_FORMS[form], label_smoothing, margin,
+            int(bool(average)), _ptr(out), _ptr(rc), _ptr(rr), _ptr(gc), _ptr(gr), _ptr(ws), ws.numel(),
+            _stream(dev)), "preference_loss")
+    return out, rc, rr, gc, gr
+
+
+def preference_loss(chosen, rejected, ref_chosen=None, ref_rejected=None, chosen_mask=None, rejected_mask=None,
+                    beta=0.1, form="sigmoid", label_smoothing=0.0, margin=0.0, average=False):
+    """Preference loss over pairs of answers given as token log-probs fp32 [B, Tc] and [B, Tr]: (a tensor of
+    PREFERENCE_OUTPUTS, reward_chosen [B], reward_rejected [B]).
+
+    Each answer counts with the sum (the mean with `average`) of its masked tokens' log_prob - ref_log_prob;
+    z = beta * (chosen - rejected) - margin goes through form "sigmoid" (with label_smoothing),
+    "hinge" or "ipo".  Without the references the log-probs count alone.  masks: bool, True where a token
+    counts.  Rows may be strided (halves of one concatenated batch)."""
+    return _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, form,
+                            label_smoothing, margin, average, False, False)[:3]
+
+
+def preference_loss_grad(chosen, rejected, ref_chosen=None, ref_rejected=None, chosen_mask=None, rejected_mask=None,
+                         beta=0.1, form="sigmoid", label_smoothing=0.0, margin=0.0, average=False):
+    """preference_loss with its gradients: (outputs, reward_chosen, reward_rejected, d loss / d chosen [B, Tc],
+    d loss / d rejected [B, Tr])."""
+    return _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, form,
+                            label_smoothing, margin, average, True, True)
+
+
+class PreferenceLossFunction(torch.autograd.Function):
+    """torch.autograd form: apply(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, options)
+    -> (loss, outputs, reward_chosen, reward_rejected), options a dict of preference_loss's other arguments.
+    Only the loss carries a gradient."""
+
+    @staticmethod
+    def forward(ctx, chosen, rejected, ref_chosen=None, ref_rejected=None, chosen_mask=None, rejected_mask=None,
+                options=None):
+        if _needs(ctx, 2) or _needs(ctx, 3):
+            raise ValueError("PreferenceLossFunction: the reference log-probs are constants; detach them")
+        o = dict(beta=0.1, form="sigmoid", label_smoothing=0.0, margin=0.0, average=False)
+        unknown = set(options or {}) - set(o)
+        if unknown:
+            raise TypeError(f"PreferenceLossFunction: unknown options {sorted(unknown)}")
+        o.update(options or {})
+        out, rc, rr, gc, gr = _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask,
+                                               **o, want_chosen=ctx.needs_input_grad[0],
+                                               want_rejected=ctx.needs_input_grad[1])
+        ctx.save_for_backward(gc, gr)
+        ctx.mark_non_differentiable(out, rc, rr)
+        return out[0].clone(), out, rc, rr
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss, *_):
+        gc, gr = ctx.saved_tensors
+        return (None if gc is None else gc * grad_loss, None if gr is None else gr * grad_loss, None, None, None, None,
+                None)
 
 
 # ----------------------------------------------------------------------------------------- KAN

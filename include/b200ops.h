@@ -312,6 +312,140 @@ int b200_leaky_backward_async(const float* input_current, const float* checkpoin
                               void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Gated linear recurrence (no reference counterpart; the trainable recurrent layer beside leaky),
+ * over [B, T, H], per channel, state and arithmetic in fp32:
+ *   h[t] = a[t] * h[t-1] + v[t],  h[-1] = state (0 when state is NULL)
+ *     B200_RECURRENCE_DECAY:    a = gate,          v = x
+ *     B200_RECURRENCE_SIGMOID:  a = sigmoid(gate), v = (1 - a) * x
+ * reset (bytes [B, T], may be NULL) != 0 drops h[t-1]: the first step of a packed document, whatever
+ * the state before it held (infinities and NaN included).  |a| <= 1 is expected: steps are composed
+ * by products of a in fp32, which must stay finite.
+ * gate, x, h and the gradients are of `dtype`; their channel axis is contiguous, their batch and time
+ * strides (in elements) come in the host array `strides`, as pairs (batch, time):
+ *   forward:   gate, x, h, reset                           (8 values)
+ *   backward:  gate, x, grad_h, grad_gate, grad_x, reset   (12 values)
+ *   step:      the row strides of gate, x and h            (3 values)
+ * Outputs may not overlap the inputs or one another.  state, final_state, grad_final and grad_state
+ * are fp32 [B, H].  final_state, checkpoints, grad_final and grad_state may be NULL.
+ *
+ * For training the forward stores the state at every tile's start
+ * (b200_linear_recurrence_checkpoint_bytes bytes, fp32) and the backward recomputes h from it:
+ *   g[t] = grad_h[t] + a[t+1] * g[t+1],  g[T-1] = grad_h[T-1] + grad_final
+ *     decay: grad_x = g, grad_gate = g * h[t-1]
+ *     sigmoid: grad_x = (1 - a) * g, grad_gate = g * (h[t-1] - x) * a * (1 - a)
+ *   grad_state = a[0] * g[0]
+ * workspace: b200_linear_recurrence_workspace_bytes(B, T, H) bytes for either direction, 16-byte
+ * aligned, zero-filled once before first use (every call leaves it ready for the next), used by one
+ * stream at a time.  Results are the same bits on every call.
+ *
+ * The step advances B rows by one token: row b reads state[slot] (fp32 [n_slots, H]) and writes
+ * h[b] and state_out[slot] (state_out may be state), slot = slots[b], or b when slots is NULL (then
+ * n_slots >= B).  Rows that name the same slot are consecutive tokens of one sequence, in row order.
+ * A row whose slot is outside [0, n_slots) is skipped: its h row is left as it was.
+ * ------------------------------------------------------------------------------------------- */
+#define B200_F32 0
+#define B200_BF16 1
+#define B200_F16 2
+#define B200_RECURRENCE_DECAY 0
+#define B200_RECURRENCE_SIGMOID 1
+int64_t b200_linear_recurrence_checkpoint_bytes(int32_t B, int32_t T, int32_t H);
+int64_t b200_linear_recurrence_workspace_bytes(int32_t B, int32_t T, int32_t H);
+int b200_linear_recurrence_async(const void* gate, const void* x, int dtype, int form, const int64_t* strides,
+                                 const float* state, const uint8_t* reset, int32_t B, int32_t T, int32_t H, void* h,
+                                 float* final_state, float* checkpoints, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+int b200_linear_recurrence_backward_async(const void* gate, const void* x, int dtype, int form,
+                                          const int64_t* strides, const float* checkpoints, const uint8_t* reset,
+                                          const void* grad_h, const float* grad_final, int32_t B, int32_t T, int32_t H,
+                                          void* grad_gate, void* grad_x, float* grad_state, void* workspace,
+                                          int64_t workspace_bytes, void* stream);
+int b200_linear_recurrence_step_async(const void* gate, const void* x, int dtype, int form, const int64_t* strides,
+                                      const float* state, float* state_out, const int32_t* slots, int32_t n_slots,
+                                      int32_t B, int32_t H, void* h, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Token log-probabilities and entropies from logits (no reference counterpart: where the
+ * current_log_prob and entropy streams of ppo_clip come from).  For each of B x T positions, with z
+ * the V logits / temperature (temperature > 0): log_prob = z[token] - log sum exp z, entropy (may be
+ * NULL) of softmax(z), both fp32 [B, T].  logits are of `dtype` with a contiguous vocabulary axis;
+ * `strides` (host array, elements): logits batch, logits time, token batch, token time.  A negative
+ * token masks its position: outputs and gradient 0, its logits not read.  token >= V gives NaN.
+ * A -inf logit has probability 0; a position whose logits are all -inf, or that has a NaN or +inf
+ * logit, gives NaN.
+ * stats (may be NULL) receives fp32 [B, T, 3] (maximum, log-sum, entropy) for the backward:
+ *   grad_logits = (grad_log_prob ([i = token] - p_i) - grad_entropy p_i (log p_i + entropy)) / temperature
+ * with grad_log_prob fp32 [B, T], grad_entropy the same or NULL, grad_logits contiguous [B, T, V] of
+ * `dtype`, which may be the logits' own memory when these are contiguous.
+ * ------------------------------------------------------------------------------------------- */
+int b200_token_logprob_async(const void* logits, int dtype, const int64_t* strides, const int64_t* token, int32_t B,
+                             int32_t T, int32_t V, double temperature, float* log_prob, float* entropy, float* stats,
+                             void* stream);
+int b200_token_logprob_backward_async(const void* logits, int dtype, const int64_t* strides, const int64_t* token,
+                                      const float* stats, const float* grad_log_prob, const float* grad_entropy,
+                                      int32_t B, int32_t T, int32_t V, double temperature, void* grad_logits,
+                                      void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Clipped policy loss over masked token log-probs with its gradients (no reference counterpart:
+ * ppo_clip gives the flat loss and its diagnostics; this is what a token policy is trained on).
+ * Per token with mask != 0 (every token when mask is NULL), d = log_prob - old_log_prob, r = exp(d):
+ *   gain = min(r A, clip(r, 1 - clip_low, 1 + clip_high) A); with dual_clip c > 1 (0: off) and A < 0,
+ *   max(gain, c A);  kl with q = ref - log_prob: B200_KL_K1 -q, _K2 q^2 / 2, _K3 exp(q) - q - 1
+ *   loss = sum w (-gain + kl_coef kl - entropy_coef entropy)
+ * w = scale / masked tokens (B200_LOSS_TOKEN_MEAN), scale / (rows with tokens * the row's tokens)
+ * (B200_LOSS_SEQUENCE_MEAN), or scale (B200_LOSS_SUM).  output (fp32 [8]): loss; the weighted sums
+ * of -gain, kl and entropy; over the masked tokens the fraction with r outside the clip range, the
+ * mean of exp(d) - 1 - d, the largest r, the mean r.  grad_log_prob and grad_entropy (fp32 contiguous
+ * [B, T], may be NULL) receive d loss / d of each; old, ref and advantage are constants.  Masked-out
+ * tokens are not looked at (NaN and infinities there do not count) and get gradient 0; without any
+ * token all outputs are 0.  ref_log_prob (then kl is 0) and entropy may be NULL.
+ * strides (host array, elements): rows of log_prob, old_log_prob, advantage; 1, or 0 when advantage
+ * holds one value per row; rows of ref_log_prob, entropy, mask.  The token axis is contiguous.
+ * workspace: b200_policy_loss_workspace_bytes(B, T) bytes, 16-byte aligned, zero-filled once before
+ * first use, used by one stream at a time.
+ * ------------------------------------------------------------------------------------------- */
+#define B200_KL_K1 0
+#define B200_KL_K2 1
+#define B200_KL_K3 2
+#define B200_LOSS_TOKEN_MEAN 0
+#define B200_LOSS_SEQUENCE_MEAN 1
+#define B200_LOSS_SUM 2
+int64_t b200_policy_loss_workspace_bytes(int32_t B, int32_t T);
+int b200_policy_loss_async(const float* log_prob, const float* old_log_prob, const float* advantage,
+                           const float* ref_log_prob, const float* entropy, const uint8_t* mask,
+                           const int64_t* strides, int32_t B, int32_t T, double clip_low, double clip_high,
+                           double dual_clip, double kl_coef, int kl_form, double entropy_coef, int reduction,
+                           double scale, float* output, float* grad_log_prob, float* grad_entropy, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Preference loss over B pairs of answers with its gradients (no reference counterpart; it trains the
+ * same token log-probs from preferences instead of advantages).  s = sum over the answer's masked tokens of
+ * log_prob - ref_log_prob (log_prob alone when both ref pointers are NULL), divided by their number
+ * when average != 0 (an answer without tokens: 0); z = beta (s_chosen - s_rejected) - margin:
+ *   B200_PREFERENCE_SIGMOID  -(1 - e) log sigmoid(z) - e log sigmoid(-z), e = label_smoothing in [0, 0.5]
+ *   B200_PREFERENCE_HINGE    max(0, 1 - z)
+ *   B200_PREFERENCE_IPO      ((z - 1/2) / beta)^2
+ * output (fp32 [3]): means over the pairs of the loss, of [s_chosen > s_rejected] and of
+ * beta (s_chosen - s_rejected); reward_* (fp32 [B]) = beta s.  grad_chosen [B, Tc] and grad_rejected
+ * [B, Tr] (fp32 contiguous, may be NULL) receive the gradients of the mean loss, 0 on masked-out
+ * tokens, which are not looked at.  B = 0 gives 0.  strides (host array, elements): rows of chosen,
+ * rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask; the token axis is contiguous.
+ * workspace: b200_preference_loss_workspace_bytes(B) bytes, 16-byte aligned, zero-filled once before
+ * first use, used by one stream at a time.
+ * ------------------------------------------------------------------------------------------- */
+#define B200_PREFERENCE_SIGMOID 0
+#define B200_PREFERENCE_HINGE 1
+#define B200_PREFERENCE_IPO 2
+int64_t b200_preference_loss_workspace_bytes(int32_t B);
+int b200_preference_loss_async(const float* chosen, const float* rejected, const float* ref_chosen,
+                               const float* ref_rejected, const uint8_t* chosen_mask, const uint8_t* rejected_mask,
+                               const int64_t* strides, int32_t B, int32_t Tc, int32_t Tr, double beta, int form,
+                               double label_smoothing, double margin, int average, float* output,
+                               float* reward_chosen, float* reward_rejected, float* grad_chosen,
+                               float* grad_rejected, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * KAN linear layer (task efficient_kan): out[B, O] = silu(x) . base_weight^T + bases(x) .
  * (spline_weight * spline_scaler)^T, with the G + K B-spline bases of order K on each input's
  * knot grid[I, G + 2K + 1].

@@ -356,3 +356,213 @@ def efficient_kan_backward(inp, grad_out, rows=None):
             "grad_x_abs": grad_x_abs, "grad_base_weight_abs": gw_base_abs,
             "grad_spline_weight_abs": gw_spl_abs * np.abs(sc[:, :, None]),
             "grad_spline_scaler_abs": (gw_spl_abs * np.abs(sw)).sum(axis=2)}
+
+
+# ------------------------------------------------------------------- gated linear recurrence
+def _f64(t):
+    if hasattr(t, "detach"):
+        t = t.detach().cpu()
+        return t.numpy() if str(t.dtype) == "torch.bool" else t.double().numpy()
+    t = np.asarray(t)
+    return t if t.dtype == bool else t.astype(np.float64)
+
+
+U32 = 2.0 ** -24  # half a step of fp32, relative
+
+
+def linear_recurrence(gate, x, state=None, reset=None, form="decay", grad_h=None, grad_final=None):
+    """The gated linear recurrence in fp64, step by step: h[t] = a h[t-1] + v (decay: a = gate, v = x;
+    sigmoid: a = s(gate), v = (1 - a) x; reset drops h[t-1]) and, with grad_h, its gradients.  Returns
+    (values, errors): errors[k] bounds the error of values[k] when every step is done in fp32, in any
+    association of the scan.
+
+    The bound: a step's result carries the error of the state it starts from, times |a|, and at most 16
+    roundings relative to M, the recurrence of the absolute values (a sigmoid: exp 4, its argument's
+    scaling 2, sum, reciprocal and product 4; a map's composition 2, the final fma 1, the step's own
+    products 3).  The backward's recurrence is bounded the same way."""
+    gate, x = _f64(gate), _f64(x)
+    B, T, H = x.shape
+    keep = np.ones((B, T, 1)) if reset is None else 1.0 - _f64(reset).astype(np.float64)[:, :, None]
+    live = keep > 0
+    if form == "decay":
+        a, na, v = gate, np.ones_like(gate), x
+    else:
+        e = np.exp(-np.abs(gate))
+        a = np.where(gate >= 0, 1.0, e) / (1.0 + e)
+        na = np.where(gate >= 0, e, 1.0) / (1.0 + e)
+        v = na * x
+    cur = np.zeros((B, H)) if state is None else _f64(state).copy()
+    mag, err = np.abs(cur), np.zeros((B, H))
+    h, prev, eh, eprev = (np.empty_like(x) for _ in range(4))
+    for t in range(T):
+        prev[:, t] = np.where(live[:, t], cur, 0.0)
+        eprev[:, t] = err * keep[:, t]
+        cur = a[:, t] * prev[:, t] + v[:, t]
+        mag = np.abs(a[:, t]) * np.where(live[:, t], mag, 0.0) + np.abs(v[:, t])
+        err = np.abs(a[:, t]) * eprev[:, t] + 16 * U32 * mag
+        h[:, t], eh[:, t] = cur, err
+    val = {"h": h, "final": cur.copy()}
+    bound = {"h": eh, "final": err.copy()}
+    if grad_h is None:
+        return val, bound
+    dh = _f64(grad_h)
+    acc = np.zeros((B, H)) if grad_final is None else _f64(grad_final).copy()
+    mag, err = np.abs(acc), np.zeros((B, H))
+    gg, gx, egg, egx = (np.empty_like(x) for _ in range(4))
+    for t in range(T - 1, -1, -1):
+        g = dh[:, t] + acc
+        mag = mag + np.abs(dh[:, t])
+        err = err + 16 * U32 * mag
+        if form == "decay":
+            gg[:, t] = g * prev[:, t]
+            egg[:, t] = err * np.abs(prev[:, t]) + np.abs(g) * eprev[:, t] + 4 * U32 * np.abs(gg[:, t])
+        else:
+            d, s = prev[:, t] - x[:, t], a[:, t] * na[:, t]
+            gg[:, t] = g * d * s
+            egg[:, t] = (err * np.abs(d) + np.abs(g) * (eprev[:, t] + U32 * np.abs(d)) + 24 * U32 * np.abs(g * d)) * s
+        gx[:, t] = na[:, t] * g
+        egx[:, t] = na[:, t] * (err + 16 * U32 * np.abs(g))
+        acc = a[:, t] * g * keep[:, t]
+        mag = np.abs(a[:, t]) * mag * keep[:, t]
+        err = np.abs(a[:, t]) * err * keep[:, t] + 16 * U32 * mag
+    val.update(grad_gate=gg, grad_x=gx, grad_state=acc)
+    bound.update(grad_gate=egg, grad_x=egx, grad_state=err)
+    return val, bound
+
+
+# ------------------------------------------------------------------------- token log-probs
+def token_logprob(logits, token, temperature=1.0, grad_log_prob=None, grad_entropy=None):
+    """log softmax(logits / temperature)[token] and the entropy in fp64 (0 where token < 0), with the gradient
+    of the logits where gradients are given.  Returns (values, errors) as linear_recurrence.
+
+    The bound: exp has a relative error of 4 u and its argument d one of 3 u |d| (difference, scaling by a
+    rounded 1 / temperature), a sum of V terms by at most 256 threads ceil(V / 256) + 16 roundings, so
+    K = ceil(V / 256) + 32 roundings cover log S and p beside the |d| part."""
+    x, tok = _f64(logits), np.asarray(token.cpu() if hasattr(token, "cpu") else token)
+    V = x.shape[-1]
+    K = -(-V // 256) + 32
+    with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
+        d = (x - x.max(-1, keepdims=True)) / temperature
+        e = np.exp(d)
+        log_s = np.log(e.sum(-1, keepdims=True))
+        logp = d - log_s
+        p = np.exp(logp)
+        plogp = np.where(p > 0, p * logp, 0.0)
+        pd = np.where(p > 0, p * np.abs(d), 0.0).sum(-1)
+    ent = -plogp.sum(-1)
+    on = tok >= 0
+    at = np.clip(tok, 0, V - 1)
+    lp = np.take_along_axis(logp, at[..., None], -1)[..., 0]
+    dt = np.abs(np.take_along_axis(d, at[..., None], -1)[..., 0])
+    base = K * U32 * (1 + np.abs(log_s[..., 0])) + 4 * U32 * pd
+    val = {"log_prob": np.where(on, lp, 0.0), "entropy": np.where(on, ent, 0.0)}
+    bound = {"log_prob": np.where(np.isfinite(dt), base + 4 * U32 * dt, 0.0) * on,
+             "entropy": (base * (1 + pd) + K * U32 * pd) * on}
+    if grad_log_prob is None:
+        return val, bound
+    gl = _f64(grad_log_prob)[..., None]
+    ge = np.zeros_like(gl) if grad_entropy is None else _f64(grad_entropy)[..., None]
+    hot = np.zeros_like(x)
+    np.put_along_axis(hot, at[..., None], 1.0, -1)
+    with np.errstate(invalid="ignore"):
+        pl = np.where(p > 0, p * (logp + ent[..., None]), 0.0)
+        g = (gl * (hot - p) - ge * pl) / temperature
+        rel = K * U32 + base[..., None] + 4 * U32 * np.where(p > 0, np.abs(d), 0.0)
+        size = np.abs(gl) * p + np.abs(ge) * p * (np.where(p > 0, np.abs(logp), 0.0) + np.abs(ent[..., None]))
+        eg = (size * rel + np.abs(ge) * p * (bound["entropy"][..., None] + base[..., None]) +
+              4 * U32 * np.abs(gl) * hot) / temperature
+    val["grad_logits"] = np.where(on[..., None], g, 0.0)
+    bound["grad_logits"] = np.where(on[..., None], eg, 0.0)
+    return val, bound
+
+
+# ------------------------------------------------------------------- policy and preference losses
+def policy_loss(log_prob, old_log_prob, advantage, mask=None, ref_log_prob=None, entropy=None, clip_low=0.2,
+                clip_high=0.2, dual_clip=None, kl_coef=0.0, kl_form="k3", entropy_coef=0.0, reduction="token_mean",
+                scale=1.0):
+    """The clipped policy loss with KL and entropy terms and its gradients in fp64.  Returns (values, errors).
+
+    The bound: a token's terms (ratio, KL, gradient) carry at most 16 roundings of fp32 relative to their
+    sizes (exp of a rounded difference: 4 + |d|), sums are in fp64, each output is rounded once."""
+    cur, old, adv = _f64(log_prob), _f64(log_prob if old_log_prob is None else old_log_prob), _f64(advantage)
+    adv = np.broadcast_to(adv if adv.ndim == 2 else adv[:, None], cur.shape)
+    m = np.ones(cur.shape, bool) if mask is None else _f64(mask)
+    cur, old, adv = (np.where(m, v, 0.0) for v in (cur, old, adv))
+    d = cur - old
+    r = np.exp(d)
+    held = np.clip(r, 1.0 - clip_low, 1.0 + clip_high)
+    gain = np.minimum(r * adv, held * adv)
+    free = r * adv <= held * adv
+    if dual_clip is not None:
+        cut = (adv < 0) & (gain < dual_clip * adv)
+        gain, free = np.where(cut, dual_clip * adv, gain), free & ~cut
+    n_row = m.sum(1)
+    n = max(1, int(m.sum()))
+    if reduction == "token_mean":
+        w = np.full(cur.shape, scale / n)
+    elif reduction == "sequence_mean":
+        w = np.broadcast_to((scale / (max(1, int((n_row > 0).sum())) * np.maximum(1, n_row)))[:, None], cur.shape)
+    else:
+        w = np.full(cur.shape, float(scale))
+    w = np.where(m, w, 0.0)
+    slope = np.where(free, -r * adv, 0.0)
+    size = np.abs(slope) * (1 + np.abs(d))
+    kl, kabs, ent, eabs = 0.0, 0.0, 0.0, 0.0
+    if ref_log_prob is not None:
+        q = np.where(m, _f64(ref_log_prob), 0.0) - cur
+        k, dk = {"k1": (-q, np.ones_like(q)), "k2": (0.5 * q * q, -q),
+                 "k3": (np.expm1(q) - q, -np.expm1(q))}[kl_form]
+        kl, kabs = (w * k).sum(), (np.abs(w * k) * (1 + np.abs(q))).sum()
+        slope = slope + kl_coef * dk
+        size = size + np.abs(kl_coef) * np.abs(dk) * (1 + np.abs(q))
+    if entropy is not None:
+        h = np.where(m, _f64(entropy), 0.0)
+        ent, eabs = (w * h).sum(), np.abs(w * h).sum()
+    pol, pabs = -(w * gain).sum(), (np.abs(w * gain) * (1 + np.abs(d))).sum()
+    out = np.array([pol + kl_coef * kl - entropy_coef * ent, pol, kl, ent, ((held != r) & m).sum() / n,
+                    np.where(m, np.expm1(d) - d, 0.0).sum() / n, np.where(m, r, 0.0).max(initial=0.0),
+                    np.where(m, r, 0.0).sum() / n])
+    size_out = np.array([pabs + abs(kl_coef) * kabs + abs(entropy_coef) * eabs, pabs, kabs, eabs, out[4],
+                         out[5] * (1 + np.abs(d).max(initial=0.0)), out[6] * (1 + np.abs(d).max(initial=0.0)),
+                         out[7] * (1 + np.abs(d).max(initial=0.0))])
+    val = {"out": out, "grad": w * slope, "grad_entropy": -w * entropy_coef}
+    bound = {"out": 16 * U32 * size_out, "grad": 16 * U32 * np.abs(w) * size,
+             "grad_entropy": 4 * U32 * np.abs(w * entropy_coef)}
+    return val, bound
+
+
+def preference_loss(chosen, rejected, ref_chosen=None, ref_rejected=None, chosen_mask=None, rejected_mask=None,
+                    beta=0.1, form="sigmoid", label_smoothing=0.0, margin=0.0, average=False):
+    """The preference loss and its gradients in fp64.  Returns (values, errors): everything up to the outputs
+    is in fp64 in the kernel too, so 4 roundings of fp32 cover each output."""
+    def side(lp, ref, mask):
+        lp = _f64(lp)
+        m = np.ones(lp.shape, bool) if mask is None else _f64(mask)
+        gap = np.where(m, lp, 0.0) - (0.0 if ref is None else np.where(m, _f64(ref), 0.0))
+        n = np.maximum(1, m.sum(1)) if average else np.ones(lp.shape[0])
+        return gap.sum(1) / n, m / n[:, None], np.abs(gap).sum(1) / n
+    (c, mc, ac), (r, mr, ar) = side(chosen, ref_chosen, chosen_mask), side(rejected, ref_rejected, rejected_mask)
+    B = max(1, len(c))
+    gap = beta * (c - r)
+    z = gap - margin
+    if form == "sigmoid":
+        loss = (1 - label_smoothing) * np.logaddexp(0, -z) + label_smoothing * np.logaddexp(0, z)
+        dz = label_smoothing - np.exp(-np.logaddexp(0, z))
+    elif form == "hinge":
+        loss, dz = np.maximum(0.0, 1 - z), np.where(z < 1, -1.0, 0.0)
+    else:
+        loss, dz = ((z - 0.5) / beta) ** 2, 2 * (z - 0.5) / beta ** 2
+    k = (beta * dz / B)[:, None]
+    val = {"out": np.array([loss.sum(), (c > r).sum(), gap.sum()]) / B, "reward_chosen": beta * c,
+           "reward_rejected": beta * r, "grad_chosen": k * mc, "grad_rejected": -k * mr}
+    # fp64 sums are off by up to 2^-40 of their terms' sizes, which the losses' slopes carry on.
+    lost = 2.0 ** -40 * beta * (ac + ar)
+    bound = {n: 4 * U32 * np.abs(v) for n, v in val.items()}
+    bound["out"] = bound["out"] + np.array([(np.abs(dz) * lost).sum(), 0.0, lost.sum()]) / B
+    bound["reward_chosen"] = bound["reward_chosen"] + lost
+    bound["reward_rejected"] = bound["reward_rejected"] + lost
+    curve = {"sigmoid": 0.25, "hinge": 0.0, "ipo": 2 / beta ** 2}[form]
+    slip = (beta * curve * lost / B)[:, None]
+    bound["grad_chosen"] = bound["grad_chosen"] + slip * mc
+    bound["grad_rejected"] = bound["grad_rejected"] + slip * mr
+    return val, bound
