@@ -64,63 +64,116 @@ struct Ctl {
 
 __host__ __device__ inline int64_t tiles(int64_t T) { return (T + kTile - 1) / kTile; }
 
-// ------------------------------------------------------------------------- per-element arithmetic
-// a and 1 - a of the sigmoid form, each with a relative error of a few ulp: 1 - a is not formed by
-// subtraction, so gates far from 0 keep the digits of both.
+// --------------------------------------------------------------------------- the lane's channels
+// A lane holds 4 bytes of a row: one fp32 channel (float), or two 16-bit ones (float2, whose products and
+// sums are packed two to an instruction; instruction issue is the next bound after memory).
+__device__ __forceinline__ float vset(float, float a) { return a; }
+__device__ __forceinline__ float2 vset(float2, float a) { return make_float2(a, a); }
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 vmul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 vadd(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 vfma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float vsub(float a, float b) { return a - b; }
+__device__ __forceinline__ float2 vsub(float2 a, float2 b) { return __ffma2_rn(b, make_float2(-1.0f, -1.0f), a); }
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// a = sigmoid(gate) and 1 - a, each with a relative error of a few ulp: with e = exp(-|gate|) they are
+// 1 / (1 + e) and e / (1 + e), and neither is formed by subtraction, so gates far from 0 keep the digits of
+// both.  (Values below 2^-126 are flushed to 0.)
 __device__ __forceinline__ void sigmoid_pair(float gate, float& a, float& na) {
-  const float e = __expf(-fabsf(gate));  // in [0, 1]
-  const float r = __fdividef(1.0f, 1.0f + e), er = e * r;
-  a = gate >= 0.0f ? r : er;
-  na = gate >= 0.0f ? er : r;
-  if (gate != gate) a = na = gate;
+  const float e = ex2(fabsf(gate) * -kLog2e), r = rcp(1.0f + e), er = e * r;
+  const bool pos = gate >= 0.0f;
+  a = pos ? r : er;
+  na = pos ? er : r;
+}
+__device__ __forceinline__ void sigmoid_pair(float2 gate, float2& a, float2& na) {
+  const float2 z = vmul(make_float2(fabsf(gate.x), fabsf(gate.y)), vset(gate, -kLog2e));
+  const float2 e = make_float2(ex2(z.x), ex2(z.y));
+  const float2 d = vadd(e, vset(e, 1.0f));
+  const float2 r = make_float2(rcp(d.x), rcp(d.y)), er = vmul(e, r);
+  const bool p0 = gate.x >= 0.0f, p1 = gate.y >= 0.0f;
+  a = make_float2(p0 ? r.x : er.x, p1 ? r.y : er.y);
+  na = make_float2(p0 ? er.x : r.x, p1 ? er.y : r.y);
 }
 
-template <int kForm>
-__device__ __forceinline__ void coeffs(float gate, float x, float& a, float& v) {
-  if (kForm == kDecay) {
-    a = gate;
-    v = x;
-  } else {
-    float na;
-    sigmoid_pair(gate, a, na);
-    v = na * x;
-  }
-}
-
-// The channels of one lane: 4 bytes of a row.
 template <typename T>
 struct Lane;
 template <>
 struct Lane<float> {
+  using V = float;
   static constexpr int kVec = 1;
-  static __device__ __forceinline__ void unpack(uint32_t u, float (&f)[1]) { f[0] = __uint_as_float(u); }
-  static __device__ __forceinline__ uint32_t pack(const float (&f)[1]) { return __float_as_uint(f[0]); }
+  static constexpr uint32_t kOne = 0x3f800000u, kInf = 0x7f800000u;
+  static __device__ __forceinline__ V unpack(uint32_t u) { return __uint_as_float(u); }
+  static __device__ __forceinline__ uint32_t pack(V f) { return __float_as_uint(f); }
 };
 template <>
 struct Lane<__nv_bfloat16> {
+  using V = float2;
   static constexpr int kVec = 2;
-  static __device__ __forceinline__ void unpack(uint32_t u, float (&f)[2]) {
-    f[0] = __uint_as_float(u << 16);
-    f[1] = __uint_as_float(u & 0xffff0000u);
+  static constexpr uint32_t kOne = 0x3f803f80u, kInf = 0x7f807f80u;
+  static __device__ __forceinline__ V unpack(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
-  static __device__ __forceinline__ uint32_t pack(const float (&f)[2]) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(f[0], f[1]);
+  static __device__ __forceinline__ uint32_t pack(V f) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&p);
   }
 };
 template <>
 struct Lane<__half> {
+  using V = float2;
   static constexpr int kVec = 2;
-  static __device__ __forceinline__ void unpack(uint32_t u, float (&f)[2]) {
-    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&u));
-    f[0] = p.x;
-    f[1] = p.y;
+  static constexpr uint32_t kOne = 0x3c003c00u, kInf = 0x7c007c00u;
+  static __device__ __forceinline__ V unpack(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
   }
-  static __device__ __forceinline__ uint32_t pack(const float (&f)[2]) {
-    const __half2 p = __floats2half2_rn(f[0], f[1]);
+  static __device__ __forceinline__ uint32_t pack(V f) {
+    const __half2 p = __floats2half2_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&p);
   }
 };
+
+// The lane's fp32 values at p (channel c of H) in a row of fp32, 0 past the last channel.
+__device__ __forceinline__ void load_row(const float* p, int c, int H, float& y) { y = c < H ? p[0] : 0.0f; }
+__device__ __forceinline__ void load_row(const float* p, int c, int H, float2& y) {
+  y.x = c < H ? p[0] : 0.0f;
+  y.y = c + 1 < H ? p[1] : 0.0f;
+}
+__device__ __forceinline__ void store_row(float* p, int c, int H, float y) {
+  if (c < H) p[0] = y;
+}
+__device__ __forceinline__ void store_row(float* p, int c, int H, float2 y) {
+  if (c < H) p[0] = y.x;
+  if (c + 1 < H) p[1] = y.y;
+}
+// One row of an output: 4 bytes where rows are aligned to them and hold whole lanes, element by element
+// otherwise.
+template <typename T>
+__device__ __forceinline__ void store_out(T* p, int c, int H, bool wide, typename Lane<T>::V y) {
+  const uint32_t u = Lane<T>::pack(y);
+  if (wide) {
+    if (c < H) *reinterpret_cast<uint32_t*>(p) = u;
+  } else if (sizeof(T) == 4) {
+    if (c < H) *reinterpret_cast<uint32_t*>(p) = u;
+  } else {
+    if (c < H) reinterpret_cast<uint16_t*>(p)[0] = uint16_t(u);
+    if (c + 1 < H) reinterpret_cast<uint16_t*>(p)[1] = uint16_t(u >> 16);
+  }
+}
 
 // ---------------------------------------------------------------------------------- moving rows
 template <int kBytes>
@@ -164,6 +217,17 @@ __device__ __forceinline__ void copy_rows(char* dst, const char* src, int64_t pi
             *reinterpret_cast<const uint16_t*>(src + r * pitch + o);
 }
 
+// Rows of a tile past the last step: filled with `word` (steps that leave the state as it is).
+__device__ __forceinline__ void fill_rows(char* dst, int rows, uint32_t word) {
+  for (int i = rows * (kRowBytes / 4) + int(threadIdx.x); i < kTile * (kRowBytes / 4); i += kThreads)
+    reinterpret_cast<uint32_t*>(dst)[i] = word;
+}
+// What a gate holds in such a step: a = 1 (and the input is 0).
+template <typename T, int kForm>
+__device__ constexpr uint32_t neutral_gate() {
+  return kForm == kDecay ? Lane<T>::kOne : Lane<T>::kInf;
+}
+
 // ------------------------------------------------------------------------------- tiles and records
 struct Grid {
   int64_t T;
@@ -188,75 +252,107 @@ __device__ __forceinline__ Tile tile_of(const Grid& g, unsigned ticket) {
   return t;
 }
 
+// A map y -> x y + b of the lane's channels.
+template <typename V>
+struct __align__(2 * sizeof(V)) Map {
+  V x, b;
+};
+
 // Shared memory beside the tile buffers.
-template <int kVec>
+template <typename V>
 struct Shared {
-  float2 map[kWarps][32 * kVec];         // the warps' maps (scan direction)
-  float2 fwd[kWarps][32 * kVec];         // the warps' forward maps (backward kernel)
-  float2 look[kMaxSpan][32 * kVec];      // records of the tiles before this one
+  Map<V> map[kWarps][32];        // the warps' maps (scan direction)
+  V fwd[kWarps][32];             // the warps' forward offsets (backward kernel; the factor is map.x)
+  Map<V> look[kMaxSpan][32];     // records of the tiles before this one
   unsigned look_cut[kMaxSpan];
-  unsigned cut[kWarps], fwd_cut[kWarps];  // the warp's steps hold a reset: its map does not see what comes in
+  unsigned cut[kWarps];          // the warp's steps hold a reset: its map does not see what comes in
   unsigned ticket[2];
 };
 
-// map applied to y; a map with a cut drops y, whatever it holds.
-__device__ __forceinline__ float apply(float2 m, bool cut, float y) { return cut ? m.y : fmaf(m.x, y, m.y); }
+// The map applied to y; a map with a cut drops y, whatever it holds.
+template <typename V>
+__device__ __forceinline__ V apply(const Map<V>& m, bool cut, V y) {
+  return cut ? m.b : vfma(m.x, y, m.b);
+}
 
+__device__ __forceinline__ void put_record(ulonglong2* r, float x, float b, unsigned tag) {
+  ll_store2<LLScope::kGpu>(r, ll_word(__float_as_uint(x), tag), ll_word(__float_as_uint(b), tag));
+}
 // Publish a record for this lane's channels: tag = epoch * 2 + cut.
-template <int kVec>
-__device__ __forceinline__ void publish(const Grid& g, const Tile& t, int64_t B, int c, const float2 (&m)[kVec],
+__device__ __forceinline__ void publish(const Grid& g, const Tile& t, int64_t B, int c, const Map<float>& m,
+                                        unsigned tag) {
+  if (c < g.H) put_record(g.recs + (int64_t(t.k) * B + t.b) * g.H + c, m.x, m.b, tag);
+}
+__device__ __forceinline__ void publish(const Grid& g, const Tile& t, int64_t B, int c, const Map<float2>& m,
                                         unsigned tag) {
   ulonglong2* r = g.recs + (int64_t(t.k) * B + t.b) * g.H + c;
-#pragma unroll
-  for (int v = 0; v < kVec; ++v)
-    if (c + v < g.H)
-      ll_store2<LLScope::kGpu>(r + v, ll_word(__float_as_uint(m[v].x), tag), ll_word(__float_as_uint(m[v].y), tag));
+  if (c < g.H) put_record(r, m.x.x, m.b.x, tag);
+  if (c + 1 < g.H) put_record(r + 1, m.x.y, m.b.y, tag);
+}
+
+// A record of this epoch: waits (at most kWaitLimitNs) until its writer has published it.
+__device__ __forceinline__ ulonglong2 wait_record(const ulonglong2* r, ulonglong2 x, unsigned epoch) {
+  unsigned long long t0 = 0;
+  for (unsigned spin = 1; unsigned(x.x >> 33) != epoch || unsigned(x.y >> 33) != epoch; ++spin) {
+    if ((spin & 63u) == 0) {
+      if (t0 == 0) {
+        t0 = global_ns();
+      } else if (global_ns() - t0 > kWaitLimitNs) {
+        atomicOr(&g_b200_fault, kFaultWaitTimeout);
+        break;
+      }
+    }
+    x = ll_load2<LLScope::kGpu>(r);
+  }
+  return x;
+}
+__device__ __forceinline__ float low_float(unsigned long long v) { return __uint_as_float(unsigned(v)); }
+
+// The record at r of this lane's channels; cut: its writer's steps held a reset.
+__device__ __forceinline__ void take_record(const ulonglong2* r, int c, int H, unsigned epoch, Map<float>& m,
+                                            unsigned& cut) {
+  m = Map<float>{1.0f, 0.0f};
+  cut = 0;
+  if (c >= H) return;
+  const ulonglong2 x = wait_record(r, ll_load2<LLScope::kGpu>(r), epoch);
+  m = Map<float>{low_float(x.x), low_float(x.y)};
+  cut = unsigned(x.x >> 32) & 1u;
+}
+__device__ __forceinline__ void take_record(const ulonglong2* r, int c, int H, unsigned epoch, Map<float2>& m,
+                                            unsigned& cut) {
+  m = Map<float2>{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
+  cut = 0;
+  if (c >= H) return;
+  const ulonglong2* r1 = c + 1 < H ? r + 1 : r;
+  ulonglong2 x = ll_load2<LLScope::kGpu>(r), y = ll_load2<LLScope::kGpu>(r1);
+  x = wait_record(r, x, epoch);
+  y = wait_record(r1, y, epoch);
+  m = Map<float2>{make_float2(low_float(x.x), low_float(y.x)), make_float2(low_float(x.y), low_float(y.y))};
+  cut = unsigned(x.x >> 32) & 1u;
 }
 
 // What comes into tile t from the tiles before it, for this lane's channels: y on entry is the value
 // before tile 0.  Every thread of the CTA calls it.
-template <int kVec>
+template <typename V>
 __device__ __forceinline__ void incoming(const Grid& g, const Tile& t, int64_t B, int c, unsigned epoch,
-                                         Shared<kVec>& sh, float (&y)[kVec]) {
+                                         Shared<V>& sh, V& y) {
   if (t.k == 0) return;
   const unsigned q = t.k % g.span;                    // tiles of the block before this one
   const unsigned n = q + (t.k >= g.span ? 1u : 0u);   // their maps, and the state at the block's start
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   const unsigned first = t.k - n;
-  unsigned long long t0 = 0;
   for (unsigned i = w; i < n; i += kWarps) {
-    const ulonglong2* r = g.recs + (int64_t(first + i) * B + t.b) * g.H + c;
-    unsigned cut = 0;
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) {
-      if (c + v >= g.H) continue;
-      ulonglong2 x = ll_load2<LLScope::kGpu>(r + v);
-      for (unsigned spin = 1; unsigned(x.x >> 33) != epoch || unsigned(x.y >> 33) != epoch; ++spin) {
-        if ((spin & 63u) == 0) {
-          if (t0 == 0) t0 = global_ns();
-          else if (global_ns() - t0 > kWaitLimitNs) {
-            atomicOr(&g_b200_fault, kFaultWaitTimeout);
-            break;
-          }
-        }
-        x = ll_load2<LLScope::kGpu>(r + v);
-      }
-      sh.look[i][lane * kVec + v] = make_float2(__uint_as_float(unsigned(x.x)), __uint_as_float(unsigned(x.y)));
-      cut |= unsigned(x.x >> 32) & 1u;
-    }
+    unsigned cut;
+    Map<V> m;
+    take_record(g.recs + (int64_t(first + i) * B + t.b) * g.H + c, c, g.H, epoch, m, cut);
+    sh.look[i][lane] = m;
     cut = __any_sync(0xffffffffu, cut);
     if (lane == 0) sh.look_cut[i] = cut;
   }
   __syncthreads();
-  for (unsigned i = 0; i < n; ++i) {
-    const bool cut = sh.look_cut[i] != 0;
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) y[v] = apply(sh.look[i][lane * kVec + v], cut, y[v]);
-  }
+  for (unsigned i = 0; i < n; ++i) y = apply(sh.look[i][lane], sh.look_cut[i] != 0, y);
 }
 
-// Publish this tile's record once the tile's map is known (and, where it ends a block, once what comes in
-// is): called twice by the last warp, before incoming() with ends = false and after it with ends = true.
 __device__ __forceinline__ bool ends_block(const Grid& g, unsigned k) { return k % g.span == g.span - 1; }
 
 // Ends the launch's use of the workspace: the last CTA to leave makes it ready for the next launch.
@@ -306,11 +402,49 @@ struct Forward {
   bool wide;       // h rows take 4-byte stores
 };
 
+// Step 1 of the warp: a and v = u of its steps, and their map.  kAny: some step may be a reset.
+template <typename T, int kForm, bool kAny, typename V>
+__device__ __forceinline__ void forward_map(const char* row, unsigned resets, V (&a)[kSteps], V (&u)[kSteps],
+                                            Map<V>& m) {
+  m = Map<V>{vset(V{}, 1.0f), vset(V{}, 0.0f)};
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const V gt = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + i * kRowBytes));
+    const V xv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
+    if (kForm == kDecay) {
+      a[i] = gt;
+      u[i] = xv;
+    } else {
+      V na;
+      sigmoid_pair(gt, a[i], na);
+      u[i] = vmul(na, xv);
+    }
+    if (kAny && ((resets >> i) & 1u)) m = Map<V>{vset(V{}, 0.0f), vset(V{}, 0.0f)};
+    m.b = vfma(a[i], m.b, u[i]);
+    m.x = vmul(m.x, a[i]);
+  }
+}
+
+// Step 4: the warp's steps from its incoming state y, written to out.  kAny: fewer steps than kSteps, or resets.
+template <typename T, bool kAny, typename V>
+__device__ __forceinline__ void forward_steps(const V (&a)[kSteps], const V (&u)[kSteps], unsigned resets, int n,
+                                              int c, int H, bool wide, T* out, int64_t pitch, V& y) {
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    if (kAny && i >= n) break;
+    if (kAny && ((resets >> i) & 1u)) y = vset(V{}, 0.0f);
+    y = vfma(a[i], y, u[i]);
+    store_out<T>(out, c, H, wide, y);
+    out += pitch;
+  }
+}
+
 template <typename T, int kForm>
 __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p) {
+  using V = typename Lane<T>::V;
   constexpr int kVec = Lane<T>::kVec, kGroup = 32 * kVec;
   extern __shared__ __align__(128) char smem[];
-  __shared__ Shared<kVec> sh;
+  __shared__ Shared<V> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
@@ -327,6 +461,10 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p
                 p.gs.t * int64_t(sizeof(T)), rows, width, p.granule);
       copy_rows(dst + kBufBytes, reinterpret_cast<const char*>(p.x + t.b * p.xs.b + t0 * p.xs.t + c0),
                 p.xs.t * int64_t(sizeof(T)), rows, width, p.granule);
+      if (rows < kTile) {
+        fill_rows(dst, rows, neutral_gate<T, kForm>());
+        fill_rows(dst + kBufBytes, rows, 0u);
+      }
     }
     cp_commit();
   };
@@ -352,31 +490,19 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p
 
     const Tile t = tile_of(p.g, ticket);
     const int64_t t0 = int64_t(t.k) * kTile + w * kSteps;  // this warp's first step
-    const int n = int(p.g.T - t0 < kSteps ? (p.g.T > t0 ? p.g.T - t0 : 0) : kSteps);
+    const int n = int(p.g.T - t0 < kSteps ? p.g.T - t0 : kSteps);  // its steps (0 or less: none)
     const int c = int(t.group) * kGroup + int(lane) * kVec;
     const char* row = smem + buf * 2 * kBufBytes + w * kSteps * kRowBytes + lane * 4;
+    const int64_t state_at = int64_t(t.b) * p.g.H + c;
 
     // 1. The warp's steps as one map per channel; a and v stay in registers for step 4.
-    float a[kSteps][kVec], u[kSteps][kVec];
-    float2 m[kVec];
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) m[v] = make_float2(1.0f, 0.0f);
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      if (i >= n) break;
-      float gt[kVec], xv[kVec];
-      Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + i * kRowBytes), gt);
-      Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes), xv);
-      const bool cut = (resets >> i) & 1u;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) {
-        coeffs<kForm>(gt[v], xv[v], a[i][v], u[i][v]);
-        m[v].y = cut ? u[i][v] : fmaf(a[i][v], m[v].y, u[i][v]);
-        m[v].x *= a[i][v];
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) sh.map[w][lane * kVec + v] = m[v];
+    V a[kSteps], u[kSteps];
+    Map<V> m;
+    if (resets == 0)
+      forward_map<T, kForm, false>(row, 0u, a, u, m);
+    else
+      forward_map<T, kForm, true>(row, resets, a, u, m);
+    sh.map[w][lane] = m;
     if (lane == 0) sh.cut[w] = resets != 0;
     __syncthreads();
 
@@ -384,64 +510,35 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p
     const bool ends = ends_block(p.g, t.k), more = t.k + 1 < p.g.n_tiles;
     bool tile_cut = false;
     if (w == kWarps - 1 && more) {
+      m = sh.map[0][lane];
+      tile_cut = sh.cut[0] != 0;
 #pragma unroll
-      for (int v = 0; v < kVec; ++v) m[v] = make_float2(1.0f, 0.0f);
-      for (int j = 0; j < kWarps; ++j) {
+      for (int j = 1; j < kWarps; ++j) {
         const bool cut = sh.cut[j] != 0;
+        const Map<V> s = sh.map[j][lane];
         tile_cut |= cut;
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-          const float2 s = sh.map[j][lane * kVec + v];
-          m[v] = make_float2(s.x * m[v].x, apply(s, cut, m[v].y));
-        }
+        m = Map<V>{vmul(s.x, m.x), apply(s, cut, m.b)};
       }
-      if (!ends) publish<kVec>(p.g, t, p.B, c, m, epoch * 2u + (tile_cut ? 1u : 0u));
+      if (!ends) publish(p.g, t, p.B, c, m, epoch * 2u + (tile_cut ? 1u : 0u));
     }
 
     // 3. The state that comes in.
-    float y[kVec];
-#pragma unroll
-    for (int v = 0; v < kVec; ++v)
-      y[v] = p.state != nullptr && t.k < p.g.span && c + v < p.g.H ? p.state[int64_t(t.b) * p.g.H + c + v] : 0.0f;
-    incoming<kVec>(p.g, t, p.B, c, epoch, sh, y);
-    if (w == kWarps - 1 && more && ends) {
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) m[v] = make_float2(0.0f, apply(m[v], tile_cut, y[v]));
-      publish<kVec>(p.g, t, p.B, c, m, epoch * 2u + 1u);
-    }
-    if (w == 0 && p.ckpt != nullptr) {
-#pragma unroll
-      for (int v = 0; v < kVec; ++v)
-        if (c + v < p.g.H) p.ckpt[(int64_t(t.b) * p.g.n_tiles + t.k) * p.g.H + c + v] = y[v];
-    }
-    for (unsigned j = 0; j < w; ++j) {
-      const bool cut = sh.cut[j] != 0;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) y[v] = apply(sh.map[j][lane * kVec + v], cut, y[v]);
-    }
+    V y = vset(V{}, 0.0f);
+    if (p.state != nullptr && t.k < p.g.span) load_row(p.state + state_at, c, p.g.H, y);
+    incoming(p.g, t, p.B, c, epoch, sh, y);
+    if (w == kWarps - 1 && more && ends)
+      publish(p.g, t, p.B, c, Map<V>{vset(V{}, 0.0f), apply(m, tile_cut, y)}, epoch * 2u + 1u);
+    if (w == 0 && p.ckpt != nullptr)
+      store_row(p.ckpt + (int64_t(t.b) * p.g.n_tiles + t.k) * p.g.H + c, c, p.g.H, y);
+    for (unsigned j = 0; j < w; ++j) y = apply(sh.map[j][lane], sh.cut[j] != 0, y);
 
     // 4. The steps from there.
     T* out = p.h + t.b * p.hs.b + t0 * p.hs.t + c;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      if (i >= n) break;
-      const bool cut = (resets >> i) & 1u;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) y[v] = cut ? u[i][v] : fmaf(a[i][v], y[v], u[i][v]);
-      if (p.wide) {
-        if (c < p.g.H) *reinterpret_cast<uint32_t*>(out) = Lane<T>::pack(y);
-      } else {
-#pragma unroll
-        for (int v = 0; v < kVec; ++v)
-          if (c + v < p.g.H) out[v] = from_f32<T>(y[v]);
-      }
-      out += p.hs.t;
-    }
-    if (p.final_state != nullptr && n > 0 && t0 + n == p.g.T) {
-#pragma unroll
-      for (int v = 0; v < kVec; ++v)
-        if (c + v < p.g.H) p.final_state[int64_t(t.b) * p.g.H + c + v] = y[v];
-    }
+    if (resets == 0 && n == kSteps)
+      forward_steps<T, false>(a, u, 0u, kSteps, c, p.g.H, p.wide, out, p.hs.t, y);
+    else
+      forward_steps<T, true>(a, u, resets, n, c, p.g.H, p.wide, out, p.hs.t, y);
+    if (p.final_state != nullptr && n > 0 && t0 + n == p.g.T) store_row(p.final_state + state_at, c, p.g.H, y);
     ticket = next;
   }
   leave(p.g, epoch);
@@ -462,23 +559,85 @@ struct Backward {
   bool wide;
 };
 
-// A pair (a, 1 - a) in one word: the smaller of the two, negative when it is 1 - a.  The other is 1 minus it,
-// which keeps its digits since the smaller is at most 1/2.
-__device__ __forceinline__ float pack_pair(float a, float na) { return a <= na ? a : -na; }
-__device__ __forceinline__ void unpack_pair(float s, float& a, float& na) {
-  const float t = 1.0f - fabsf(s);
-  const bool neg = __float_as_int(s) < 0;
-  a = neg ? t : s;
-  na = neg ? -s : t;
+// Step 1 of the warp: a and 1 - a of its steps (decay: a alone), its forward map f and its backward map.  In the
+// order of time the backward map of steps 0 .. i is c -> P_i c + sum_j P_j grad_h[j], P_i the product of a
+// up to step i, so it needs no second pass and its factor is the forward map's.
+template <typename T, int kForm, bool kAny, typename V>
+__device__ __forceinline__ void backward_map(const char* row, unsigned resets, V (&a)[kSteps], V (&na)[kSteps], V& f,
+                                             Map<V>& m) {
+  f = vset(V{}, 0.0f);
+  m = Map<V>{vset(V{}, 1.0f), vset(V{}, 0.0f)};
+  bool cut = false;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const V gt = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + i * kRowBytes));
+    V u = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
+    const V dv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + 2 * kBufBytes + i * kRowBytes));
+    if (kForm == kDecay) {
+      a[i] = gt;
+    } else {
+      sigmoid_pair(gt, a[i], na[i]);
+      u = vmul(na[i], u);
+    }
+    if (kAny && ((resets >> i) & 1u)) {
+      f = vset(V{}, 0.0f);
+      cut = true;  // what lies behind a reset reaches no step before it
+    }
+    f = vfma(a[i], f, u);
+    m.x = vmul(m.x, a[i]);
+    if (!kAny || !cut) m.b = vfma(m.x, dv, m.b);
+  }
+}
+
+// The states before the warp's steps from the state s before its first, turned into what multiplies g in
+// grad_gate: h[t-1], or (h[t-1] - x) a (1 - a).
+template <typename T, int kForm, bool kAny, typename V>
+__device__ __forceinline__ void backward_states(const char* row, unsigned resets, const V (&a)[kSteps],
+                                                const V (&na)[kSteps], V s, V (&d)[kSteps]) {
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const V xv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
+    if (kAny && ((resets >> i) & 1u)) s = vset(V{}, 0.0f);
+    if (kForm == kDecay) {
+      d[i] = s;
+      s = vfma(a[i], s, xv);
+    } else {
+      d[i] = vmul(vsub(s, xv), vmul(a[i], na[i]));
+      s = vfma(a[i], s, vmul(na[i], xv));
+    }
+  }
+}
+
+// The warp's steps backwards from the gradient y that comes in.
+template <typename T, int kForm, bool kAny, typename V>
+__device__ __forceinline__ void backward_steps(const char* row, unsigned resets, int n, const V (&a)[kSteps],
+                                               const V (&na)[kSteps], const V (&d)[kSteps], int c, int H, bool wide,
+                                               T* og, int64_t gpitch, T* ox, int64_t xpitch, V& y) {
+  og += (kSteps - 1) * gpitch;
+  ox += (kSteps - 1) * xpitch;
+#pragma unroll
+  for (int i = kSteps - 1; i >= 0; --i) {
+    if (!kAny || i < n) {
+      const V dv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + 2 * kBufBytes + i * kRowBytes));
+      const V g = vadd(dv, y);
+      store_out<T>(og, c, H, wide, vmul(g, d[i]));
+      store_out<T>(ox, c, H, wide, kForm == kDecay ? g : vmul(na[i], g));
+      y = vmul(a[i], g);
+      if (kAny && ((resets >> i) & 1u)) y = vset(V{}, 0.0f);
+    }
+    og -= gpitch;
+    ox -= xpitch;
+  }
 }
 
 // Tiles run from the last to the first (position k is time tile n_tiles - 1 - k).  The states h[t-1] of a
 // tile are formed again from its checkpoint.
 template <typename T, int kForm>
 __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T> p) {
+  using V = typename Lane<T>::V;
   constexpr int kVec = Lane<T>::kVec, kGroup = 32 * kVec;
   extern __shared__ __align__(128) char smem[];
-  __shared__ Shared<kVec> sh;
+  __shared__ Shared<V> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
@@ -497,6 +656,11 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T>
                 p.xs.t * int64_t(sizeof(T)), rows, width, p.granule);
       copy_rows(dst + 2 * kBufBytes, reinterpret_cast<const char*>(p.dh + t.b * p.ds.b + t0 * p.ds.t + c0),
                 p.ds.t * int64_t(sizeof(T)), rows, width, p.granule);
+      if (rows < kTile) {
+        fill_rows(dst, rows, neutral_gate<T, kForm>());
+        fill_rows(dst + kBufBytes, rows, 0u);
+        fill_rows(dst + 2 * kBufBytes, rows, 0u);
+      }
     }
     cp_commit();
   };
@@ -516,12 +680,11 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T>
     const Tile t = tile_of(p.g, ticket);
     const unsigned kt = p.g.n_tiles - 1 - t.k;  // the time tile
     const int64_t t0 = int64_t(kt) * kTile + w * kSteps;
-    const int n = int(p.g.T - t0 < kSteps ? (p.g.T > t0 ? p.g.T - t0 : 0) : kSteps);
+    const int n = int(p.g.T - t0 < kSteps ? p.g.T - t0 : kSteps);
     const int c = int(t.group) * kGroup + int(lane) * kVec;
-    float s[kVec];  // the state before the tile
-#pragma unroll
-    for (int v = 0; v < kVec; ++v)
-      s[v] = c + v < p.g.H ? p.ckpt[(int64_t(t.b) * p.g.n_tiles + kt) * p.g.H + c + v] : 0.0f;
+    const int64_t state_at = int64_t(t.b) * p.g.H + c;
+    V s;  // the state before the tile
+    load_row(p.ckpt + (int64_t(t.b) * p.g.n_tiles + kt) * p.g.H + c, c, p.g.H, s);
     cp_wait_all();
     const unsigned resets = __ballot_sync(0xffffffffu, reset_byte != 0);
     __syncthreads();
@@ -530,47 +693,15 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T>
     reset_byte = load_reset(next);
     const char* row = smem + buf * 3 * kBufBytes + w * kSteps * kRowBytes + lane * 4;
 
-    // 1. The warp's forward and backward maps.  ap: a (decay: read again instead), or the pair (a, 1 - a).
-    float ap[kSteps][kVec];
-    float2 f[kVec], m[kVec];
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) f[v] = m[v] = make_float2(1.0f, 0.0f);
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      if (i >= n) break;
-      float gt[kVec], xv[kVec];
-      Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + i * kRowBytes), gt);
-      Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes), xv);
-      const bool cut = (resets >> i) & 1u;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) {
-        float a = gt[v], na = 1.0f;
-        if (kForm == kSigmoid) sigmoid_pair(gt[v], a, na);
-        ap[i][v] = kForm == kSigmoid ? pack_pair(a, na) : a;
-        const float u = na * xv[v];
-        f[v].y = cut ? u : fmaf(a, f[v].y, u);
-        f[v].x *= a;
-      }
-    }
-#pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i) {
-      if (i >= n) continue;
-      float dv[kVec];
-      Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + 2 * kBufBytes + i * kRowBytes), dv);
-      const bool cut = (resets >> i) & 1u;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) {
-        float a = ap[i][v], na;
-        if (kForm == kSigmoid) unpack_pair(ap[i][v], a, na);
-        m[v].y = cut ? 0.0f : a * (dv[v] + m[v].y);
-        m[v].x *= a;
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) {
-      sh.map[w][lane * kVec + v] = m[v];
-      sh.fwd[w][lane * kVec + v] = f[v];
-    }
+    // 1. The warp's forward and backward maps.
+    V a[kSteps], na[kSteps], d[kSteps], f;
+    Map<V> m;
+    if (resets == 0)
+      backward_map<T, kForm, false>(row, 0u, a, na, f, m);
+    else
+      backward_map<T, kForm, true>(row, resets, a, na, f, m);
+    sh.map[w][lane] = m;
+    sh.fwd[w][lane] = f;
     if (lane == 0) sh.cut[w] = resets != 0;
     __syncthreads();
 
@@ -578,97 +709,41 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T>
     const bool ends = ends_block(p.g, t.k), more = t.k + 1 < p.g.n_tiles;
     bool tile_cut = false;
     if (w == 0 && more) {
+      m = sh.map[kWarps - 1][lane];
+      tile_cut = sh.cut[kWarps - 1] != 0;
 #pragma unroll
-      for (int v = 0; v < kVec; ++v) m[v] = make_float2(1.0f, 0.0f);
-      for (int j = kWarps - 1; j >= 0; --j) {
+      for (int j = kWarps - 2; j >= 0; --j) {
         const bool cut = sh.cut[j] != 0;
+        const Map<V> q = sh.map[j][lane];
         tile_cut |= cut;
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-          const float2 q = sh.map[j][lane * kVec + v];
-          m[v] = make_float2(q.x * m[v].x, apply(q, cut, m[v].y));
-        }
+        m = Map<V>{vmul(q.x, m.x), apply(q, cut, m.b)};
       }
-      if (!ends) publish<kVec>(p.g, t, p.B, c, m, epoch * 2u + (tile_cut ? 1u : 0u));
+      if (!ends) publish(p.g, t, p.B, c, m, epoch * 2u + (tile_cut ? 1u : 0u));
     }
 
     // The states before each step, from the checkpoint.
-    for (unsigned j = 0; j < w; ++j) {
-      const bool cut = sh.cut[j] != 0;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) s[v] = apply(sh.fwd[j][lane * kVec + v], cut, s[v]);
-    }
-    float prev[kSteps][kVec];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      if (i >= n) break;
-      float xv[kVec];
-      Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes), xv);
-      const bool cut = (resets >> i) & 1u;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) {
-        float a = ap[i][v], na = 1.0f;
-        if (kForm == kSigmoid) unpack_pair(ap[i][v], a, na);
-        prev[i][v] = cut ? 0.0f : s[v];
-        const float u = na * xv[v];
-        s[v] = cut ? u : fmaf(a, s[v], u);
-      }
-    }
+    for (unsigned j = 0; j < w; ++j) s = apply(Map<V>{sh.map[j][lane].x, sh.fwd[j][lane]}, sh.cut[j] != 0, s);
+    if (resets == 0)
+      backward_states<T, kForm, false>(row, 0u, a, na, s, d);
+    else
+      backward_states<T, kForm, true>(row, resets, a, na, s, d);
 
     // 3. The gradient that comes in.
-    float y[kVec];
-#pragma unroll
-    for (int v = 0; v < kVec; ++v)
-      y[v] = p.grad_final != nullptr && t.k < p.g.span && c + v < p.g.H ? p.grad_final[int64_t(t.b) * p.g.H + c + v]
-                                                                          : 0.0f;
-    incoming<kVec>(p.g, t, p.B, c, epoch, sh, y);
-    if (w == 0 && more && ends) {
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) m[v] = make_float2(0.0f, apply(m[v], tile_cut, y[v]));
-      publish<kVec>(p.g, t, p.B, c, m, epoch * 2u + 1u);
-    }
-    for (int j = kWarps - 1; j > int(w); --j) {
-      const bool cut = sh.cut[j] != 0;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) y[v] = apply(sh.map[j][lane * kVec + v], cut, y[v]);
-    }
+    V y = vset(V{}, 0.0f);
+    if (p.grad_final != nullptr && t.k < p.g.span) load_row(p.grad_final + state_at, c, p.g.H, y);
+    incoming(p.g, t, p.B, c, epoch, sh, y);
+    if (w == 0 && more && ends)
+      publish(p.g, t, p.B, c, Map<V>{vset(V{}, 0.0f), apply(m, tile_cut, y)}, epoch * 2u + 1u);
+    for (int j = kWarps - 1; j > int(w); --j) y = apply(sh.map[j][lane], sh.cut[j] != 0, y);
 
     // 4. The steps from there, backwards.
     T* og = p.grad_gate + t.b * p.ggs.b + t0 * p.ggs.t + c;
     T* ox = p.grad_x + t.b * p.gxs.b + t0 * p.gxs.t + c;
-#pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i) {
-      if (i >= n) continue;
-      float xv[kVec], dv[kVec], gg[kVec], gx[kVec];
-      Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes), xv);
-      Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + 2 * kBufBytes + i * kRowBytes), dv);
-      const bool cut = (resets >> i) & 1u;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) {
-        float a = ap[i][v], na = 1.0f;
-        if (kForm == kSigmoid) unpack_pair(ap[i][v], a, na);
-        const float g = dv[v] + y[v];
-        gx[v] = na * g;
-        gg[v] = kForm == kSigmoid ? g * (prev[i][v] - xv[v]) * (a * na) : g * prev[i][v];
-        y[v] = cut ? 0.0f : a * g;
-      }
-      T *pg = og + i * p.ggs.t, *px = ox + i * p.gxs.t;
-      if (p.wide) {
-        if (c < p.g.H) {
-          *reinterpret_cast<uint32_t*>(pg) = Lane<T>::pack(gg);
-          *reinterpret_cast<uint32_t*>(px) = Lane<T>::pack(gx);
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < kVec; ++v)
-          if (c + v < p.g.H) pg[v] = from_f32<T>(gg[v]), px[v] = from_f32<T>(gx[v]);
-      }
-    }
-    if (p.grad_state != nullptr && t0 == 0) {
-#pragma unroll
-      for (int v = 0; v < kVec; ++v)
-        if (c + v < p.g.H) p.grad_state[int64_t(t.b) * p.g.H + c + v] = y[v];
-    }
+    if (resets == 0 && n == kSteps)
+      backward_steps<T, kForm, false>(row, 0u, kSteps, a, na, d, c, p.g.H, p.wide, og, p.ggs.t, ox, p.gxs.t, y);
+    else
+      backward_steps<T, kForm, true>(row, resets, n, a, na, d, c, p.g.H, p.wide, og, p.ggs.t, ox, p.gxs.t, y);
+    if (p.grad_state != nullptr && t0 == 0) store_row(p.grad_state + state_at, c, p.g.H, y);
     ticket = next;
   }
   leave(p.g, epoch);
@@ -719,8 +794,12 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const T* __restrict_
   float s = state[int64_t(slot) * H + c];
   for (int j = b; j < B; ++j) {
     if (j != b && slots[j] != slot) continue;
-    float a, v;
-    coeffs<kForm>(to_f32(gate[j * gsb + c]), to_f32(x[j * xsb + c]), a, v);
+    float a = to_f32(gate[j * gsb + c]), v = to_f32(x[j * xsb + c]);
+    if (kForm == kSigmoid) {
+      float na;
+      sigmoid_pair(a, a, na);
+      v = na * v;
+    }
     s = fmaf(a, s, v);
     h[j * hsb + c] = from_f32<T>(s);
     if (!again) break;
