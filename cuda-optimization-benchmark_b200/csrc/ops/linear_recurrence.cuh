@@ -17,8 +17,8 @@
 // A tile is kTile = 128 steps of one group of channels, 128 bytes wide (64 channels of 16 bits, 32 of
 // 32): each of 8 warps takes 16 steps, each lane 4 bytes of channels, so every load and store of a warp is a
 // full line.  CTAs are persistent and take tiles in time order from a ticket counter: while one tile
-// is worked on, the next one's rows arrive in the other shared-memory buffer (cp.async), so the loads
-// never pause.  A tile is read once:
+// is worked on, the next one's rows arrive in the other shared-memory buffer (one tensor load per input,
+// or cp.async where rows are not on 16 bytes), so the loads never pause.  A tile is read once:
 //   1. each warp composes its 16 steps into one map per channel;
 //   2. the 8 maps meet in shared memory; the tile's map goes out as a record in global memory;
 //   3. the state coming into the tile is formed from the records of the tiles before it;
@@ -38,6 +38,7 @@
 #include "../common/bulk.cuh"
 #include "../common/dtype.cuh"
 #include "../common/ll.cuh"
+#include "../common/tcgen05.cuh"
 
 namespace b200 {
 namespace linrec {
@@ -91,23 +92,29 @@ __device__ __forceinline__ float rcp(float v) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// a = sigmoid(gate) and 1 - a, each with a relative error of a few ulp: with e = exp(-|gate|) they are
+// The gate clamped at -87 from below (NaN kept): exp(87) is still finite in fp32, and sigmoid(-87), about
+// 2^-125.5, is as good as 0.
+constexpr float kLowGate = -87.0f;
+__device__ __forceinline__ float clamp_gate(float g) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(g), "f"(kLowGate));
+  return r;
+}
+
+// a = sigmoid(gate) and 1 - a, each with a relative error of a few ulp: with e = exp(-gate) they are
 // 1 / (1 + e) and e / (1 + e), and neither is formed by subtraction, so gates far from 0 keep the digits of
-// both.  (Values below 2^-126 are flushed to 0.)
+// both.  gate >= kLowGate.
 __device__ __forceinline__ void sigmoid_pair(float gate, float& a, float& na) {
-  const float e = ex2(fabsf(gate) * -kLog2e), r = rcp(1.0f + e), er = e * r;
-  const bool pos = gate >= 0.0f;
-  a = pos ? r : er;
-  na = pos ? er : r;
+  const float e = ex2(gate * -kLog2e);
+  a = rcp(1.0f + e);
+  na = e * a;
 }
 __device__ __forceinline__ void sigmoid_pair(float2 gate, float2& a, float2& na) {
-  const float2 z = vmul(make_float2(fabsf(gate.x), fabsf(gate.y)), vset(gate, -kLog2e));
+  const float2 z = vmul(gate, vset(gate, -kLog2e));
   const float2 e = make_float2(ex2(z.x), ex2(z.y));
   const float2 d = vadd(e, vset(e, 1.0f));
-  const float2 r = make_float2(rcp(d.x), rcp(d.y)), er = vmul(e, r);
-  const bool p0 = gate.x >= 0.0f, p1 = gate.y >= 0.0f;
-  a = make_float2(p0 ? r.x : er.x, p1 ? r.y : er.y);
-  na = make_float2(p0 ? er.x : r.x, p1 ? er.y : r.y);
+  a = make_float2(rcp(d.x), rcp(d.y));
+  na = vmul(e, a);
 }
 
 template <typename T>
@@ -116,17 +123,21 @@ template <>
 struct Lane<float> {
   using V = float;
   static constexpr int kVec = 1;
-  static constexpr uint32_t kOne = 0x3f800000u, kInf = 0x7f800000u;
   static __device__ __forceinline__ V unpack(uint32_t u) { return __uint_as_float(u); }
+  static __device__ __forceinline__ V unpack_gate(uint32_t u) { return clamp_gate(__uint_as_float(u)); }
   static __device__ __forceinline__ uint32_t pack(V f) { return __float_as_uint(f); }
 };
 template <>
 struct Lane<__nv_bfloat16> {
   using V = float2;
   static constexpr int kVec = 2;
-  static constexpr uint32_t kOne = 0x3f803f80u, kInf = 0x7f807f80u;
   static __device__ __forceinline__ V unpack(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+  static __device__ __forceinline__ V unpack_gate(uint32_t u) {
+    const __nv_bfloat162 g = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&u),
+                                         __floats2bfloat162_rn(kLowGate, kLowGate));
+    return unpack(*reinterpret_cast<const uint32_t*>(&g));
   }
   static __device__ __forceinline__ uint32_t pack(V f) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(f.x, f.y);
@@ -137,9 +148,11 @@ template <>
 struct Lane<__half> {
   using V = float2;
   static constexpr int kVec = 2;
-  static constexpr uint32_t kOne = 0x3c003c00u, kInf = 0x7c007c00u;
   static __device__ __forceinline__ V unpack(uint32_t u) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  }
+  static __device__ __forceinline__ V unpack_gate(uint32_t u) {
+    return __half22float2(__hmax2_nan(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(kLowGate, kLowGate)));
   }
   static __device__ __forceinline__ uint32_t pack(V f) {
     const __half2 p = __floats2half2_rn(f.x, f.y);
@@ -165,9 +178,7 @@ __device__ __forceinline__ void store_row(float* p, int c, int H, float2 y) {
 template <typename T>
 __device__ __forceinline__ void store_out(T* p, int c, int H, bool wide, typename Lane<T>::V y) {
   const uint32_t u = Lane<T>::pack(y);
-  if (wide) {
-    if (c < H) *reinterpret_cast<uint32_t*>(p) = u;
-  } else if (sizeof(T) == 4) {
+  if (wide || sizeof(T) == 4) {
     if (c < H) *reinterpret_cast<uint32_t*>(p) = u;
   } else {
     if (c < H) reinterpret_cast<uint16_t*>(p)[0] = uint16_t(u);
@@ -217,17 +228,6 @@ __device__ __forceinline__ void copy_rows(char* dst, const char* src, int64_t pi
             *reinterpret_cast<const uint16_t*>(src + r * pitch + o);
 }
 
-// Rows of a tile past the last step: filled with `word` (steps that leave the state as it is).
-__device__ __forceinline__ void fill_rows(char* dst, int rows, uint32_t word) {
-  for (int i = rows * (kRowBytes / 4) + int(threadIdx.x); i < kTile * (kRowBytes / 4); i += kThreads)
-    reinterpret_cast<uint32_t*>(dst)[i] = word;
-}
-// What a gate holds in such a step: a = 1 (and the input is 0).
-template <typename T, int kForm>
-__device__ constexpr uint32_t neutral_gate() {
-  return kForm == kDecay ? Lane<T>::kOne : Lane<T>::kInf;
-}
-
 // ------------------------------------------------------------------------------- tiles and records
 struct Grid {
   int64_t T;
@@ -238,9 +238,10 @@ struct Grid {
   ulonglong2* recs;  // [n_tiles, B, H]
 };
 
-struct Tile {
-  unsigned k;       // position in the order of the scan
+struct __align__(16) Tile {
+  unsigned k;  // position in the order of the scan
   unsigned b, group;
+  unsigned live;  // 0: the ticket lies past the last tile
 };
 
 __device__ __forceinline__ Tile tile_of(const Grid& g, unsigned ticket) {
@@ -249,6 +250,7 @@ __device__ __forceinline__ Tile tile_of(const Grid& g, unsigned ticket) {
   const unsigned chain = ticket - t.k * g.chains;
   t.b = chain / g.groups;
   t.group = chain - t.b * g.groups;
+  t.live = ticket < g.total;
   return t;
 }
 
@@ -266,7 +268,8 @@ struct Shared {
   Map<V> look[kMaxSpan][32];     // records of the tiles before this one
   unsigned look_cut[kMaxSpan];
   unsigned cut[kWarps];          // the warp's steps hold a reset: its map does not see what comes in
-  unsigned ticket[2];
+  Tile tile;                     // the next tile
+  uint64_t full[2];              // the tile buffers' loads have landed (tensor loads)
 };
 
 // The map applied to y; a map with a cut drops y, whatever it holds.
@@ -337,7 +340,7 @@ template <typename V>
 __device__ __forceinline__ void incoming(const Grid& g, const Tile& t, int64_t B, int c, unsigned epoch,
                                          Shared<V>& sh, V& y) {
   if (t.k == 0) return;
-  const unsigned q = t.k % g.span;                    // tiles of the block before this one
+  const unsigned q = t.k & (g.span - 1);              // tiles of the block before this one
   const unsigned n = q + (t.k >= g.span ? 1u : 0u);   // their maps, and the state at the block's start
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   const unsigned first = t.k - n;
@@ -353,7 +356,7 @@ __device__ __forceinline__ void incoming(const Grid& g, const Tile& t, int64_t B
   for (unsigned i = 0; i < n; ++i) y = apply(sh.look[i][lane], sh.look_cut[i] != 0, y);
 }
 
-__device__ __forceinline__ bool ends_block(const Grid& g, unsigned k) { return k % g.span == g.span - 1; }
+__device__ __forceinline__ bool ends_block(const Grid& g, unsigned k) { return (k & (g.span - 1)) == g.span - 1; }
 
 // Ends the launch's use of the workspace: the last CTA to leave makes it ready for the next launch.
 __device__ __forceinline__ void leave(const Grid& g, unsigned epoch) {
@@ -367,9 +370,13 @@ __device__ __forceinline__ void leave(const Grid& g, unsigned epoch) {
   }
 }
 
-__device__ __forceinline__ unsigned next_ticket(const Grid& g, unsigned last) {
-  return g.ctl != nullptr ? atomicAdd(&g.ctl->ticket, 1u) : last + gridDim.x;
-}
+// Thread 0's supply of tickets: after the first, taken one ahead so that no tile waits for the counter.
+struct Tickets {
+  unsigned ahead;
+  __device__ __forceinline__ unsigned take(const Grid& g, unsigned last) const {
+    return g.ctl != nullptr ? atomicAdd(&g.ctl->ticket, 1u) : last + gridDim.x;
+  }
+};
 
 // The launch's epoch: 31 bits, never 0 (a zero-filled record belongs to no launch).
 __device__ __forceinline__ unsigned launch_epoch(const Grid& g) {
@@ -387,36 +394,66 @@ struct Resets {
   }
 };
 
+// An input of the scan: rows of T at p, and the tensor map over [B, T, H] that loads a tile at once where
+// `tma` (16-byte rows); `swap`: the map's second axis is the batch and its third the time.
+template <typename T>
+struct __align__(64) Input {
+  CUtensorMap map;
+  const T* p;
+  Strides s;
+  int swap;
+};
+
+template <typename T>
+__device__ __forceinline__ void load_tile(const Input<T>& in, char* dst, const Tile& t, int64_t t0, int64_t Tn, int H,
+                                          bool tma, int granule, uint64_t* bar) {
+  constexpr int kGroup = kRowBytes / int(sizeof(T));
+  const int c0 = int(t.group) * kGroup;
+  if (tma) {  // one thread
+    const int a = int(t0), b = int(t.b);
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(smem_addr(dst)),
+        "l"(&in.map), "r"(c0), "r"(in.swap ? b : a), "r"(in.swap ? a : b), "r"(smem_addr(bar))
+        : "memory");
+  } else {
+    const int rows = int(Tn - t0 < kTile ? Tn - t0 : kTile);
+    copy_rows(dst, reinterpret_cast<const char*>(in.p + t.b * in.s.b + t0 * in.s.t + c0), in.s.t * int64_t(sizeof(T)),
+              rows, min(kGroup, H - c0) * int(sizeof(T)), granule);
+  }
+}
+
 // ------------------------------------------------------------------------------------- forward
 template <typename T>
 struct Forward {
+  Input<T> gate, x;
   Grid g;
-  const T *gate, *x;
-  Strides gs, xs, hs;
+  Strides hs;
   const float* state;
   Resets reset;
   int64_t B;
   T* h;
   float *final_state, *ckpt;
   int granule;     // bytes that divide every row's address in gate and x
-  bool wide;       // h rows take 4-byte stores
+  bool tma, wide;  // tiles come by tensor loads; h rows take 4-byte stores
 };
 
-// Step 1 of the warp: a and v = u of its steps, and their map.  kAny: some step may be a reset.
+// Step 1 of the warp: a and v = u of its n steps, and their map.  kAny: fewer steps than kSteps, or resets.
 template <typename T, int kForm, bool kAny, typename V>
-__device__ __forceinline__ void forward_map(const char* row, unsigned resets, V (&a)[kSteps], V (&u)[kSteps],
+__device__ __forceinline__ void forward_map(const char* row, unsigned resets, int n, V (&a)[kSteps], V (&u)[kSteps],
                                             Map<V>& m) {
   m = Map<V>{vset(V{}, 1.0f), vset(V{}, 0.0f)};
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const V gt = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + i * kRowBytes));
+    if (kAny && i >= n) break;
+    const uint32_t gt = *reinterpret_cast<const uint32_t*>(row + i * kRowBytes);
     const V xv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
     if (kForm == kDecay) {
-      a[i] = gt;
+      a[i] = Lane<T>::unpack(gt);
       u[i] = xv;
     } else {
       V na;
-      sigmoid_pair(gt, a[i], na);
+      sigmoid_pair(Lane<T>::unpack_gate(gt), a[i], na);
       u[i] = vmul(na, xv);
     }
     if (kAny && ((resets >> i) & 1u)) m = Map<V>{vset(V{}, 0.0f), vset(V{}, 0.0f)};
@@ -425,7 +462,8 @@ __device__ __forceinline__ void forward_map(const char* row, unsigned resets, V 
   }
 }
 
-// Step 4: the warp's steps from its incoming state y, written to out.  kAny: fewer steps than kSteps, or resets.
+// Step 4: the warp's steps from its incoming state y, written to out.  !kAny: kSteps steps without resets,
+// 4-byte stores.
 template <typename T, bool kAny, typename V>
 __device__ __forceinline__ void forward_steps(const V (&a)[kSteps], const V (&u)[kSteps], unsigned resets, int n,
                                               int c, int H, bool wide, T* out, int64_t pitch, V& y) {
@@ -434,13 +472,13 @@ __device__ __forceinline__ void forward_steps(const V (&a)[kSteps], const V (&u)
     if (kAny && i >= n) break;
     if (kAny && ((resets >> i) & 1u)) y = vset(V{}, 0.0f);
     y = vfma(a[i], y, u[i]);
-    store_out<T>(out, c, H, wide, y);
+    store_out<T>(out, c, H, !kAny || wide, y);
     out += pitch;
   }
 }
 
 template <typename T, int kForm>
-__global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p) {
+__global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_constant__ Forward<T> p) {
   using V = typename Lane<T>::V;
   constexpr int kVec = Lane<T>::kVec, kGroup = 32 * kVec;
   extern __shared__ __align__(128) char smem[];
@@ -449,46 +487,52 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
 
-  const auto prefetch = [&](unsigned ticket, int buf) {
-    if (ticket < p.g.total) {
-      const Tile t = tile_of(p.g, ticket);
+  const auto prefetch = [&](const Tile& t, int buf) {
+    if (t.live && (!p.tma || threadIdx.x == 0)) {
       const int64_t t0 = int64_t(t.k) * kTile;
-      const int rows = int(p.g.T - t0 < kTile ? p.g.T - t0 : kTile);
-      const int c0 = int(t.group) * kGroup;
-      const int width = min(kGroup, p.g.H - c0) * int(sizeof(T));
       char* dst = smem + buf * 2 * kBufBytes;
-      copy_rows(dst, reinterpret_cast<const char*>(p.gate + t.b * p.gs.b + t0 * p.gs.t + c0),
-                p.gs.t * int64_t(sizeof(T)), rows, width, p.granule);
-      copy_rows(dst + kBufBytes, reinterpret_cast<const char*>(p.x + t.b * p.xs.b + t0 * p.xs.t + c0),
-                p.xs.t * int64_t(sizeof(T)), rows, width, p.granule);
-      if (rows < kTile) {
-        fill_rows(dst, rows, neutral_gate<T, kForm>());
-        fill_rows(dst + kBufBytes, rows, 0u);
-      }
+      if (p.tma) mbar_arrive_expect_tx(&sh.full[buf], 2 * kBufBytes);
+      load_tile(p.gate, dst, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
+      load_tile(p.x, dst + kBufBytes, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
     }
-    cp_commit();
+    if (!p.tma) cp_commit();
   };
-  const auto load_reset = [&](unsigned ticket) {
-    if (ticket >= p.g.total) return uint8_t(0);
-    const Tile t = tile_of(p.g, ticket);
-    return p.reset.load(t.b, int64_t(t.k) * kTile + w * kSteps + lane, p.g.T);
+  const auto load_reset = [&](const Tile& t) {
+    return t.live ? p.reset.load(t.b, int64_t(t.k) * kTile + w * kSteps + lane, p.g.T) : uint8_t(0);
   };
 
-  if (threadIdx.x == 0) sh.ticket[0] = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
+  Tickets tickets;
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.full[0], 1);
+    mbar_init(&sh.full[1], 1);
+    fence_barrier_init();
+    const unsigned first = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
+    sh.tile = tile_of(p.g, first);
+    tickets.ahead = first;
+  }
   __syncthreads();
-  unsigned ticket = sh.ticket[0];
-  prefetch(ticket, 0);
-  uint8_t reset_byte = load_reset(ticket);
-  for (int buf = 0; ticket < p.g.total; buf ^= 1) {
-    if (threadIdx.x == 0) sh.ticket[1] = next_ticket(p.g, ticket);
-    cp_wait_all();
+  Tile t = sh.tile;
+  prefetch(t, 0);
+  uint8_t reset_byte = load_reset(t);
+  __syncthreads();  // sh.tile is read
+  for (unsigned it = 0; t.live; ++it) {
+    const unsigned buf = it & 1u;
+    if (p.tma)
+      mbar_wait(&sh.full[buf], (it >> 1) & 1u);
+    else
+      cp_wait_all();
     const unsigned resets = __ballot_sync(0xffffffffu, reset_byte != 0);
-    __syncthreads();  // this tile's rows and the next ticket are here; the other buffer is free
-    const unsigned next = sh.ticket[1];
+    if (threadIdx.x == 0) {
+      // The second ticket waits for the first tile's rows: by then every CTA has its first.
+      if (it == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
+      sh.tile = tile_of(p.g, tickets.ahead);
+    }
+    __syncthreads();  // this tile's rows and the next tile are here; the other buffer is free
+    const Tile next = sh.tile;
     prefetch(next, buf ^ 1);
     reset_byte = load_reset(next);
+    if (threadIdx.x == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
 
-    const Tile t = tile_of(p.g, ticket);
     const int64_t t0 = int64_t(t.k) * kTile + w * kSteps;  // this warp's first step
     const int n = int(p.g.T - t0 < kSteps ? p.g.T - t0 : kSteps);  // its steps (0 or less: none)
     const int c = int(t.group) * kGroup + int(lane) * kVec;
@@ -498,10 +542,11 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p
     // 1. The warp's steps as one map per channel; a and v stay in registers for step 4.
     V a[kSteps], u[kSteps];
     Map<V> m;
-    if (resets == 0)
-      forward_map<T, kForm, false>(row, 0u, a, u, m);
+    const bool plain = resets == 0 && n >= kSteps;
+    if (plain)
+      forward_map<T, kForm, false>(row, 0u, kSteps, a, u, m);
     else
-      forward_map<T, kForm, true>(row, resets, a, u, m);
+      forward_map<T, kForm, true>(row, resets, n, a, u, m);
     sh.map[w][lane] = m;
     if (lane == 0) sh.cut[w] = resets != 0;
     __syncthreads();
@@ -534,12 +579,12 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p
 
     // 4. The steps from there.
     T* out = p.h + t.b * p.hs.b + t0 * p.hs.t + c;
-    if (resets == 0 && n == kSteps)
+    if (plain && p.wide)
       forward_steps<T, false>(a, u, 0u, kSteps, c, p.g.H, p.wide, out, p.hs.t, y);
     else
       forward_steps<T, true>(a, u, resets, n, c, p.g.H, p.wide, out, p.hs.t, y);
     if (p.final_state != nullptr && n > 0 && t0 + n == p.g.T) store_row(p.final_state + state_at, c, p.g.H, y);
-    ticket = next;
+    t = next;
   }
   leave(p.g, epoch);
 }
@@ -547,36 +592,37 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const Forward<T> p
 // ------------------------------------------------------------------------------------ backward
 template <typename T>
 struct Backward {
+  Input<T> gate, x, dh;
   Grid g;
-  const T *gate, *x, *dh;
-  Strides gs, xs, ds, ggs, gxs;
+  Strides ggs, gxs;
   const float *ckpt, *grad_final;
   Resets reset;
   int64_t B;
   T *grad_gate, *grad_x;
   float* grad_state;
   int granule;
-  bool wide;
+  bool tma, wide;
 };
 
 // Step 1 of the warp: a and 1 - a of its steps (decay: a alone), its forward map f and its backward map.  In the
 // order of time the backward map of steps 0 .. i is c -> P_i c + sum_j P_j grad_h[j], P_i the product of a
 // up to step i, so it needs no second pass and its factor is the forward map's.
 template <typename T, int kForm, bool kAny, typename V>
-__device__ __forceinline__ void backward_map(const char* row, unsigned resets, V (&a)[kSteps], V (&na)[kSteps], V& f,
-                                             Map<V>& m) {
+__device__ __forceinline__ void backward_map(const char* row, unsigned resets, int n, V (&a)[kSteps],
+                                             V (&na)[kSteps], V& f, Map<V>& m) {
   f = vset(V{}, 0.0f);
   m = Map<V>{vset(V{}, 1.0f), vset(V{}, 0.0f)};
   bool cut = false;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const V gt = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + i * kRowBytes));
+    if (kAny && i >= n) break;
+    const uint32_t gt = *reinterpret_cast<const uint32_t*>(row + i * kRowBytes);
     V u = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
     const V dv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + 2 * kBufBytes + i * kRowBytes));
     if (kForm == kDecay) {
-      a[i] = gt;
+      a[i] = Lane<T>::unpack(gt);
     } else {
-      sigmoid_pair(gt, a[i], na[i]);
+      sigmoid_pair(Lane<T>::unpack_gate(gt), a[i], na[i]);
       u = vmul(na[i], u);
     }
     if (kAny && ((resets >> i) & 1u)) {
@@ -592,10 +638,11 @@ __device__ __forceinline__ void backward_map(const char* row, unsigned resets, V
 // The states before the warp's steps from the state s before its first, turned into what multiplies g in
 // grad_gate: h[t-1], or (h[t-1] - x) a (1 - a).
 template <typename T, int kForm, bool kAny, typename V>
-__device__ __forceinline__ void backward_states(const char* row, unsigned resets, const V (&a)[kSteps],
+__device__ __forceinline__ void backward_states(const char* row, unsigned resets, int n, const V (&a)[kSteps],
                                                 const V (&na)[kSteps], V s, V (&d)[kSteps]) {
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
+    if (kAny && i >= n) break;
     const V xv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
     if (kAny && ((resets >> i) & 1u)) s = vset(V{}, 0.0f);
     if (kForm == kDecay) {
@@ -620,8 +667,8 @@ __device__ __forceinline__ void backward_steps(const char* row, unsigned resets,
     if (!kAny || i < n) {
       const V dv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + 2 * kBufBytes + i * kRowBytes));
       const V g = vadd(dv, y);
-      store_out<T>(og, c, H, wide, vmul(g, d[i]));
-      store_out<T>(ox, c, H, wide, kForm == kDecay ? g : vmul(na[i], g));
+      store_out<T>(og, c, H, !kAny || wide, vmul(g, d[i]));
+      store_out<T>(ox, c, H, !kAny || wide, kForm == kDecay ? g : vmul(na[i], g));
       y = vmul(a[i], g);
       if (kAny && ((resets >> i) & 1u)) y = vset(V{}, 0.0f);
     }
@@ -633,7 +680,7 @@ __device__ __forceinline__ void backward_steps(const char* row, unsigned resets,
 // Tiles run from the last to the first (position k is time tile n_tiles - 1 - k).  The states h[t-1] of a
 // tile are formed again from its checkpoint.
 template <typename T, int kForm>
-__global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T> p) {
+__global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_constant__ Backward<T> p) {
   using V = typename Lane<T>::V;
   constexpr int kVec = Lane<T>::kVec, kGroup = 32 * kVec;
   extern __shared__ __align__(128) char smem[];
@@ -642,42 +689,38 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T>
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
 
-  const auto prefetch = [&](unsigned ticket, int buf) {
-    if (ticket < p.g.total) {
-      const Tile t = tile_of(p.g, ticket);
+  const auto prefetch = [&](const Tile& t, int buf) {
+    if (t.live && (!p.tma || threadIdx.x == 0)) {
       const int64_t t0 = int64_t(p.g.n_tiles - 1 - t.k) * kTile;
-      const int rows = int(p.g.T - t0 < kTile ? p.g.T - t0 : kTile);
-      const int c0 = int(t.group) * kGroup;
-      const int width = min(kGroup, p.g.H - c0) * int(sizeof(T));
       char* dst = smem + buf * 3 * kBufBytes;
-      copy_rows(dst, reinterpret_cast<const char*>(p.gate + t.b * p.gs.b + t0 * p.gs.t + c0),
-                p.gs.t * int64_t(sizeof(T)), rows, width, p.granule);
-      copy_rows(dst + kBufBytes, reinterpret_cast<const char*>(p.x + t.b * p.xs.b + t0 * p.xs.t + c0),
-                p.xs.t * int64_t(sizeof(T)), rows, width, p.granule);
-      copy_rows(dst + 2 * kBufBytes, reinterpret_cast<const char*>(p.dh + t.b * p.ds.b + t0 * p.ds.t + c0),
-                p.ds.t * int64_t(sizeof(T)), rows, width, p.granule);
-      if (rows < kTile) {
-        fill_rows(dst, rows, neutral_gate<T, kForm>());
-        fill_rows(dst + kBufBytes, rows, 0u);
-        fill_rows(dst + 2 * kBufBytes, rows, 0u);
-      }
+      if (p.tma) mbar_arrive_expect_tx(&sh.full[buf], 3 * kBufBytes);
+      load_tile(p.gate, dst, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
+      load_tile(p.x, dst + kBufBytes, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
+      load_tile(p.dh, dst + 2 * kBufBytes, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
     }
-    cp_commit();
+    if (!p.tma) cp_commit();
   };
-  const auto load_reset = [&](unsigned ticket) {
-    if (ticket >= p.g.total) return uint8_t(0);
-    const Tile t = tile_of(p.g, ticket);
-    return p.reset.load(t.b, int64_t(p.g.n_tiles - 1 - t.k) * kTile + w * kSteps + lane, p.g.T);
+  const auto load_reset = [&](const Tile& t) {
+    return t.live ? p.reset.load(t.b, int64_t(p.g.n_tiles - 1 - t.k) * kTile + w * kSteps + lane, p.g.T)
+                  : uint8_t(0);
   };
 
-  if (threadIdx.x == 0) sh.ticket[0] = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
+  Tickets tickets;
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.full[0], 1);
+    mbar_init(&sh.full[1], 1);
+    fence_barrier_init();
+    const unsigned first = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
+    sh.tile = tile_of(p.g, first);
+    tickets.ahead = first;
+  }
   __syncthreads();
-  unsigned ticket = sh.ticket[0];
-  prefetch(ticket, 0);
-  uint8_t reset_byte = load_reset(ticket);
-  for (int buf = 0; ticket < p.g.total; buf ^= 1) {
-    if (threadIdx.x == 0) sh.ticket[1] = next_ticket(p.g, ticket);
-    const Tile t = tile_of(p.g, ticket);
+  Tile t = sh.tile;
+  prefetch(t, 0);
+  uint8_t reset_byte = load_reset(t);
+  __syncthreads();  // sh.tile is read
+  for (unsigned it = 0; t.live; ++it) {
+    const unsigned buf = it & 1u;
     const unsigned kt = p.g.n_tiles - 1 - t.k;  // the time tile
     const int64_t t0 = int64_t(kt) * kTile + w * kSteps;
     const int n = int(p.g.T - t0 < kSteps ? p.g.T - t0 : kSteps);
@@ -685,21 +728,31 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T>
     const int64_t state_at = int64_t(t.b) * p.g.H + c;
     V s;  // the state before the tile
     load_row(p.ckpt + (int64_t(t.b) * p.g.n_tiles + kt) * p.g.H + c, c, p.g.H, s);
-    cp_wait_all();
+    if (p.tma)
+      mbar_wait(&sh.full[buf], (it >> 1) & 1u);
+    else
+      cp_wait_all();
     const unsigned resets = __ballot_sync(0xffffffffu, reset_byte != 0);
-    __syncthreads();
-    const unsigned next = sh.ticket[1];
+    if (threadIdx.x == 0) {
+      // The second ticket waits for the first tile's rows: by then every CTA has its first.
+      if (it == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
+      sh.tile = tile_of(p.g, tickets.ahead);
+    }
+    __syncthreads();  // this tile's rows and the next tile are here; the other buffer is free
+    const Tile next = sh.tile;
     prefetch(next, buf ^ 1);
     reset_byte = load_reset(next);
+    if (threadIdx.x == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
     const char* row = smem + buf * 3 * kBufBytes + w * kSteps * kRowBytes + lane * 4;
 
     // 1. The warp's forward and backward maps.
     V a[kSteps], na[kSteps], d[kSteps], f;
     Map<V> m;
-    if (resets == 0)
-      backward_map<T, kForm, false>(row, 0u, a, na, f, m);
+    const bool plain = resets == 0 && n >= kSteps;
+    if (plain)
+      backward_map<T, kForm, false>(row, 0u, kSteps, a, na, f, m);
     else
-      backward_map<T, kForm, true>(row, resets, a, na, f, m);
+      backward_map<T, kForm, true>(row, resets, n, a, na, f, m);
     sh.map[w][lane] = m;
     sh.fwd[w][lane] = f;
     if (lane == 0) sh.cut[w] = resets != 0;
@@ -723,10 +776,10 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T>
 
     // The states before each step, from the checkpoint.
     for (unsigned j = 0; j < w; ++j) s = apply(Map<V>{sh.map[j][lane].x, sh.fwd[j][lane]}, sh.cut[j] != 0, s);
-    if (resets == 0)
-      backward_states<T, kForm, false>(row, 0u, a, na, s, d);
+    if (plain)
+      backward_states<T, kForm, false>(row, 0u, kSteps, a, na, s, d);
     else
-      backward_states<T, kForm, true>(row, resets, a, na, s, d);
+      backward_states<T, kForm, true>(row, resets, n, a, na, s, d);
 
     // 3. The gradient that comes in.
     V y = vset(V{}, 0.0f);
@@ -739,12 +792,12 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Backward<T>
     // 4. The steps from there, backwards.
     T* og = p.grad_gate + t.b * p.ggs.b + t0 * p.ggs.t + c;
     T* ox = p.grad_x + t.b * p.gxs.b + t0 * p.gxs.t + c;
-    if (resets == 0 && n == kSteps)
+    if (plain && p.wide)
       backward_steps<T, kForm, false>(row, 0u, kSteps, a, na, d, c, p.g.H, p.wide, og, p.ggs.t, ox, p.gxs.t, y);
     else
       backward_steps<T, kForm, true>(row, resets, n, a, na, d, c, p.g.H, p.wide, og, p.ggs.t, ox, p.gxs.t, y);
     if (p.grad_state != nullptr && t0 == 0) store_row(p.grad_state + state_at, c, p.g.H, y);
-    ticket = next;
+    t = next;
   }
   leave(p.g, epoch);
 }
@@ -797,7 +850,7 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const T* __restrict_
     float a = to_f32(gate[j * gsb + c]), v = to_f32(x[j * xsb + c]);
     if (kForm == kSigmoid) {
       float na;
-      sigmoid_pair(a, a, na);
+      sigmoid_pair(clamp_gate(a), a, na);
       v = na * v;
     }
     s = fmaf(a, s, v);
@@ -858,6 +911,31 @@ inline int plan(Kernel kernel, int smem, int vec, int64_t B, int64_t T, int64_t 
   return kOk;
 }
 
+// The tensor map of an input over [B, T, H], boxes of kTile steps of one channel group.  false: the layout
+// does not take one (rows off 16 bytes, shared rows, strides that are no multiples of one another).
+template <typename T>
+inline bool make_input_map(Input<T>* in, int64_t B, int64_t Tn, int64_t H) {
+  const int64_t size = sizeof(T);
+  int64_t st = in->s.t * size, sb = in->s.b * size;
+  const int64_t row = (H * size + 15) / 16 * 16;
+  in->swap = B > 1 && Tn > 1 && sb < st;
+  if (Tn == 1) st = B == 1 ? row : sb;  // an axis of one step has no stride of its own
+  if (B == 1) sb = st * Tn;
+  const int64_t s1 = in->swap ? sb : st, s2 = in->swap ? st : sb;
+  if (!aligned16(in->p) || s1 <= 0 || s1 % 16 != 0 || s2 % s1 != 0 || s2 >= (int64_t(1) << 40)) return false;
+  const auto fn = tc::encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3] = {cuuint64_t(H), cuuint64_t(in->swap ? B : Tn), cuuint64_t(in->swap ? Tn : B)};
+  const cuuint64_t strides[2] = {cuuint64_t(s1), cuuint64_t(s2)};
+  const cuuint32_t box[3] = {cuuint32_t(kRowBytes / size), cuuint32_t(in->swap ? 1 : kTile),
+                             cuuint32_t(in->swap ? kTile : 1)};
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUtensorMapDataType type = size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  return fn(&in->map, type, 3, const_cast<T*>(in->p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 inline bool strides_ok(const int64_t* s, int n) {
   for (int i = 0; i < n; ++i)
     if (s[i] < 0) return false;
@@ -880,13 +958,14 @@ inline int forward(const void* gate, const void* x, int dtype, int form, const i
     using E = decltype(e);
     return with_form(form, [&](auto f) {
       Forward<E> p;
-      p.gate = static_cast<const E*>(gate), p.x = static_cast<const E*>(x), p.h = static_cast<E*>(h);
-      p.gs = Strides{strides[0], strides[1]}, p.xs = Strides{strides[2], strides[3]};
+      p.gate.p = static_cast<const E*>(gate), p.x.p = static_cast<const E*>(x), p.h = static_cast<E*>(h);
+      p.gate.s = Strides{strides[0], strides[1]}, p.x.s = Strides{strides[2], strides[3]};
       p.hs = Strides{strides[4], strides[5]};
       p.reset = Resets{reset, Strides{strides[6], strides[7]}};
       p.state = state, p.B = B, p.final_state = final_state, p.ckpt = ckpt;
       Granule in, out;
-      in.add(gate, p.gs, sizeof(E)), in.add(x, p.xs, sizeof(E)), out.add(h, p.hs, sizeof(E));
+      in.add(gate, p.gate.s, sizeof(E)), in.add(x, p.x.s, sizeof(E)), out.add(h, p.hs, sizeof(E));
+      p.tma = make_input_map(&p.gate, B, T, H) && make_input_map(&p.x, B, T, H);
       p.granule = in.bytes();
       p.wide = out.bytes() >= 4 && H % Lane<E>::kVec == 0;
       constexpr int kSmem = 4 * kBufBytes;
@@ -917,15 +996,16 @@ inline int backward(const void* gate, const void* x, int dtype, int form, const 
     using E = decltype(e);
     return with_form(form, [&](auto f) {
       Backward<E> p;
-      p.gate = static_cast<const E*>(gate), p.x = static_cast<const E*>(x), p.dh = static_cast<const E*>(grad_h);
+      p.gate.p = static_cast<const E*>(gate), p.x.p = static_cast<const E*>(x), p.dh.p = static_cast<const E*>(grad_h);
       p.grad_gate = static_cast<E*>(grad_gate), p.grad_x = static_cast<E*>(grad_x);
-      p.gs = Strides{strides[0], strides[1]}, p.xs = Strides{strides[2], strides[3]};
-      p.ds = Strides{strides[4], strides[5]}, p.ggs = Strides{strides[6], strides[7]};
+      p.gate.s = Strides{strides[0], strides[1]}, p.x.s = Strides{strides[2], strides[3]};
+      p.dh.s = Strides{strides[4], strides[5]}, p.ggs = Strides{strides[6], strides[7]};
       p.gxs = Strides{strides[8], strides[9]};
       p.reset = Resets{reset, Strides{strides[10], strides[11]}};
       p.ckpt = ckpt, p.grad_final = grad_final, p.B = B, p.grad_state = grad_state;
       Granule in, out;
-      in.add(gate, p.gs, sizeof(E)), in.add(x, p.xs, sizeof(E)), in.add(grad_h, p.ds, sizeof(E));
+      in.add(gate, p.gate.s, sizeof(E)), in.add(x, p.x.s, sizeof(E)), in.add(grad_h, p.dh.s, sizeof(E));
+      p.tma = make_input_map(&p.gate, B, T, H) && make_input_map(&p.x, B, T, H) && make_input_map(&p.dh, B, T, H);
       out.add(grad_gate, p.ggs, sizeof(E)), out.add(grad_x, p.gxs, sizeof(E));
       p.granule = in.bytes();
       p.wide = out.bytes() >= 4 && H % Lane<E>::kVec == 0;

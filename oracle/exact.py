@@ -379,7 +379,10 @@ def linear_recurrence(gate, x, state=None, reset=None, form="decay", grad_h=None
     The bound: a step's result carries the error of the state it starts from, times |a|, and at most 16
     roundings relative to M, the recurrence of the absolute values (a sigmoid: exp 4, its argument's
     scaling 2, sum, reciprocal and product 4; a map's composition 2, the final fma 1, the step's own
-    products 3).  The backward's recurrence is bounded the same way."""
+    products 3).  A sigmoid below 2^-125 may be off by that much (the smallest normal fp32 value is 2^-126, and
+    what lies below it may be flushed to 0), and so may 1 - a.  The backward's recurrence is bounded the
+    same way."""
+    low = 2.0 ** -125 if form == "sigmoid" else 0.0
     gate, x = _f64(gate), _f64(x)
     B, T, H = x.shape
     keep = np.ones((B, T, 1)) if reset is None else 1.0 - _f64(reset).astype(np.float64)[:, :, None]
@@ -399,7 +402,7 @@ def linear_recurrence(gate, x, state=None, reset=None, form="decay", grad_h=None
         eprev[:, t] = err * keep[:, t]
         cur = a[:, t] * prev[:, t] + v[:, t]
         mag = np.abs(a[:, t]) * np.where(live[:, t], mag, 0.0) + np.abs(v[:, t])
-        err = np.abs(a[:, t]) * eprev[:, t] + 16 * U32 * mag
+        err = np.abs(a[:, t]) * eprev[:, t] + 16 * U32 * mag + low * (np.abs(prev[:, t]) + np.abs(x[:, t]))
         h[:, t], eh[:, t] = cur, err
     val = {"h": h, "final": cur.copy()}
     bound = {"h": eh, "final": err.copy()}
@@ -419,12 +422,12 @@ def linear_recurrence(gate, x, state=None, reset=None, form="decay", grad_h=None
         else:
             d, s = prev[:, t] - x[:, t], a[:, t] * na[:, t]
             gg[:, t] = g * d * s
-            egg[:, t] = (err * np.abs(d) + np.abs(g) * (eprev[:, t] + U32 * np.abs(d)) + 24 * U32 * np.abs(g * d)) * s
+            egg[:, t] = (err * np.abs(d) + np.abs(g) * (eprev[:, t] + U32 * np.abs(d)) + 24 * U32 * np.abs(g * d)) * s + low * np.abs(g * d)
         gx[:, t] = na[:, t] * g
-        egx[:, t] = na[:, t] * (err + 16 * U32 * np.abs(g))
+        egx[:, t] = na[:, t] * (err + 16 * U32 * np.abs(g)) + low * np.abs(g)
         acc = a[:, t] * g * keep[:, t]
         mag = np.abs(a[:, t]) * mag * keep[:, t]
-        err = np.abs(a[:, t]) * err * keep[:, t] + 16 * U32 * mag
+        err = np.abs(a[:, t]) * err * keep[:, t] + 16 * U32 * mag + low * np.abs(g)
     val.update(grad_gate=gg, grad_x=gx, grad_state=acc)
     bound.update(grad_gate=egg, grad_x=egx, grad_state=err)
     return val, bound
