@@ -854,6 +854,16 @@ def _token_args(logits, token):
     return logits.device, DTYPE_CODES[logits.dtype], B, T, V, st
 
 
+def _check_over(out, logits):
+    """out is memory of its own, or exactly the logits (contiguous)."""
+    if out.numel() == 0 or (out.data_ptr() == logits.data_ptr() and logits.is_contiguous()):
+        return
+    reach = 1 + sum((n - 1) * s for n, s in zip(logits.shape, logits.stride()))
+    size = logits.element_size()
+    if out.data_ptr() < logits.data_ptr() + reach * size and logits.data_ptr() < out.data_ptr() + out.numel() * size:
+        raise ValueError("out overlaps the logits without being them")
+
+
 def _temperature(temperature):
     temperature = float(temperature)
     if not 0.0 < temperature < float("inf"):
@@ -880,14 +890,15 @@ def token_logprob(logits, token, temperature=1.0, entropy=True):
 
     logits: fp32, bf16 or fp16 [N, V] or [B, T, V] with a contiguous vocabulary axis (views such as
     logits[:, :-1] are taken as they are); token: int64 of the leading shape.  A negative token masks its
-    position (outputs 0); a token >= V gives NaN."""
+    position (outputs 0); a token >= V gives NaN, and so does a position whose logits are all -inf or hold a
+    NaN or +inf."""
     lp, ent, _ = _token_logprob(logits, token, temperature, entropy, False)
     return lp, ent
 
 
 def token_logprob_train(logits, token, temperature=1.0, entropy=True):
     """token_logprob for training: (log_prob, entropy, stats), stats (fp32 [..., 3]) for
-    token_logprob_backward."""
+    token_logprob_backward (with grad_entropy only if `entropy`)."""
     return _token_logprob(logits, token, temperature, entropy, True)
 
 
@@ -910,6 +921,7 @@ def token_logprob_backward(logits, token, stats, grad_log_prob, grad_entropy=Non
             _need(out, "out", logits.dtype, dev)
             if out.shape != logits.shape:
                 raise ValueError("out must have logits' shape")
+            _check_over(out, logits)
         _native.check(_lib().b200_token_logprob_backward_async(
             _ptr(logits), dt, st, _ptr(token), _ptr(stats), _ptr(grad_log_prob), _ptr(grad_entropy), B, T, V,
             temperature, _ptr(out), _stream(dev)), "token_logprob_backward")

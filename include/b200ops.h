@@ -372,10 +372,11 @@ int b200_linear_recurrence_step_async(const void* gate, const void* x, int dtype
  * token masks its position: outputs and gradient 0, its logits not read.  token >= V gives NaN.
  * A -inf logit has probability 0; a position whose logits are all -inf, or that has a NaN or +inf
  * logit, gives NaN.
- * stats (may be NULL) receives fp32 [B, T, 3] (maximum, log-sum, entropy) for the backward:
+ * stats (may be NULL) receives fp32 [B, T, 3] (maximum, log-sum, entropy; NaN for the last when
+ * entropy is NULL) for the backward:
  *   grad_logits = (grad_log_prob ([i = token] - p_i) - grad_entropy p_i (log p_i + entropy)) / temperature
  * with grad_log_prob fp32 [B, T], grad_entropy the same or NULL, grad_logits contiguous [B, T, V] of
- * `dtype`, which may be the logits' own memory when these are contiguous.
+ * `dtype`, which may be the logits' own memory when these are contiguous, and else does not overlap it.
  * ------------------------------------------------------------------------------------------- */
 int b200_token_logprob_async(const void* logits, int dtype, const int64_t* strides, const int64_t* token, int32_t B,
                              int32_t T, int32_t V, double temperature, float* log_prob, float* entropy, float* stats,

@@ -270,6 +270,9 @@ def test_empty_and_refusals(ops):
                 lambda: ops.token_logprob_backward(x, k, stats[..., :2], g),
                 lambda: ops.token_logprob_backward(x, k, stats, g.half()),
                 lambda: ops.token_logprob_backward(x, k, stats, g[:1]),
-                lambda: ops.token_logprob_backward(x, k, stats, g, out=x[:1])):
+                lambda: ops.token_logprob_backward(x, k, stats, g, out=x[:1]),
+                lambda: ops.token_logprob_backward(x.flatten()[:25].view(5, 5), k[:1, 0].expand(5), stats[0, 0].expand(5, 3)
+                                                   .contiguous(), g[0, 0].expand(5).contiguous(),
+                                                   out=x.flatten()[1:26].view(5, 5))):
         with pytest.raises((ValueError, TypeError)):
             bad()
