@@ -16,7 +16,9 @@
 // unrounded pair of floats (s, e) against log(1 + clip_high) and log(1 - clip_low) as pairs.
 #pragma once
 
-#include "../common/dtype.cuh"
+#include <math.h>
+
+#include "../common/vec.cuh"
 #include "../common/workspace.cuh"
 
 namespace b200 {
@@ -47,11 +49,15 @@ __device__ __forceinline__ void two_diff(float a, float b, float& s, float& e) {
 __device__ __forceinline__ bool above(float s, float e, Pair p) { return s > p.hi || (s == p.hi && e > p.lo); }
 __device__ __forceinline__ bool below(float s, float e, Pair p) { return s < p.hi || (s == p.hi && e < p.lo); }
 
-// exp(q) - 1 - q without the cancellation near 0: its Taylor series up to q^8 / 8! for |q| < 1/4
-// (the next term is below 2^-24 of the value), the plain difference beyond.
+// exp(q) - 1 - q without the cancellation near 0: its Taylor series up to q^12 / 12! for |q| <= 1 (the next
+// term is below 2^-31 of the value), the difference beyond, where it costs at most some bits of expm1's.
 __device__ __forceinline__ float exp_minus_1_minus(float q) {
-  if (fabsf(q) >= 0.25f) return expm1f(q) - q;
-  float p = 1.0f / 40320.0f;
+  if (fabsf(q) > 1.0f) return expm1f(q) - q;
+  float p = 1.0f / 479001600.0f;
+  p = fmaf(p, q, 1.0f / 39916800.0f);
+  p = fmaf(p, q, 1.0f / 3628800.0f);
+  p = fmaf(p, q, 1.0f / 362880.0f);
+  p = fmaf(p, q, 1.0f / 40320.0f);
   p = fmaf(p, q, 1.0f / 5040.0f);
   p = fmaf(p, q, 1.0f / 720.0f);
   p = fmaf(p, q, 1.0f / 120.0f);
@@ -61,175 +67,356 @@ __device__ __forceinline__ float exp_minus_1_minus(float q) {
   return q * q * p;
 }
 
+// i / d for i < 2^31 by a multiplication (d >= 1).
+struct FastDiv {
+  unsigned d, mul, shift;
+  __device__ __forceinline__ unsigned div(unsigned i) const { return d == 1u ? i : __umulhi(i, mul) >> shift; }
+};
+inline FastDiv fast_div(unsigned d) {
+  unsigned l = 0;
+  while ((uint64_t(1) << l) < d) ++l;  // 2^(l-1) < d <= 2^l
+  return FastDiv{d, unsigned(((uint64_t(1) << (31 + l)) + d - 1) / d), l > 0 ? l - 1 : 0u};
+}
+
 struct Params {
   const float *cur, *old, *adv, *ref, *ent;
   const uint8_t* mask;
-  int64_t cur_s, old_s, adv_s, adv_e, ref_s, ent_s, mask_s;  // row strides; adv_e: 1, or 0 for one per row
+  int64_t cur_s, old_s, adv_s, ref_s, ent_s, mask_s;  // row strides
   int B, T;
+  unsigned n;      // B * T
+  FastDiv by_T;
+  bool dense;      // every stream's row stride is T: a token has one offset in all of them
+  bool adv_rows;   // one advantage per row
+  bool need_row;   // a token's row is needed
   Pair log_high, log_low, log_dual;
   float high, low, dual;  // 1 + clip_high, 1 - clip_low, c (0: off)
-  float kl_coef, ent_coef;
+  float kl_coef;
   int kl_form, reduction;
   double scale, kl_coef_d, ent_coef_d;
   float *grad, *grad_ent, *out;
 };
 
-struct Token {
-  float pg, kl, d_cur, ratio, diff;
-  bool outside;
+// Weighted sums of the policy, kl and entropy terms; over the masked tokens the sums of exp(d) - 1 - d and of
+// r, the largest r, and the counts of tokens and of those outside the clip range.
+struct Sums {
+  double pg, kl, ent, diff, ratio;
+  float max_ratio;
+  unsigned outside, tokens;
 };
 
-__device__ __forceinline__ float kl_term(int form, float q, float& dkl) {
-  if (form == kK1) {
-    dkl = 1.0f;
-    return -q;
-  }
-  if (form == kK2) {
-    dkl = -q;
-    return 0.5f * q * q;
-  }
-  dkl = -expm1f(q);
-  return exp_minus_1_minus(q);
+// The workspace's control words: zero before the first call, and again after each.
+struct Ctl {
+  unsigned done, rows;
+  unsigned long long tokens;
+};
+
+__device__ __forceinline__ float token_weight(const Params& p, unsigned long long tokens, unsigned rows, int row_tokens) {
+  if (p.reduction == kTokenMean) return float(p.scale / double(tokens > 0 ? tokens : 1ull));
+  if (p.reduction == kSequenceMean)
+    return float(p.scale / (double(rows > 0 ? rows : 1u) * double(row_tokens > 0 ? row_tokens : 1)));
+  return float(p.scale);
 }
 
-__device__ __forceinline__ Token token_loss(const Params& p, float cur, float old, float adv, float ref) {
-  Token k;
-  float s, e;
-  two_diff(cur, old, s, e);
-  const bool hi = above(s, e, p.log_high), lo = below(s, e, p.log_low);
-  k.ratio = expf(s);
-  k.diff = exp_minus_1_minus(s);
-  k.outside = hi || lo;
-  const bool dual = p.dual > 0.0f && adv < 0.0f && above(s, e, p.log_dual);
-  const bool clipped = (adv > 0.0f && hi) || (adv < 0.0f && lo) || dual || adv == 0.0f;
-  const float held = dual ? p.dual : hi ? p.high : lo ? p.low : k.ratio;
-  k.pg = adv == 0.0f ? 0.0f : clipped ? -held * adv : -k.ratio * adv;
-  k.d_cur = clipped ? 0.0f : -k.ratio * adv;
-  k.kl = 0.0f;
-  if (p.ref != nullptr) {
-    float dkl;
-    k.kl = kl_term(p.kl_form, __fsub_rn(ref, cur), dkl);
-    k.d_cur = fmaf(p.kl_coef, dkl, k.d_cur);
+// One token as it is read.
+struct Raw {
+  float cur, old, adv, ref, ent;
+  unsigned row;
+  bool on;
+};
+
+__device__ __forceinline__ Raw load_token(const Params& p, unsigned i) {
+  Raw r = {};
+  if (i >= p.n) return r;
+  unsigned t = i;
+  if (p.need_row) {
+    r.row = p.by_T.div(i);
+    t = i - r.row * unsigned(p.T);
+  }
+  const int64_t b = r.row;
+  const auto at = [&](int64_t stride) { return p.dense ? int64_t(i) : b * stride + t; };
+  r.on = p.mask == nullptr || p.mask[at(p.mask_s)] != 0;
+  if (r.on) {
+    r.cur = p.cur[at(p.cur_s)];
+    r.old = p.old[at(p.old_s)];
+    r.adv = p.adv_rows ? p.adv[b * p.adv_s] : p.adv[at(p.adv_s)];
+    if (p.ref != nullptr) r.ref = p.ref[at(p.ref_s)];
+    if (p.ent != nullptr) r.ent = p.ent[at(p.ent_s)];
+  }
+  return r;
+}
+
+// What a token adds (policy, kl and entropy terms weighted with w), and its gradient, which is written.
+struct Terms {
+  float pg, kl, ent, diff, ratio;
+};
+
+__device__ __forceinline__ Terms take_token(const Params& p, unsigned i, const Raw& r, float w, float w_ent, Sums& a) {
+  Terms k = {};
+  float g = 0.0f;
+  if (r.on) {
+    const float s = __fsub_rn(r.cur, r.old);
+    bool hi = s > p.log_high.hi, lo = s < p.log_low.hi;
+    bool dual = p.dual > 0.0f && r.adv < 0.0f && s > p.log_dual.hi;
+    if (s == p.log_high.hi || s == p.log_low.hi || s == p.log_dual.hi) {  // the rounding decides: look at it
+      float e;
+      two_diff(r.cur, r.old, k.diff, e);
+      hi = above(s, e, p.log_high);
+      lo = below(s, e, p.log_low);
+      dual = p.dual > 0.0f && r.adv < 0.0f && above(s, e, p.log_dual);
+    }
+    k.ratio = exp2_approx(s * 1.4426950408889634f);
+    k.diff = exp_minus_1_minus(s);
+    const bool clipped = (r.adv > 0.0f && hi) || (r.adv < 0.0f && lo) || dual || r.adv == 0.0f;
+    const float held = dual ? p.dual : hi ? p.high : lo ? p.low : k.ratio;
+    const float pg = r.adv == 0.0f ? 0.0f : (clipped ? held : k.ratio) * -r.adv;
+    g = clipped ? 0.0f : pg;
+    if (p.ref != nullptr) {
+      const float q = __fsub_rn(r.ref, r.cur);
+      float dkl;
+      if (p.kl_form == kK1) {
+        k.kl = -q, dkl = 1.0f;
+      } else if (p.kl_form == kK2) {
+        k.kl = 0.5f * q * q, dkl = -q;
+      } else {
+        k.kl = exp_minus_1_minus(q), dkl = -(q + k.kl);  // 1 - exp(q)
+      }
+      g = fmaf(p.kl_coef, dkl, g);
+      k.kl *= w;
+    }
+    k.pg = pg * w;
+    k.ent = r.ent * w;
+    g *= w;
+    a.max_ratio = fmaxf(a.max_ratio, k.ratio);
+    a.outside += hi || lo;
+    a.tokens += 1u;
+  }
+  if (i < p.n) {
+    if (p.grad) p.grad[i] = g;
+    if (p.grad_ent) p.grad_ent[i] = r.on ? w_ent : 0.0f;
   }
   return k;
 }
 
-// Sums over tokens: weighted policy, kl and entropy terms; counts; diagnostics.
-struct Sums {
-  double pg, kl, ent, diff, ratio, outside;
-  float max_ratio;
-};
+// kPer tokens of one lane: their terms are added in fp32 in a tree and then to the running sums in fp64.
+constexpr int kPer = 4;
 
-struct Norm {
-  double tokens, rows;
-};
-
-__device__ __forceinline__ double weight(const Params& p, double tokens, double rows, int row_count) {
-  if (p.reduction == kTokenMean) return p.scale / (tokens > 0 ? tokens : 1.0);
-  if (p.reduction == kSequenceMean) return p.scale / ((rows > 0 ? rows : 1.0) * double(row_count > 0 ? row_count : 1));
-  return p.scale;
+__device__ __forceinline__ void add_terms(Sums& a, const Terms (&k)[kPer]) {
+  a.pg += double((k[0].pg + k[1].pg) + (k[2].pg + k[3].pg));
+  a.kl += double((k[0].kl + k[1].kl) + (k[2].kl + k[3].kl));
+  a.ent += double((k[0].ent + k[1].ent) + (k[2].ent + k[3].ent));
+  a.diff += double((k[0].diff + k[1].diff) + (k[2].diff + k[3].diff));
+  a.ratio += double((k[0].ratio + k[1].ratio) + (k[2].ratio + k[3].ratio));
 }
 
-__global__ void __launch_bounds__(kThreads) count_kernel(Params p, int* __restrict__ counts) {
-  pdl_begin();
-  const int b = blockIdx.x;
-  unsigned n = 0;
-  for (int t = threadIdx.x; t < p.T; t += kThreads) n += p.mask == nullptr || p.mask[b * p.mask_s + t] != 0;
-  __shared__ unsigned part[kThreads / 32];
-  n = warp_sum_u32(n);
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = n;
+// The warp's sums, in a fixed order; lane 0 has them all.
+__device__ __forceinline__ void sum_warp(Sums& a) {
+  a.pg = warp_sum(a.pg);
+  a.kl = warp_sum(a.kl);
+  a.ent = warp_sum(a.ent);
+  a.diff = warp_sum(a.diff);
+  a.ratio = warp_sum(a.ratio);
+  a.max_ratio = warp_max(a.max_ratio);
+  a.outside = warp_sum_u32(a.outside);
+  a.tokens = warp_sum_u32(a.tokens);
+}
+template <int kW>
+__device__ __forceinline__ void sum_block(Sums& a) {
+  __shared__ Sums part[kW];
+  const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
+  sum_warp(a);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    unsigned s = 0;
-    for (int i = 0; i < kThreads / 32; ++i) s += part[i];
-    counts[b] = int(s);
-  }
-}
-
-__global__ void norm_kernel(Params p, const int* __restrict__ counts, Norm* norm) {
-  pdl_begin();
-  double tokens = 0.0, rows = 0.0;
-  for (int b = threadIdx.x; b < p.B; b += 32) {
-    tokens += counts[b];
-    rows += counts[b] > 0;
-  }
-  tokens = warp_sum(tokens);
-  rows = warp_sum(rows);
-  if (threadIdx.x == 0) *norm = Norm{tokens, rows};
-}
-
-__global__ void __launch_bounds__(kThreads) token_kernel(Params p, const int* __restrict__ counts,
-                                                         const Norm* __restrict__ norm, Sums* __restrict__ sums) {
-  pdl_begin();
-  const int64_t b = blockIdx.x;
-  const double w = weight(p, norm->tokens, norm->rows, counts[b]);
-  const float wf = float(w);
-  Sums a = {};
-  for (int64_t t = threadIdx.x; t < p.T; t += kThreads) {
-    const bool m = p.mask == nullptr || p.mask[b * p.mask_s + t] != 0;
-    float g = 0.0f, ge = 0.0f;
-    if (m) {
-      const float cur = p.cur[b * p.cur_s + t];
-      const Token k = token_loss(p, cur, p.old[b * p.old_s + t], p.adv[b * p.adv_s + t * p.adv_e],
-                                 p.ref ? p.ref[b * p.ref_s + t] : 0.0f);
-      a.pg += k.pg;
-      a.kl += k.kl;
-      if (p.ent) a.ent += p.ent[b * p.ent_s + t];
-      a.diff += k.diff;
-      a.ratio += k.ratio;
-      a.outside += k.outside;
-      a.max_ratio = fmaxf(a.max_ratio, k.ratio);
-      g = k.d_cur * wf;
-      ge = float(-w * p.ent_coef_d);
-    }
-    if (p.grad) p.grad[b * p.T + t] = g;
-    if (p.grad_ent) p.grad_ent[b * p.T + t] = ge;
-  }
-  __shared__ Sums part[kThreads];
-  part[threadIdx.x] = a;
+  if (lane == 0) part[w] = a;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kThreads; ++i) {
-      a.pg += part[i].pg;
-      a.kl += part[i].kl;
-      a.ent += part[i].ent;
-      a.diff += part[i].diff;
-      a.ratio += part[i].ratio;
-      a.outside += part[i].outside;
-      a.max_ratio = fmaxf(a.max_ratio, part[i].max_ratio);
-    }
-    a.pg *= w;
-    a.kl *= w;
-    a.ent *= w;
-    sums[b] = a;
+  if (w == 0) {
+    a = lane < kW ? part[lane] : Sums{};
+    sum_warp(a);
   }
 }
 
-__global__ void finish_kernel(Params p, const Norm* __restrict__ norm, const Sums* __restrict__ sums) {
-  pdl_begin();
-  Sums a = {};
-  for (int b = 0; b < p.B; ++b) {
-    a.pg += sums[b].pg;
-    a.kl += sums[b].kl;
-    a.ent += sums[b].ent;
-    a.diff += sums[b].diff;
-    a.ratio += sums[b].ratio;
-    a.outside += sums[b].outside;
-    a.max_ratio = fmaxf(a.max_ratio, sums[b].max_ratio);
-  }
-  const double n = norm->tokens > 0 ? norm->tokens : 1.0;
+// tokens: fp64 holds the counts' sum of any size.
+__device__ __forceinline__ void write_outputs(const Params& p, const Sums& a, double tokens, double outside) {
+  const double n = tokens > 0 ? tokens : 1.0;
   p.out[0] = float(a.pg + p.kl_coef_d * a.kl - p.ent_coef_d * a.ent);
   p.out[1] = float(a.pg);
   p.out[2] = float(a.kl);
   p.out[3] = float(a.ent);
-  p.out[4] = float(a.outside / n);
+  p.out[4] = float(outside / n);
   p.out[5] = float(a.diff / n);
   p.out[6] = a.max_ratio;
   p.out[7] = float(a.ratio / n);
 }
 
-inline int64_t workspace_bytes(int32_t B, int32_t) {
-  return int64_t(256 + align256(size_t(B) * sizeof(int)) + align256(size_t(B) * sizeof(Sums)));
+// --------------------------------------------------------------------------- few tokens: one CTA
+constexpr int kSmallThreads = 1024;
+constexpr unsigned kSmallTokens = kPer * kSmallThreads;
+constexpr int kSmallRows = 2048;
+
+__global__ void __launch_bounds__(kSmallThreads) small_kernel(const Params p) {
+  __shared__ int row_tokens[kSmallRows];
+  __shared__ unsigned total, rows;
+  const bool per_row = p.reduction == kSequenceMean;
+  if (per_row)
+    for (int b = threadIdx.x; b < p.B; b += kSmallThreads) row_tokens[b] = 0;
+  if (threadIdx.x == 0) total = rows = 0u;
+  pdl_begin();
+  __syncthreads();
+  Raw raw[kPer];
+  unsigned on = 0;
+  const unsigned base = threadIdx.x / 32 * (32 * kPer) + threadIdx.x % 32;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    raw[j] = load_token(p, base + j * 32);
+    on += raw[j].on;
+    if (per_row && raw[j].on) atomicAdd(&row_tokens[raw[j].row], 1);
+  }
+  on = warp_sum_u32(on);
+  if (threadIdx.x % 32 == 0 && on > 0) atomicAdd(&total, on);
+  __syncthreads();
+  if (per_row) {
+    for (int b = threadIdx.x; b < p.B; b += kSmallThreads)
+      if (row_tokens[b] > 0) atomicAdd(&rows, 1u);
+    __syncthreads();
+  }
+  Sums a = {};
+  float w = per_row ? 0.0f : token_weight(p, total, rows, 0);
+  Terms k[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (per_row) w = token_weight(p, total, rows, row_tokens[raw[j].row]);
+    k[j] = take_token(p, base + j * 32, raw[j], w, float(-double(w) * p.ent_coef_d), a);
+  }
+  add_terms(a, k);
+  sum_block<kSmallThreads / 32>(a);
+  if (threadIdx.x == 0) write_outputs(p, a, double(a.tokens), double(a.outside));
+}
+
+// ------------------------------------------------------------------- many tokens: counts, then terms
+// Counts of the masked tokens, in all (token mean) or per row (sequence mean): rows cut into stretches, a warp
+// each.  Whole-number atomics, so the order does not matter.
+constexpr int kStretch = 4096;
+
+__global__ void __launch_bounds__(kThreads) count_kernel(const Params p, unsigned stretches, Ctl* ctl, int* counts) {
+  pdl_begin();
+  const unsigned lane = threadIdx.x % 32;
+  const uint64_t warps = uint64_t(gridDim.x) * (kThreads / 32);
+  unsigned long long tokens = 0;
+  unsigned rows = 0;
+  for (uint64_t u = uint64_t(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32; u < uint64_t(p.B) * stretches; u += warps) {
+    const int64_t b = int64_t(u / stretches);
+    const int t0 = int(u - uint64_t(b) * stretches) * kStretch;
+    const int len = min(kStretch, p.T - t0);
+    const uint8_t* m = p.mask + b * p.mask_s + t0;
+    const int head = min(len, int((16 - (reinterpret_cast<uintptr_t>(m) & 15u)) & 15u));
+    const int vecs = (len - head) / 16, tail = head + vecs * 16;
+    unsigned c = 0;
+    if (int(lane) < head) c += m[lane] != 0;
+    if (tail + int(lane) < len) c += m[tail + lane] != 0;
+    const uint4* v = reinterpret_cast<const uint4*>(m + head);
+#pragma unroll 4
+    for (int i = lane; i < vecs; i += 32) {
+      const uint4 x = __ldg(v + i);
+      c += __popc(__vminu4(x.x, 0x01010101u)) + __popc(__vminu4(x.y, 0x01010101u)) +
+           __popc(__vminu4(x.z, 0x01010101u)) + __popc(__vminu4(x.w, 0x01010101u));
+    }
+    c = warp_sum_u32(c);
+    if (lane == 0 && c > 0) {
+      if (p.reduction == kSequenceMean)
+        rows += atomicAdd(&counts[b], int(c)) == 0;  // the add that finds an empty row counts it
+      tokens += c;
+    }
+  }
+  __shared__ unsigned long long s_tokens;
+  __shared__ unsigned s_rows;
+  if (threadIdx.x == 0) s_tokens = 0ull, s_rows = 0u;
+  __syncthreads();
+  if (lane == 0 && tokens > 0) {
+    atomicAdd(&s_tokens, tokens);
+    atomicAdd(&s_rows, rows);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && s_tokens > 0) {
+    atomicAdd(&ctl->tokens, s_tokens);
+    if (s_rows > 0) atomicAdd(&ctl->rows, s_rows);
+  }
+}
+
+// Bytes of all streams' L2 prefetch, at most: lines prefetched beyond it would be evicted before their use.
+constexpr int64_t kPrefetchBytes = 48 << 20;
+
+// A CTA takes stretches of kThreads * kPer tokens, grid-stride.  counted: count_kernel ran before; while it does, this kernel brings
+// its first stretches into L2 (their own reads wait for it).
+__global__ void __launch_bounds__(kThreads) token_kernel(const Params p, bool counted, unsigned prefetch, Ctl* ctl,
+                                                         int* counts, Sums* sums) {
+  constexpr unsigned kUnit = kThreads * kPer;
+  const unsigned units = (p.n + kUnit - 1) / kUnit;
+  if (counted && p.dense) {
+    const float* streams[5] = {p.cur, p.old, p.adv_rows ? nullptr : p.adv, p.ref, p.ent};
+    for (unsigned u = blockIdx.x, k = 0; u < units && k < prefetch; u += gridDim.x, ++k) {
+      const unsigned at = u * kUnit + threadIdx.x * 32;  // a 128-byte line per thread
+      if (threadIdx.x < kUnit / 32 && at < p.n)
+#pragma unroll
+        for (int s = 0; s < 5; ++s)
+          if (streams[s] != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(streams[s] + at));
+    }
+  }
+  pdl_begin();
+  const bool per_row = p.reduction == kSequenceMean;
+  const unsigned rows = counted ? ld_cg_u32(&ctl->rows) : unsigned(p.B);
+  const unsigned long long tokens =
+      counted ? *reinterpret_cast<volatile unsigned long long*>(&ctl->tokens) : (unsigned long long)(p.n);
+  float w = token_weight(p, tokens, rows, p.T);
+  float w_ent = float(-double(w) * p.ent_coef_d);
+  Sums a = {};
+  for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
+    const unsigned base = u * kUnit + threadIdx.x / 32 * (32 * kPer) + threadIdx.x % 32;
+    Raw raw[kPer];
+    Terms k[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) raw[j] = load_token(p, base + j * 32);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (per_row && counted) {
+        w = token_weight(p, tokens, rows, raw[j].on ? counts[raw[j].row] : 1);
+        w_ent = float(-double(w) * p.ent_coef_d);
+      }
+      k[j] = take_token(p, base + j * 32, raw[j], w, w_ent, a);
+    }
+    add_terms(a, k);
+  }
+  sum_block<kThreads / 32>(a);
+  if (threadIdx.x == 0) sums[blockIdx.x] = a;
+  if (!elect_last_cta(&ctl->done)) return;
+  a = Sums{};
+  double all = 0.0, out = 0.0;
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += kThreads) {
+    const Sums& s = sums[i];
+    a.pg += __ldcg(&s.pg);
+    a.kl += __ldcg(&s.kl);
+    a.ent += __ldcg(&s.ent);
+    a.diff += __ldcg(&s.diff);
+    a.ratio += __ldcg(&s.ratio);
+    a.max_ratio = fmaxf(a.max_ratio, __ldcg(&s.max_ratio));
+    a.outside += __ldcg(&s.outside);
+    a.tokens += __ldcg(&s.tokens);
+  }
+  sum_block<kThreads / 32>(a);
+  if (threadIdx.x == 0) {
+    all = double(a.tokens), out = double(a.outside);
+    write_outputs(p, a, all, out);
+    ctl->tokens = 0ull;
+    ctl->rows = 0u;
+  }
+  if (per_row && counted)
+    for (int b = threadIdx.x; b < p.B; b += kThreads) counts[b] = 0;
+}
+
+// ------------------------------------------------------------------------------------ host side
+constexpr int kMaxCtas = 2048;
+constexpr size_t kSumsBytes = kMaxCtas * sizeof(Sums);
+
+inline int64_t workspace_bytes(int32_t B, int32_t T) {
+  if (int64_t(B) * T <= kSmallTokens && B <= kSmallRows) return 0;
+  return int64_t(256 + kSumsBytes + align256(size_t(B) * sizeof(int)));
 }
 
 // strides (host array): rows of log_prob, old, advantage, its elements (0 or 1), ref, entropy, mask.
@@ -241,36 +428,57 @@ inline int run(const float* cur, const float* old, const float* adv, const float
   if (!(clip_low >= 0.0 && clip_low < 1.0) || !(clip_high >= 0.0) || !(dual_clip == 0.0 || dual_clip > 1.0))
     return kInvalidArgument;
   if (kl_form < kK1 || kl_form > kK3 || reduction < kTokenMean || reduction > kSum) return kInvalidArgument;
-  if (strides[3] != 0 && strides[3] != 1) return kInvalidArgument;
+  for (int i = 0; i < 7; ++i)
+    if (strides[i] < 0) return kInvalidArgument;
+  if (strides[3] > 1) return kInvalidArgument;
   if (B == 0 || T == 0)
     return cudaMemsetAsync(out, 0, kOutputs * sizeof(float), stream) == cudaSuccess ? kOk : kCudaError;
   if (cur == nullptr || old == nullptr || adv == nullptr || (grad_ent != nullptr && ent == nullptr))
     return kInvalidArgument;
-  if (ws == nullptr || ws_bytes < workspace_bytes(B, T)) return kWorkspaceTooSmall;
-  Params p;
+  const int64_t n = int64_t(B) * T;
+  if (n > 0x7fffffff - 2 * int64_t(kSmallTokens)) return kUnsupported;  // token indexes are 31 bits
+  const int64_t need = workspace_bytes(B, T);
+  if (need > 0 && (ws == nullptr || ws_bytes < need)) return kWorkspaceTooSmall;
+  if (need > 0 && !aligned16(ws)) return kInvalidArgument;
+  Params p = {};
   p.cur = cur, p.old = old, p.adv = adv, p.ref = ref, p.ent = ent, p.mask = mask;
-  p.cur_s = strides[0], p.old_s = strides[1], p.adv_s = strides[2], p.adv_e = strides[3];
+  p.cur_s = strides[0], p.old_s = strides[1], p.adv_s = strides[2], p.adv_rows = strides[3] == 0;
   p.ref_s = strides[4], p.ent_s = strides[5], p.mask_s = strides[6];
-  p.B = B, p.T = T;
+  p.B = B, p.T = T, p.n = unsigned(n), p.by_T = fast_div(unsigned(T));
+  const auto dense = [&](const void* q, int64_t s) { return q == nullptr || s == T || B == 1; };
+  p.dense = dense(cur, p.cur_s) && dense(old, p.old_s) && (p.adv_rows || dense(adv, p.adv_s)) && dense(ref, p.ref_s) &&
+            dense(ent, p.ent_s) && dense(mask, p.mask_s);
+  p.need_row = !p.dense || p.adv_rows || reduction == kSequenceMean;
   p.log_high = make_pair_of(log1p(clip_high)), p.log_low = make_pair_of(log1p(-clip_low));
-  p.log_dual = make_pair_of(dual_clip > 0.0 ? log(dual_clip) : 0.0);
+  p.log_dual = make_pair_of(dual_clip > 0.0 ? log(dual_clip) : double(NAN));  // NaN: no difference is it
   p.high = float(1.0 + clip_high), p.low = float(1.0 - clip_low), p.dual = float(dual_clip);
-  p.kl_coef = float(kl_coef), p.ent_coef = float(ent_coef), p.kl_form = kl_form, p.reduction = reduction;
+  p.kl_coef = float(kl_coef), p.kl_form = kl_form, p.reduction = reduction;
   p.scale = scale, p.kl_coef_d = kl_coef, p.ent_coef_d = ent_coef;
   p.grad = grad, p.grad_ent = grad_ent, p.out = out;
+  if (need == 0) return launch_pdl(small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, p);
+
   char* w = static_cast<char*>(ws);
-  Norm* norm = reinterpret_cast<Norm*>(w + 64);
-  int* counts = reinterpret_cast<int*>(w + 256);
-  Sums* sums = reinterpret_cast<Sums*>(w + 256 + align256(size_t(B) * sizeof(int)));
-  int st = launch_pdl(count_kernel, dim3(B), dim3(kThreads), 0, stream, p, counts);
-  if (st == kOk) st = launch_pdl(norm_kernel, dim3(1), dim3(32), 0, stream, p, static_cast<const int*>(counts), norm);
-  if (st == kOk)
-    st = launch_pdl(token_kernel, dim3(B), dim3(kThreads), 0, stream, p, static_cast<const int*>(counts),
-                    static_cast<const Norm*>(norm), sums);
-  if (st == kOk)
-    st = launch_pdl(finish_kernel, dim3(1), dim3(1), 0, stream, p, static_cast<const Norm*>(norm),
-                    static_cast<const Sums*>(sums));
-  return st;
+  Ctl* ctl = reinterpret_cast<Ctl*>(w);
+  Sums* sums = reinterpret_cast<Sums*>(w + 256);
+  int* counts = reinterpret_cast<int*>(w + 256 + kSumsBytes);
+  const bool counted = mask != nullptr && reduction != kSum;
+  if (counted) {
+    const unsigned stretches = unsigned((int64_t(T) + kStretch - 1) / kStretch);
+    const int64_t warps = int64_t(B) * stretches;
+    const int64_t want = (warps + kThreads / 32 - 1) / (kThreads / 32), most = int64_t(sm_count()) * 4;
+    const int st = launch_pdl(count_kernel, dim3(unsigned(want < most ? want : most)), dim3(kThreads), 0, stream, p,
+                              stretches, ctl, counts);
+    if (st != kOk) return st;
+  }
+  const int64_t units = (n + kThreads * kPer - 1) / (kThreads * kPer);
+  int64_t ctas = int64_t(sm_count()) * resident_ctas_per_sm(token_kernel, kThreads, 0);
+  if (ctas > kMaxCtas) ctas = kMaxCtas;
+  if (ctas > units) ctas = units;
+  const int streams = 2 + !p.adv_rows + (ref != nullptr) + (ent != nullptr);
+  const int64_t unit_bytes = int64_t(kThreads) * kPer * 4 * streams;
+  const unsigned prefetch = unsigned(kPrefetchBytes / (unit_bytes * ctas));
+  return launch_pdl(token_kernel, dim3(unsigned(ctas)), dim3(kThreads), 0, stream, p, counted, prefetch, ctl, counts,
+                    sums);
 }
 
 }  // namespace policy

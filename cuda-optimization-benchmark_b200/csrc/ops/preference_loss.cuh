@@ -12,6 +12,7 @@
 // The sums are in fp64: their difference, a small part of them, is what the loss sees.
 #pragma once
 
+#include "../common/bulk.cuh"
 #include "../common/dtype.cuh"
 #include "../common/workspace.cuh"
 
@@ -61,65 +62,164 @@ struct PairOut {
   double loss, win, gap;
 };
 
-__global__ void __launch_bounds__(kThreads) pair_kernel(Params p, PairOut* __restrict__ pairs) {
-  pdl_begin();
-  const int64_t b = blockIdx.x;
-  __shared__ double part[kThreads];
-  __shared__ unsigned cnt[kThreads];
+// An answer's sum and number of tokens.
+struct Part {
+  double s;
+  unsigned n;
+};
+
+// The workspace's control words: zero before the first call, and again after each.
+struct Ctl {
+  unsigned done;
+};
+
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kPer = 8;  // tokens of a lane in flight: log-prob and reference of each
+
+// This CTA's stretch of answer b: tokens [t0, t1), lanes on consecutive ones.
+__device__ __forceinline__ Part sum_stretch(const Side& d, int64_t b, int t0, int t1) {
+  const float *lp = d.lp + b * d.lp_s, *ref = d.ref == nullptr ? nullptr : d.ref + b * d.ref_s;
+  const uint8_t* m = d.mask == nullptr ? nullptr : d.mask + b * d.mask_s;
+  double s = 0.0;
+  unsigned n = 0;
+  for (int t = t0 + int(threadIdx.x); t < t1; t += kPer * kThreads) {
+    float x[kPer], r[kPer];
+    bool on[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int at = t + k * kThreads;
+      on[k] = at < t1 && (m == nullptr || m[at] != 0);
+      x[k] = at < t1 ? lp[at] : 0.0f;
+      r[k] = ref != nullptr && at < t1 ? ref[at] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (!on[k]) continue;
+      s += double(x[k]) - double(r[k]);
+      ++n;
+    }
+  }
+  return Part{s, n};
+}
+
+__device__ __forceinline__ void write_stretch(const Side& d, int64_t b, int t0, int t1, float slope) {
+  if (d.grad == nullptr) return;
+  const uint8_t* m = d.mask == nullptr ? nullptr : d.mask + b * d.mask_s;
+  float* g = d.grad + b * d.T;
+  for (int t = t0 + int(threadIdx.x); t < t1; t += kPer * kThreads) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int at = t + k * kThreads;
+      if (at < t1) g[at] = m == nullptr || m[at] != 0 ? slope : 0.0f;
+    }
+  }
+}
+
+// A cluster of `parts` CTAs per pair, each on a stretch of both answers: the CTAs exchange their sums through
+// shared memory, every one forms the pair's slope from all of them in the same order and writes its
+// stretch of the gradients.  The last CTA of the grid adds up the pairs in their order.
+__global__ void __launch_bounds__(kThreads) pair_kernel(const Params p, unsigned parts, Ctl* ctl, PairOut* pairs) {
+  __shared__ Part warp_part[2][kWarps];
+  __shared__ Part cta_part[2][kMaxCluster];
   __shared__ float slope[2];
-  double s[2];
-  unsigned n[2];
+  __shared__ double total[3][kWarps];
+  const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
+  const unsigned part = blockIdx.x % parts;
+  const int64_t b = blockIdx.x / parts;
+  pdl_begin();
+  // Every CTA of the cluster runs before any of them writes to another (waited for below).
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  int t0[2], t1[2];
+#pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const Side& d = p.side[k];
-    double a = 0.0;
-    unsigned c = 0;
-    for (int64_t t = threadIdx.x; t < d.T; t += kThreads) {
-      if (d.mask != nullptr && d.mask[b * d.mask_s + t] == 0) continue;
-      a += double(d.lp[b * d.lp_s + t]) - (d.ref ? double(d.ref[b * d.ref_s + t]) : 0.0);
-      ++c;
+    const int per = int((unsigned(p.side[k].T) + parts - 1) / parts);
+    t0[k] = int(min(int64_t(p.side[k].T), int64_t(per) * part));
+    t1[k] = int(min(int64_t(p.side[k].T), int64_t(t0[k]) + per));
+    Part a = sum_stretch(p.side[k], b, t0[k], t1[k]);
+    a.s = warp_sum(a.s);
+    a.n = warp_sum_u32(a.n);
+    if (lane == 0) warp_part[k][w] = a;
+  }
+  if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  __syncthreads();
+  if (w < 2) {  // warp k: answer k
+    Part a = lane < kWarps ? warp_part[w][lane] : Part{0.0, 0u};
+    a.s = warp_sum(a.s);
+    a.n = warp_sum_u32(a.n);
+    if (lane < parts) {  // into CTA `lane`'s cta_part[w][part]
+      if (parts == 1) {
+        cta_part[w][0] = a;
+      } else {
+        uint32_t dst;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                     : "=r"(dst)
+                     : "r"(smem_addr(&cta_part[w][part])), "r"(lane));
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst), "d"(a.s) : "memory");
+        asm volatile("st.shared::cluster.u32 [%0 + 8], %1;" ::"r"(dst), "r"(a.n) : "memory");
+      }
     }
-    part[threadIdx.x] = a;
-    cnt[threadIdx.x] = c;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < kThreads; ++i) a += part[i], c += cnt[i];
-      s[k] = a;
-      n[k] = c;
-    }
+  }
+  if (parts > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    double inv[2] = {1.0, 1.0};
-    for (int k = 0; k < 2; ++k)
-      if (p.average) inv[k] = 1.0 / (n[k] > 0 ? n[k] : 1), s[k] *= inv[k];
-    const double rc = p.beta * s[0], rr = p.beta * s[1];
+    double s[2], inv[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      Part a = cta_part[k][0];
+      for (unsigned i = 1; i < parts; ++i) a.s += cta_part[k][i].s, a.n += cta_part[k][i].n;
+      inv[k] = p.average ? 1.0 / double(a.n > 0 ? a.n : 1u) : 1.0;
+      s[k] = a.s * inv[k];
+    }
+    const double gap = p.beta * (s[0] - s[1]);
     double dz;
-    const double loss = pair_loss(p, p.beta * (s[0] - s[1]) - p.margin, dz);
-    pairs[b] = PairOut{loss, s[0] > s[1] ? 1.0 : 0.0, p.beta * (s[0] - s[1])};
-    p.side[0].reward[b] = float(rc);
-    p.side[1].reward[b] = float(rr);
+    const double loss = pair_loss(p, gap - p.margin, dz);
+    if (part == 0) {
+      pairs[b] = PairOut{loss, s[0] > s[1] ? 1.0 : 0.0, gap};
+      p.side[0].reward[b] = float(p.beta * s[0]);
+      p.side[1].reward[b] = float(p.beta * s[1]);
+    }
     slope[0] = float(p.beta * dz * inv[0] / p.B);
     slope[1] = float(-p.beta * dz * inv[1] / p.B);
   }
   __syncthreads();
-  for (int k = 0; k < 2; ++k) {
-    const Side& d = p.side[k];
-    if (d.grad == nullptr) continue;
-    for (int64_t t = threadIdx.x; t < d.T; t += kThreads)
-      d.grad[b * d.T + t] = d.mask != nullptr && d.mask[b * d.mask_s + t] == 0 ? 0.0f : slope[k];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) write_stretch(p.side[k], b, t0[k], t1[k], slope[k]);
+  if (!elect_last_cta(&ctl->done)) return;
+  double a[3] = {0.0, 0.0, 0.0};
+  for (int i = threadIdx.x; i < p.B; i += kThreads) {
+    a[0] += __ldcg(&pairs[i].loss);
+    a[1] += __ldcg(&pairs[i].win);
+    a[2] += __ldcg(&pairs[i].gap);
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    a[k] = warp_sum(a[k]);
+    if (lane == 0) total[k][w] = a[k];
+  }
+  __syncthreads();
+  if (w == 0) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const double s = warp_sum(lane < kWarps ? total[k][lane] : 0.0);
+      if (lane == 0) p.out[k] = float(s / p.B);
+    }
   }
 }
 
-__global__ void finish_kernel(Params p, const PairOut* __restrict__ pairs) {
-  pdl_begin();
-  PairOut a = {};
-  for (int b = 0; b < p.B; ++b) a.loss += pairs[b].loss, a.win += pairs[b].win, a.gap += pairs[b].gap;
-  p.out[0] = float(a.loss / p.B);
-  p.out[1] = float(a.win / p.B);
-  p.out[2] = float(a.gap / p.B);
-}
-
 inline int64_t workspace_bytes(int32_t B) { return int64_t(256 + align256(size_t(B) * sizeof(PairOut))); }
+
+// CTAs per pair: 1 once two CTAs per SM have a pair each, else enough for that, but no CTA with fewer than
+// 2048 tokens.
+inline unsigned cluster_of(int64_t pairs, int64_t tokens) {
+  unsigned c = 1;
+  while (c < unsigned(kMaxCluster) && pairs * c < 2 * sm_count() && tokens / (2 * c) >= 2048) c *= 2;
+  return c;
+}
 
 // strides (host array): rows of chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask.
 inline int run(const float* chosen, const float* rejected, const float* ref_chosen, const float* ref_rejected,
@@ -132,21 +232,40 @@ inline int run(const float* chosen, const float* rejected, const float* ref_chos
     return kInvalidArgument;
   if (form != kSigmoid && smoothing != 0.0) return kInvalidArgument;
   if ((ref_chosen == nullptr) != (ref_rejected == nullptr) && Tc > 0 && Tr > 0) return kInvalidArgument;
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] < 0) return kInvalidArgument;
   if (B == 0) return cudaMemsetAsync(out, 0, kOutputs * sizeof(float), stream) == cudaSuccess ? kOk : kCudaError;
   if ((Tc > 0 && chosen == nullptr) || (Tr > 0 && rejected == nullptr) || reward_chosen == nullptr ||
       reward_rejected == nullptr)
     return kInvalidArgument;
+  // Token indexes run in ints, up to a round of the CTA past the end.
+  if (Tc > 0x7fffffff - kPer * kThreads || Tr > 0x7fffffff - kPer * kThreads) return kUnsupported;
   if (ws == nullptr || ws_bytes < workspace_bytes(B)) return kWorkspaceTooSmall;
+  if (!aligned16(ws)) return kInvalidArgument;
   Params p;
   p.side[0] = Side{chosen, ref_chosen, chosen_mask, strides[0], strides[2], strides[4], Tc, reward_chosen, grad_chosen};
   p.side[1] =
       Side{rejected, ref_rejected, rejected_mask, strides[1], strides[3], strides[5], Tr, reward_rejected, grad_rejected};
   p.B = B, p.beta = beta, p.smoothing = smoothing, p.margin = margin, p.form = form, p.average = average != 0;
   p.out = out;
-  PairOut* pairs = reinterpret_cast<PairOut*>(static_cast<char*>(ws) + 256);
-  int st = launch_pdl(pair_kernel, dim3(B), dim3(kThreads), 0, stream, p, pairs);
-  if (st == kOk) st = launch_pdl(finish_kernel, dim3(1), dim3(1), 0, stream, p, static_cast<const PairOut*>(pairs));
-  return st;
+  const unsigned parts = cluster_of(B, int64_t(Tc) + Tr);
+  if (int64_t(B) * parts > 0x7fffffff) return kUnsupported;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(B) * parts);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = parts;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = parts > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, pair_kernel, p, parts, static_cast<Ctl*>(ws),
+                            reinterpret_cast<PairOut*>(static_cast<char*>(ws) + 256)) == cudaSuccess
+             ? kOk
+             : kCudaError;
 }
 
 }  // namespace pref

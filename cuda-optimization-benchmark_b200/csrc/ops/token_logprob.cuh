@@ -34,7 +34,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;          // vectors in flight per thread
 constexpr int kMaxCluster = 8;
-constexpr int64_t kWarpRowV = 1024;
+constexpr int64_t kWarpRowV = 8192;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Below this, 2^z is 0 in fp32: z is held above it so that 0 * z stays 0 (z = -inf at masked logits).
@@ -91,23 +91,41 @@ __device__ __forceinline__ void add_one(Acc& a, float x, float c2) {
   if (kEnt) a.u = fmaf(e, z, a.u);
 }
 
-// A running row part: packed sums over pairs of elements.
+// A running row part: packed sums over pairs of elements, in kSets sets: one where many threads share a row
+// (registers are occupancy there), two where a warp has a row for itself (shorter chains of additions).
+template <int kSets>
 struct Run {
   float m;
-  float2 s, u;
+  float2 s[kSets], u[kSets];
 };
+template <int kSets>
+__device__ __forceinline__ void start_run(Run<kSets>& r, const Acc& a) {
+  r.m = a.m;
+#pragma unroll
+  for (int k = 0; k < kSets; ++k) {
+    r.s[k] = make_float2(k == 0 ? a.s : 0.0f, 0.0f);
+    r.u[k] = make_float2(k == 0 ? a.u : 0.0f, 0.0f);
+  }
+}
+template <int kSets>
+__device__ __forceinline__ Acc total(const Run<kSets>& r) {
+  float2 s = r.s[0], u = r.u[0];
+#pragma unroll
+  for (int k = 1; k < kSets; ++k) s = add2(s, r.s[k]), u = add2(u, r.u[k]);
+  return Acc{r.m, s.x + s.y, u.x + u.y};
+}
 
 // kN vectors, of which the first n are there.
-template <typename T, bool kEnt, int kN>
-__device__ __forceinline__ void add_vectors(Run& r, const uint4 (&v)[kN], int n, float c2) {
+template <typename T, bool kEnt, int kN, int kSets>
+__device__ __forceinline__ void add_vectors(Run<kSets>& r, const uint4 (&v)[kN], int n, float c2) {
   float top = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kN; ++k)
     if (k < n) top = fmaxf(top, max16<T>(v[k]));
   if (top > r.m) {
-    Acc a{r.m, r.s.x + r.s.y, r.u.x + r.u.y};
+    Acc a = total(r);
     rebase(a, top, c2);
-    r = Run{a.m, make_float2(a.s, 0.0f), make_float2(a.u, 0.0f)};
+    start_run(r, a);
   }
   const float2 neg = splat2(r.m > -INFINITY ? -r.m : 0.0f), c = splat2(c2);
 #pragma unroll
@@ -120,8 +138,9 @@ __device__ __forceinline__ void add_vectors(Run& r, const uint4 (&v)[kN], int n,
       float2 z = mul2(add2(f[j], neg), c);
       if (kEnt) z = make_float2(max_nan(z.x, kLowZ), max_nan(z.y, kLowZ));
       const float2 e = make_float2(exp2_approx(z.x), exp2_approx(z.y));
-      r.s = add2(r.s, e);
-      if (kEnt) r.u = fma2(e, z, r.u);
+      const int set = j % kSets;
+      r.s[set] = add2(r.s[set], e);
+      if (kEnt) r.u[set] = fma2(e, z, r.u[set]);
     }
   }
 }
@@ -138,29 +157,32 @@ template <typename T, bool kEnt, int kN>
 __device__ __forceinline__ Acc row_part(const T* row, int64_t V, unsigned part, unsigned parts, int tid, float c2) {
   constexpr int kE = Vec16<T>::kElems;
   const int64_t head = head_elems(row, V), nv = (V - head) / kE;
-  const int64_t v0 = nv * part / parts, v1 = nv * (part + 1) / parts;
+  const unsigned per = (unsigned(nv) + parts - 1) / parts;
+  const int64_t v0 = int64_t(per) * part, v1 = min(nv, v0 + per);
   const uint4* vec = reinterpret_cast<const uint4*>(row + head);
-  Run r{-INFINITY, splat2(0.0f), splat2(0.0f)};
+  // The elements before and behind the vectors, loaded first so that their wait overlaps the vectors'.
+  const int64_t rest = head + nv * kE + tid;
+  const bool has_head = part == 0 && tid < head, has_rest = part == 0 && rest < V;
+  const float x_head = has_head ? to_f32(row[tid]) : 0.0f, x_rest = has_rest ? to_f32(row[rest]) : 0.0f;
+  Run<kN == 32 ? 2 : 1> r;
+  start_run(r, empty_acc());
   int64_t i = v0 + tid;
   for (; i + (kUnroll - 1) * kN < v1; i += kUnroll * kN) {
     uint4 v[kUnroll];
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) v[k] = ld_stream_u4(vec + i + k * kN);
-    add_vectors<T, kEnt, kUnroll>(r, v, kUnroll, c2);
+    add_vectors<T, kEnt>(r, v, kUnroll, c2);
   }
   if (i < v1) {
     uint4 v[kUnroll - 1];
     const int n = int((v1 - i + kN - 1) / kN);
 #pragma unroll
     for (int k = 0; k < kUnroll - 1; ++k) v[k] = k < n ? ld_stream_u4(vec + i + k * kN) : make_uint4(0, 0, 0, 0);
-    add_vectors<T, kEnt, kUnroll - 1>(r, v, n, c2);
+    add_vectors<T, kEnt>(r, v, n, c2);
   }
-  Acc a{r.m, r.s.x + r.s.y, r.u.x + r.u.y};
-  if (part == 0) {
-    if (tid < head) add_one<kEnt>(a, to_f32(row[tid]), c2);
-    const int64_t rest = head + nv * kE + tid;
-    if (rest < V) add_one<kEnt>(a, to_f32(row[rest]), c2);
-  }
+  Acc a = total(r);
+  if (has_head) add_one<kEnt>(a, x_head, c2);
+  if (has_rest) add_one<kEnt>(a, x_rest, c2);
   return a;
 }
 
@@ -308,11 +330,13 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, unsigne
                     __funnelshift_r(lo.z, lo.w, bits), __funnelshift_r(lo.w, next, bits));
 }
 
-// Rows cut into pieces of kPieceVecs vectors, a CTA (a warp of it for short rows) each.
+// Rows cut into equal pieces of at most kPieceVecs vectors, a CTA (a warp of it for short rows) each.
 constexpr int kPieceVecs = kThreads * kUnroll;
 
+// Occupancy, measured at 4096 rows of 131072 bf16 logits: 6 CTAs per SM 335 us, 4 CTAs 384 us (4096 logits a
+// row, warps: 5 CTAs 328 us, 6 CTAs, which spill, 352 us).
 template <typename T, bool kEnt, bool kWarpRows>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const T* x, const int64_t* __restrict__ token, Rows q,
+__global__ void __launch_bounds__(kThreads, kWarpRows ? 5 : 6) backward_kernel(const T* x, const int64_t* __restrict__ token, Rows q,
                                                             float inv, unsigned pieces, Grad g, T* out) {
   pdl_begin();
   constexpr int kE = Vec16<T>::kElems;
@@ -338,8 +362,8 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const T* x, const in
     const int64_t room = (V - head) * int64_t(sizeof(T)) + delta;  // bytes from the first aligned block to the end
     nv = min(nv, room / 16 - 1);  // at least 0: room is above 16
   }
-  const int64_t per = kWarpRows ? nv : int64_t(kPieceVecs);
-  const int64_t v0 = int64_t(piece) * per, v1 = min(nv, v0 + per);
+  const unsigned per = (unsigned(nv) + pieces - 1) / pieces;
+  const int64_t v0 = int64_t(per) * piece, v1 = min(nv, v0 + per);
   const char* src = reinterpret_cast<const char*>(row + head) - delta;
   uint4* vec = reinterpret_cast<uint4*>(dst + head);
   const int64_t tail = head + nv * kE;
@@ -362,24 +386,39 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const T* x, const in
     k.k_e = -inv * ge * kLn2;
     k.k_tok = inv * gl;
   }
-  for (int64_t i = v0 + tid; i < v1; i += kUnroll * kN) {
-    uint4 v[kUnroll];
-    if (delta == 0) {
+  if (delta == 0) {
+    for (int64_t i = v0 + tid; i < v1; i += kUnroll * kN) {
+      uint4 v[kUnroll];
 #pragma unroll
       for (int j = 0; j < kUnroll; ++j)
         if (i + j * kN < v1) v[j] = ld_once_u4(src + 16 * (i + j * kN));
-    } else {
 #pragma unroll
-      for (int j = 0; j < kUnroll; ++j)
-        if (i + j * kN < v1) {
-          const uint4* s = reinterpret_cast<const uint4*>(src) + i + j * kN;
-          v[j] = shifted(__ldg(s), __ldg(s + 1), delta);
-        }
+      for (int j = 0; j < kUnroll; ++j) {
+        const int64_t at = i + j * kN;
+        if (at < v1) st_stream_u4(vec + at, grad_vector<T, kEnt>(v[j], head + at * kE, tok, k, c2));
+      }
     }
+  } else {
+    // A lane's second block is the next lane's first, so whole warps go round together.
+    for (int64_t i = v0 + tid; i - lane < v1; i += 2 * kN) {
+      uint4 v[2], last[2];  // last: lane 31's second block
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int64_t at = i + j * kN;
-      if (at < v1) st_stream_u4(vec + at, grad_vector<T, kEnt>(v[j], head + at * kE, tok, k, c2));
+      for (int j = 0; j < 2; ++j) {
+        const int64_t at = i + j * kN;
+        v[j] = at <= v1 ? ld_stream_u4(src + 16 * at) : make_uint4(0, 0, 0, 0);
+        last[j] = lane == 31 && at < v1 ? ld_stream_u4(src + 16 * (at + 1)) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint4 n;
+        n.x = __shfl_down_sync(0xffffffffu, v[j].x, 1);
+        n.y = __shfl_down_sync(0xffffffffu, v[j].y, 1);
+        n.z = __shfl_down_sync(0xffffffffu, v[j].z, 1);
+        n.w = __shfl_down_sync(0xffffffffu, v[j].w, 1);
+        const int64_t at = i + j * kN;
+        const uint4 x4 = shifted(v[j], lane == 31 ? last[j] : n, delta);
+        if (at < v1) st_stream_u4(vec + at, grad_vector<T, kEnt>(x4, head + at * kE, tok, k, c2));
+      }
     }
   }
   if (piece == 0) {
@@ -413,10 +452,11 @@ inline int with_flag(bool flag, F&& f) {
 }
 
 // CTAs per row: 1 once two CTAs per SM have a row each, else enough for that, but no CTA with fewer than
-// 2048 logits.
+// 8192 logits: joining a cluster costs more than it saves there (64 rows of 50001 bf16 logits: 5.2 us with
+// 4 CTAs a row, 6.2 us with 8; 2044 rows: 37 us with one, 42 us with 2, 56 us with 4).
 inline unsigned cluster_of(int64_t rows, int64_t V) {
   unsigned c = 1;
-  while (c < unsigned(kMaxCluster) && rows * c < 2 * sm_count() && V / (2 * c) >= 2048) c *= 2;
+  while (c < unsigned(kMaxCluster) && rows * c < 2 * sm_count() && V / (2 * c) >= 8192) c *= 2;
   return c;
 }
 

@@ -439,11 +439,12 @@ def token_logprob(logits, token, temperature=1.0, grad_log_prob=None, grad_entro
     of the logits where gradients are given.  Returns (values, errors) as linear_recurrence.
 
     The bound: exp has a relative error of 4 u and its argument d one of 3 u |d| (difference, scaling by a
-    rounded 1 / temperature), a sum of V terms by at most 256 threads ceil(V / 256) + 16 roundings, so
-    K = ceil(V / 256) + 32 roundings cover log S and p beside the |d| part."""
+    rounded 1 / temperature).  A sum of V terms is taken in at least 128 interleaved chains (a warp, two sets of
+    pairs) that meet in a tree: ceil(V / 128) + 16 roundings, so K = ceil(V / 128) + 32 roundings cover log S
+    and p beside the |d| part."""
     x, tok = _f64(logits), np.asarray(token.cpu() if hasattr(token, "cpu") else token)
     V = x.shape[-1]
-    K = -(-V // 256) + 32
+    K = -(-V // 128) + 32
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
         d = (x - x.max(-1, keepdims=True)) / temperature
         e = np.exp(d)
