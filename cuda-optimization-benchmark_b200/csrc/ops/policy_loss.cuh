@@ -86,11 +86,12 @@ struct Params {
   unsigned n;      // B * T
   FastDiv by_T;
   bool dense;      // every stream's row stride is T: a token has one offset in all of them
+  bool vec;        // four consecutive tokens are one aligned vector of every stream
   bool adv_rows;   // one advantage per row
   bool need_row;   // a token's row is needed
   Pair log_high, log_low, log_dual;
   float high, low, dual;  // 1 + clip_high, 1 - clip_low, c (0: off)
-  float kl_coef;
+  float kl_coef, ent_coef;
   int kl_form, reduction;
   double scale, kl_coef_d, ent_coef_d;
   float *grad, *grad_ent, *out;
@@ -117,95 +118,161 @@ __device__ __forceinline__ float token_weight(const Params& p, unsigned long lon
   return float(p.scale);
 }
 
-// One token as it is read.
+// The tokens of one lane as they are read: kPer consecutive ones (p.vec), or kPer a warp's width apart.  What
+// masked-out tokens hold is read with the others and not used.
+constexpr int kPer = 4;
+
 struct Raw {
-  float cur, old, adv, ref, ent;
-  unsigned row;
-  bool on;
+  float cur[kPer], old[kPer], adv[kPer], ref[kPer], ent[kPer];
+  unsigned row[kPer];
+  unsigned on;  // bit j: token j counts
 };
 
-__device__ __forceinline__ Raw load_token(const Params& p, unsigned i) {
-  Raw r = {};
-  if (i >= p.n) return r;
-  unsigned t = i;
-  if (p.need_row) {
-    r.row = p.by_T.div(i);
-    t = i - r.row * unsigned(p.T);
-  }
-  const int64_t b = r.row;
-  const auto at = [&](int64_t stride) { return p.dense ? int64_t(i) : b * stride + t; };
-  r.on = p.mask == nullptr || p.mask[at(p.mask_s)] != 0;
-  if (r.on) {
-    r.cur = p.cur[at(p.cur_s)];
-    r.old = p.old[at(p.old_s)];
-    r.adv = p.adv_rows ? p.adv[b * p.adv_s] : p.adv[at(p.adv_s)];
-    if (p.ref != nullptr) r.ref = p.ref[at(p.ref_s)];
-    if (p.ent != nullptr) r.ent = p.ent[at(p.ent_s)];
-  }
-  return r;
+__device__ __forceinline__ void load4(const float* p, int64_t at, float (&f)[kPer]) {
+  const float4 v = ld_stream_f4(p + at);
+  f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
 }
 
-// What a token adds (policy, kl and entropy terms weighted with w), and its gradient, which is written.
+// First token and distance between the tokens of a lane, in stretch u of `threads` * kPer tokens.
+template <bool kVec>
+__device__ __forceinline__ unsigned first_token(unsigned u, unsigned threads) {
+  const unsigned at = u * threads * kPer;
+  return kVec ? at + threadIdx.x * kPer : at + threadIdx.x / 32 * (32 * kPer) + threadIdx.x % 32;
+}
+template <bool kVec>
+__device__ __forceinline__ unsigned token_of(unsigned first, int j) {
+  return kVec ? first + j : first + j * 32;
+}
+
+template <bool kVec>
+__device__ __forceinline__ void load_tokens(const Params& p, unsigned first, Raw& r) {
+  r.on = 0u;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) r.cur[j] = r.old[j] = r.adv[j] = r.ref[j] = r.ent[j] = 0.0f, r.row[j] = 0u;
+  if (kVec && first + kPer <= p.n) {
+    unsigned t = first;
+    if (p.need_row) {
+      if (p.T % kPer == 0) {
+        r.row[0] = p.by_T.div(first);
+        t = first - r.row[0] * unsigned(p.T);
+        r.row[1] = r.row[2] = r.row[3] = r.row[0];
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) r.row[j] = p.by_T.div(first + j);
+      }
+    }
+    const int64_t b = r.row[0];
+    const auto at = [&](int64_t stride) { return p.dense ? int64_t(first) : b * stride + t; };
+    uint32_t m = 0x01010101u;
+    if (p.mask != nullptr) m = __vminu4(*reinterpret_cast<const uint32_t*>(p.mask + at(p.mask_s)), 0x01010101u);
+    load4(p.cur, at(p.cur_s), r.cur);
+    load4(p.old, at(p.old_s), r.old);
+    if (p.adv_rows) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) r.adv[j] = p.adv[int64_t(r.row[j]) * p.adv_s];
+    } else {
+      load4(p.adv, at(p.adv_s), r.adv);
+    }
+    if (p.ref != nullptr) load4(p.ref, at(p.ref_s), r.ref);
+    if (p.ent != nullptr) load4(p.ent, at(p.ent_s), r.ent);
+    r.on = (m * 0x10204080u) >> 28;  // bit 8 j of m to bit j
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const unsigned i = token_of<kVec>(first, j);
+      if (i >= p.n) continue;
+      unsigned t = i;
+      if (p.need_row) {
+        r.row[j] = p.by_T.div(i);
+        t = i - r.row[j] * unsigned(p.T);
+      }
+      const int64_t b = r.row[j];
+      const auto at = [&](int64_t stride) { return p.dense ? int64_t(i) : b * stride + t; };
+      if (p.mask == nullptr || p.mask[at(p.mask_s)] != 0) r.on |= 1u << j;
+      r.cur[j] = ld_stream_f1(p.cur + at(p.cur_s));
+      r.old[j] = ld_stream_f1(p.old + at(p.old_s));
+      r.adv[j] = p.adv_rows ? p.adv[b * p.adv_s] : ld_stream_f1(p.adv + at(p.adv_s));
+      if (p.ref != nullptr) r.ref[j] = ld_stream_f1(p.ref + at(p.ref_s));
+      if (p.ent != nullptr) r.ent[j] = ld_stream_f1(p.ent + at(p.ent_s));
+    }
+  }
+}
+
+// What a token adds: policy, kl and entropy terms weighted with w, exp(d) - 1 - d, r; and its gradient.
 struct Terms {
   float pg, kl, ent, diff, ratio;
 };
 
-__device__ __forceinline__ Terms take_token(const Params& p, unsigned i, const Raw& r, float w, float w_ent, Sums& a) {
-  Terms k = {};
-  float g = 0.0f;
-  if (r.on) {
-    const float s = __fsub_rn(r.cur, r.old);
-    bool hi = s > p.log_high.hi, lo = s < p.log_low.hi;
-    bool dual = p.dual > 0.0f && r.adv < 0.0f && s > p.log_dual.hi;
-    if (s == p.log_high.hi || s == p.log_low.hi || s == p.log_dual.hi) {  // the rounding decides: look at it
-      float e;
-      two_diff(r.cur, r.old, k.diff, e);
-      hi = above(s, e, p.log_high);
-      lo = below(s, e, p.log_low);
-      dual = p.dual > 0.0f && r.adv < 0.0f && above(s, e, p.log_dual);
-    }
-    k.ratio = exp2_approx(s * 1.4426950408889634f);
-    k.diff = exp_minus_1_minus(s);
-    const bool clipped = (r.adv > 0.0f && hi) || (r.adv < 0.0f && lo) || dual || r.adv == 0.0f;
-    const float held = dual ? p.dual : hi ? p.high : lo ? p.low : k.ratio;
-    const float pg = r.adv == 0.0f ? 0.0f : (clipped ? held : k.ratio) * -r.adv;
-    g = clipped ? 0.0f : pg;
-    if (p.ref != nullptr) {
-      const float q = __fsub_rn(r.ref, r.cur);
-      float dkl;
-      if (p.kl_form == kK1) {
-        k.kl = -q, dkl = 1.0f;
-      } else if (p.kl_form == kK2) {
-        k.kl = 0.5f * q * q, dkl = -q;
-      } else {
-        k.kl = exp_minus_1_minus(q), dkl = -(q + k.kl);  // 1 - exp(q)
-      }
-      g = fmaf(p.kl_coef, dkl, g);
-      k.kl *= w;
-    }
-    k.pg = pg * w;
-    k.ent = r.ent * w;
-    g *= w;
-    a.max_ratio = fmaxf(a.max_ratio, k.ratio);
-    a.outside += hi || lo;
-    a.tokens += 1u;
+__device__ __forceinline__ float take_token(const Params& p, const Raw& r, int j, float w, Sums& a, Terms& k) {
+  k = Terms{0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  if (((r.on >> j) & 1u) == 0u) return 0.0f;
+  const float cur = r.cur[j], adv = r.adv[j];
+  const float s = __fsub_rn(cur, r.old[j]);
+  bool hi = s > p.log_high.hi, lo = s < p.log_low.hi;
+  bool dual = adv < 0.0f && s > p.log_dual.hi;
+  if (s == p.log_high.hi || s == p.log_low.hi || s == p.log_dual.hi) {  // the rounding decides: look at it
+    float d, e;
+    two_diff(cur, r.old[j], d, e);
+    hi = above(s, e, p.log_high);
+    lo = below(s, e, p.log_low);
+    dual = adv < 0.0f && above(s, e, p.log_dual);
   }
-  if (i < p.n) {
-    if (p.grad) p.grad[i] = g;
-    if (p.grad_ent) p.grad_ent[i] = r.on ? w_ent : 0.0f;
+  k.ratio = exp2_approx(s * 1.4426950408889634f);
+  k.diff = exp_minus_1_minus(s);
+  const bool clipped = (adv > 0.0f && hi) || (adv < 0.0f && lo) || dual || adv == 0.0f;
+  const float held = dual ? p.dual : hi ? p.high : p.low;
+  const float pg = adv == 0.0f ? 0.0f : (clipped ? held : k.ratio) * -adv;
+  float g = clipped ? 0.0f : pg;
+  if (p.ref != nullptr) {
+    const float q = __fsub_rn(r.ref[j], cur);
+    float dkl;
+    if (p.kl_form == kK1) {
+      k.kl = -q, dkl = 1.0f;
+    } else if (p.kl_form == kK2) {
+      k.kl = 0.5f * q * q, dkl = -q;
+    } else {
+      k.kl = exp_minus_1_minus(q), dkl = -(q + k.kl);  // 1 - exp(q)
+    }
+    g = fmaf(p.kl_coef, dkl, g);
+    k.kl *= w;
   }
-  return k;
+  k.pg = pg * w;
+  k.ent = r.ent[j] * w;
+  a.max_ratio = fmaxf(a.max_ratio, k.ratio);
+  a.outside += hi || lo;
+  return g * w;
 }
 
-// kPer tokens of one lane: their terms are added in fp32 in a tree and then to the running sums in fp64.
-constexpr int kPer = 4;
-
-__device__ __forceinline__ void add_terms(Sums& a, const Terms (&k)[kPer]) {
+// The tokens of one lane: their terms are added in fp32 in a tree and then to the running sums in fp64, their
+// gradients are written.  w: each token's weight.
+template <bool kVec>
+__device__ __forceinline__ void take_tokens(const Params& p, unsigned first, const Raw& r, const float (&w)[kPer],
+                                            Sums& a) {
+  Terms k[kPer];
+  float g[kPer], ge[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    g[j] = take_token(p, r, j, w[j], a, k[j]);
+    ge[j] = ((r.on >> j) & 1u) != 0u ? -w[j] * p.ent_coef : 0.0f;
+  }
+  a.tokens += __popc(r.on);
   a.pg += double((k[0].pg + k[1].pg) + (k[2].pg + k[3].pg));
-  a.kl += double((k[0].kl + k[1].kl) + (k[2].kl + k[3].kl));
-  a.ent += double((k[0].ent + k[1].ent) + (k[2].ent + k[3].ent));
+  if (p.ref != nullptr) a.kl += double((k[0].kl + k[1].kl) + (k[2].kl + k[3].kl));
+  if (p.ent != nullptr) a.ent += double((k[0].ent + k[1].ent) + (k[2].ent + k[3].ent));
   a.diff += double((k[0].diff + k[1].diff) + (k[2].diff + k[3].diff));
   a.ratio += double((k[0].ratio + k[1].ratio) + (k[2].ratio + k[3].ratio));
+  if (kVec && first + kPer <= p.n) {
+    if (p.grad) st_stream_f4(p.grad + first, make_float4(g[0], g[1], g[2], g[3]));
+    if (p.grad_ent) st_stream_f4(p.grad_ent + first, make_float4(ge[0], ge[1], ge[2], ge[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const unsigned i = token_of<kVec>(first, j);
+      if (i >= p.n) continue;
+      if (p.grad) p.grad[i] = g[j];
+      if (p.grad_ent) p.grad_ent[i] = ge[j];
+    }
+  }
 }
 
 // The warp's sums, in a fixed order; lane 0 has them all.
@@ -251,7 +318,8 @@ constexpr int kSmallThreads = 1024;
 constexpr unsigned kSmallTokens = kPer * kSmallThreads;
 constexpr int kSmallRows = 2048;
 
-__global__ void __launch_bounds__(kSmallThreads) small_kernel(const Params p) {
+template <bool kVec>
+__global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_constant__ Params p) {
   __shared__ int row_tokens[kSmallRows];
   __shared__ unsigned total, rows;
   const bool per_row = p.reduction == kSequenceMean;
@@ -260,17 +328,16 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const Params p) {
   if (threadIdx.x == 0) total = rows = 0u;
   pdl_begin();
   __syncthreads();
-  Raw raw[kPer];
-  unsigned on = 0;
-  const unsigned base = threadIdx.x / 32 * (32 * kPer) + threadIdx.x % 32;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    raw[j] = load_token(p, base + j * 32);
-    on += raw[j].on;
-    if (per_row && raw[j].on) atomicAdd(&row_tokens[raw[j].row], 1);
-  }
-  on = warp_sum_u32(on);
+  Raw r;
+  const unsigned first = first_token<kVec>(0u, kSmallThreads);
+  load_tokens<kVec>(p, first, r);
+  const unsigned on = warp_sum_u32(__popc(r.on));
   if (threadIdx.x % 32 == 0 && on > 0) atomicAdd(&total, on);
+  if (per_row) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if ((r.on >> j) & 1u) atomicAdd(&row_tokens[r.row[j]], 1);
+  }
   __syncthreads();
   if (per_row) {
     for (int b = threadIdx.x; b < p.B; b += kSmallThreads)
@@ -278,14 +345,11 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const Params p) {
     __syncthreads();
   }
   Sums a = {};
-  float w = per_row ? 0.0f : token_weight(p, total, rows, 0);
-  Terms k[kPer];
+  float w[kPer];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (per_row) w = token_weight(p, total, rows, row_tokens[raw[j].row]);
-    k[j] = take_token(p, base + j * 32, raw[j], w, float(-double(w) * p.ent_coef_d), a);
-  }
-  add_terms(a, k);
+  for (int j = 0; j < kPer; ++j)
+    w[j] = per_row || j == 0 ? token_weight(p, total, rows, per_row ? row_tokens[r.row[j]] : 0) : w[0];
+  take_tokens<kVec>(p, first, r, w, a);
   sum_block<kSmallThreads / 32>(a);
   if (threadIdx.x == 0) write_outputs(p, a, double(a.tokens), double(a.outside));
 }
@@ -343,10 +407,11 @@ __global__ void __launch_bounds__(kThreads) count_kernel(const Params p, unsigne
 // Bytes of all streams' L2 prefetch, at most: lines prefetched beyond it would be evicted before their use.
 constexpr int64_t kPrefetchBytes = 48 << 20;
 
-// A CTA takes stretches of kThreads * kPer tokens, grid-stride.  counted: count_kernel ran before; while it does, this kernel brings
-// its first stretches into L2 (their own reads wait for it).
-__global__ void __launch_bounds__(kThreads) token_kernel(const Params p, bool counted, unsigned prefetch, Ctl* ctl,
-                                                         int* counts, Sums* sums) {
+// A CTA takes stretches of kThreads * kPer tokens, grid-stride.  counted: count_kernel ran before; while it does,
+// this kernel brings its first stretches into L2 (their own reads wait for it).
+template <bool kVec>
+__global__ void __launch_bounds__(kThreads, 4) token_kernel(const __grid_constant__ Params p, bool counted,
+                                                            unsigned prefetch, Ctl* ctl, int* counts, Sums* sums) {
   constexpr unsigned kUnit = kThreads * kPer;
   const unsigned units = (p.n + kUnit - 1) / kUnit;
   if (counted && p.dense) {
@@ -364,24 +429,20 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const Params p, bool co
   const unsigned rows = counted ? ld_cg_u32(&ctl->rows) : unsigned(p.B);
   const unsigned long long tokens =
       counted ? *reinterpret_cast<volatile unsigned long long*>(&ctl->tokens) : (unsigned long long)(p.n);
-  float w = token_weight(p, tokens, rows, p.T);
-  float w_ent = float(-double(w) * p.ent_coef_d);
+  float w[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) w[j] = j == 0 ? token_weight(p, tokens, rows, p.T) : w[0];
   Sums a = {};
   for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
-    const unsigned base = u * kUnit + threadIdx.x / 32 * (32 * kPer) + threadIdx.x % 32;
-    Raw raw[kPer];
-    Terms k[kPer];
+    const unsigned first = first_token<kVec>(u, kThreads);
+    Raw r;
+    load_tokens<kVec>(p, first, r);
+    if (per_row && counted) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) raw[j] = load_token(p, base + j * 32);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (per_row && counted) {
-        w = token_weight(p, tokens, rows, raw[j].on ? counts[raw[j].row] : 1);
-        w_ent = float(-double(w) * p.ent_coef_d);
-      }
-      k[j] = take_token(p, base + j * 32, raw[j], w, w_ent, a);
+      for (int j = 0; j < kPer; ++j)
+        w[j] = kVec && j > 0 && r.row[j] == r.row[j - 1] ? w[j - 1] : token_weight(p, tokens, rows, counts[r.row[j]]);
     }
-    add_terms(a, k);
+    take_tokens<kVec>(p, first, r, w, a);
   }
   sum_block<kThreads / 32>(a);
   if (threadIdx.x == 0) sums[blockIdx.x] = a;
@@ -452,10 +513,18 @@ inline int run(const float* cur, const float* old, const float* adv, const float
   p.log_high = make_pair_of(log1p(clip_high)), p.log_low = make_pair_of(log1p(-clip_low));
   p.log_dual = make_pair_of(dual_clip > 0.0 ? log(dual_clip) : double(NAN));  // NaN: no difference is it
   p.high = float(1.0 + clip_high), p.low = float(1.0 - clip_low), p.dual = float(dual_clip);
-  p.kl_coef = float(kl_coef), p.kl_form = kl_form, p.reduction = reduction;
+  p.kl_coef = float(kl_coef), p.ent_coef = float(ent_coef), p.kl_form = kl_form, p.reduction = reduction;
   p.scale = scale, p.kl_coef_d = kl_coef, p.ent_coef_d = ent_coef;
   p.grad = grad, p.grad_ent = grad_ent, p.out = out;
-  if (need == 0) return launch_pdl(small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, p);
+  const auto aligned = [&](const void* q, int64_t s) {
+    return q == nullptr || (aligned16(q) && (p.dense || (T % kPer == 0 && s % kPer == 0)));
+  };
+  p.vec = aligned(cur, p.cur_s) && aligned(old, p.old_s) && (p.adv_rows || aligned(adv, p.adv_s)) &&
+          aligned(ref, p.ref_s) && aligned(ent, p.ent_s) && aligned(grad, T) && aligned(grad_ent, T) &&
+          (mask == nullptr || (reinterpret_cast<uintptr_t>(mask) % kPer == 0 &&
+                               (p.dense || (T % kPer == 0 && p.mask_s % kPer == 0))));
+  if (need == 0)
+    return launch_pdl(p.vec ? small_kernel<true> : small_kernel<false>, dim3(1), dim3(kSmallThreads), 0, stream, p);
 
   char* w = static_cast<char*>(ws);
   Ctl* ctl = reinterpret_cast<Ctl*>(w);
@@ -471,13 +540,13 @@ inline int run(const float* cur, const float* old, const float* adv, const float
     if (st != kOk) return st;
   }
   const int64_t units = (n + kThreads * kPer - 1) / (kThreads * kPer);
-  int64_t ctas = int64_t(sm_count()) * resident_ctas_per_sm(token_kernel, kThreads, 0);
+  int64_t ctas = int64_t(sm_count()) * resident_ctas_per_sm(token_kernel<true>, kThreads, 0);
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   if (ctas > units) ctas = units;
   const int streams = 2 + !p.adv_rows + (ref != nullptr) + (ent != nullptr);
   const int64_t unit_bytes = int64_t(kThreads) * kPer * 4 * streams;
   const unsigned prefetch = unsigned(kPrefetchBytes / (unit_bytes * ctas));
-  return launch_pdl(token_kernel, dim3(unsigned(ctas)), dim3(kThreads), 0, stream, p, counted, prefetch, ctl, counts,
+  return launch_pdl(p.vec ? token_kernel<true> : token_kernel<false>, dim3(unsigned(ctas)), dim3(kThreads), 0, stream, p, counted, prefetch, ctl, counts,
                     sums);
 }
 

@@ -21,7 +21,6 @@ namespace pref {
 
 enum Form : int { kSigmoid = 0, kHinge = 1, kIpo = 2 };
 
-constexpr int kThreads = 256;
 constexpr int kOutputs = 3;
 
 struct Side {
@@ -30,6 +29,7 @@ struct Side {
   int64_t lp_s, ref_s, mask_s;  // row strides
   int T;
   float *reward, *grad;
+  bool vec_in, vec_out;  // rows of lp, ref and mask (of grad) take vectors of four tokens
 };
 
 struct Params {
@@ -73,45 +73,98 @@ struct Ctl {
   unsigned done;
 };
 
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kPer = 8;  // tokens of a lane in flight: log-prob and reference of each
+constexpr int kVecs = 2;      // vectors of four tokens of a lane in flight, log-probs and references
+constexpr int kPer = 4 * kVecs;
 
-// This CTA's stretch of answer b: tokens [t0, t1), lanes on consecutive ones.
+__device__ __forceinline__ double gap_of(float x, float r, bool on) {
+  return on ? double(x) - double(r) : 0.0;
+}
+
+// This CTA's stretch of answer b: tokens [t0, t1), t0 a multiple of 4.  What masked-out tokens hold is read with
+// the others and not used.
+template <int kThreads>
 __device__ __forceinline__ Part sum_stretch(const Side& d, int64_t b, int t0, int t1) {
   const float *lp = d.lp + b * d.lp_s, *ref = d.ref == nullptr ? nullptr : d.ref + b * d.ref_s;
   const uint8_t* m = d.mask == nullptr ? nullptr : d.mask + b * d.mask_s;
   double s = 0.0;
   unsigned n = 0;
+  if (d.vec_in) {
+    const int t1v = t1 & ~3;
+    for (int t = t0 + int(threadIdx.x) * 4; t < t1v; t += kPer * kThreads) {
+      float4 x[kVecs], r[kVecs];
+      uint32_t on[kVecs];
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int at = t + k * 4 * kThreads;
+        const bool in = at < t1v;
+        x[k] = in ? ld_stream_f4(lp + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        r[k] = in && ref != nullptr ? ld_stream_f4(ref + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        on[k] = !in ? 0u : m == nullptr ? 0x01010101u : __vminu4(*reinterpret_cast<const uint32_t*>(m + at), 0x01010101u);
+      }
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        s += (gap_of(x[k].x, r[k].x, on[k] & 0xffu) + gap_of(x[k].y, r[k].y, on[k] & 0xff00u)) +
+             (gap_of(x[k].z, r[k].z, on[k] & 0xff0000u) + gap_of(x[k].w, r[k].w, on[k] & 0xff000000u));
+        n += __popc(on[k]);
+      }
+    }
+    t0 = t1v;  // at most three tokens are left
+  }
   for (int t = t0 + int(threadIdx.x); t < t1; t += kPer * kThreads) {
     float x[kPer], r[kPer];
     bool on[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int at = t + k * kThreads;
-      on[k] = at < t1 && (m == nullptr || m[at] != 0);
-      x[k] = at < t1 ? lp[at] : 0.0f;
-      r[k] = ref != nullptr && at < t1 ? ref[at] : 0.0f;
+      const bool in = at < t1;
+      x[k] = in ? ld_stream_f1(lp + at) : 0.0f;
+      r[k] = in && ref != nullptr ? ld_stream_f1(ref + at) : 0.0f;
+      on[k] = in && (m == nullptr || m[at] != 0);
     }
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      if (!on[k]) continue;
-      s += double(x[k]) - double(r[k]);
-      ++n;
+      s += gap_of(x[k], r[k], on[k]);
+      n += on[k];
     }
   }
   return Part{s, n};
 }
 
+template <int kThreads>
 __device__ __forceinline__ void write_stretch(const Side& d, int64_t b, int t0, int t1, float slope) {
   if (d.grad == nullptr) return;
   const uint8_t* m = d.mask == nullptr ? nullptr : d.mask + b * d.mask_s;
   float* g = d.grad + b * d.T;
+  if (d.vec_in && d.vec_out) {
+    for (int t = t0 + int(threadIdx.x) * 4; t < t1; t += kPer * kThreads) {  // T is a multiple of 4
+      uint32_t on[kVecs];
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int at = t + k * 4 * kThreads;
+        on[k] = at < t1 && m != nullptr ? *reinterpret_cast<const uint32_t*>(m + at) : ~0u;
+      }
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int at = t + k * 4 * kThreads;
+        if (at < t1)
+          st_stream_f4(g + at, make_float4(on[k] & 0xffu ? slope : 0.0f, on[k] & 0xff00u ? slope : 0.0f,
+                                           on[k] & 0xff0000u ? slope : 0.0f, on[k] & 0xff000000u ? slope : 0.0f));
+      }
+    }
+    return;
+  }
   for (int t = t0 + int(threadIdx.x); t < t1; t += kPer * kThreads) {
+    bool on[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int at = t + k * kThreads;
-      if (at < t1) g[at] = m == nullptr || m[at] != 0 ? slope : 0.0f;
+      on[k] = at < t1 && (m == nullptr || m[at] != 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int at = t + k * kThreads;
+      if (at < t1) g[at] = on[k] ? slope : 0.0f;
     }
   }
 }
@@ -119,7 +172,9 @@ __device__ __forceinline__ void write_stretch(const Side& d, int64_t b, int t0, 
 // A cluster of `parts` CTAs per pair, each on a stretch of both answers: the CTAs exchange their sums through
 // shared memory, every one forms the pair's slope from all of them in the same order and writes its
 // stretch of the gradients.  The last CTA of the grid adds up the pairs in their order.
-__global__ void __launch_bounds__(kThreads) pair_kernel(const Params p, unsigned parts, Ctl* ctl, PairOut* pairs) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ Params p, unsigned parts, Ctl* ctl, PairOut* pairs) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ Part warp_part[2][kWarps];
   __shared__ Part cta_part[2][kMaxCluster];
   __shared__ float slope[2];
@@ -133,10 +188,10 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const Params p, unsigned
   int t0[2], t1[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int per = int((unsigned(p.side[k].T) + parts - 1) / parts);
+    const int per = int((unsigned(p.side[k].T) + 4 * parts - 1) / (4 * parts)) * 4;
     t0[k] = int(min(int64_t(p.side[k].T), int64_t(per) * part));
     t1[k] = int(min(int64_t(p.side[k].T), int64_t(t0[k]) + per));
-    Part a = sum_stretch(p.side[k], b, t0[k], t1[k]);
+    Part a = sum_stretch<kThreads>(p.side[k], b, t0[k], t1[k]);
     a.s = warp_sum(a.s);
     a.n = warp_sum_u32(a.n);
     if (lane == 0) warp_part[k][w] = a;
@@ -188,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const Params p, unsigned
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) write_stretch(p.side[k], b, t0[k], t1[k], slope[k]);
+  for (int k = 0; k < 2; ++k) write_stretch<kThreads>(p.side[k], b, t0[k], t1[k], slope[k]);
   if (!elect_last_cta(&ctl->done)) return;
   double a[3] = {0.0, 0.0, 0.0};
   for (int i = threadIdx.x; i < p.B; i += kThreads) {
@@ -210,6 +265,11 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const Params p, unsigned
     }
   }
 }
+
+// Threads of a CTA: with few pairs (the largest cluster each) a CTA has an SM for itself, and only more threads
+// keep more of its stretch in flight.
+constexpr int kPairThreads = 256;
+constexpr int kLongThreads = 1024;
 
 inline int64_t workspace_bytes(int32_t B) { return int64_t(256 + align256(size_t(B) * sizeof(PairOut))); }
 
@@ -239,20 +299,28 @@ inline int run(const float* chosen, const float* rejected, const float* ref_chos
       reward_rejected == nullptr)
     return kInvalidArgument;
   // Token indexes run in ints, up to a round of the CTA past the end.
-  if (Tc > 0x7fffffff - kPer * kThreads || Tr > 0x7fffffff - kPer * kThreads) return kUnsupported;
+  if (Tc > 0x7fffffff - 2 * kPer * kLongThreads || Tr > 0x7fffffff - 2 * kPer * kLongThreads) return kUnsupported;
   if (ws == nullptr || ws_bytes < workspace_bytes(B)) return kWorkspaceTooSmall;
   if (!aligned16(ws)) return kInvalidArgument;
   Params p;
   p.side[0] = Side{chosen, ref_chosen, chosen_mask, strides[0], strides[2], strides[4], Tc, reward_chosen, grad_chosen};
   p.side[1] =
       Side{rejected, ref_rejected, rejected_mask, strides[1], strides[3], strides[5], Tr, reward_rejected, grad_rejected};
+  for (Side& d : p.side) {
+    const auto rows = [](const void* q, int64_t s, int bytes) {
+      return q == nullptr || (reinterpret_cast<uintptr_t>(q) % bytes == 0 && s % 4 == 0);
+    };
+    d.vec_in = rows(d.lp, d.lp_s, 16) && rows(d.ref, d.ref_s, 16) && rows(d.mask, d.mask_s, 4);
+    d.vec_out = rows(d.grad, d.T, 16);
+  }
   p.B = B, p.beta = beta, p.smoothing = smoothing, p.margin = margin, p.form = form, p.average = average != 0;
   p.out = out;
   const unsigned parts = cluster_of(B, int64_t(Tc) + Tr);
   if (int64_t(B) * parts > 0x7fffffff) return kUnsupported;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(B) * parts);
-  cfg.blockDim = dim3(kThreads);
+  const bool wide = parts == unsigned(kMaxCluster);
+  cfg.blockDim = dim3(wide ? kLongThreads : kPairThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -262,7 +330,7 @@ inline int run(const float* chosen, const float* rejected, const float* ref_chos
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = parts > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, pair_kernel, p, parts, static_cast<Ctl*>(ws),
+  return cudaLaunchKernelEx(&cfg, wide ? pair_kernel<kLongThreads> : pair_kernel<kPairThreads>, p, parts, static_cast<Ctl*>(ws),
                             reinterpret_cast<PairOut*>(static_cast<char*>(ws) + 256)) == cudaSuccess
              ? kOk
              : kCudaError;
