@@ -8,6 +8,7 @@ Every function raises on a non-CUDA tensor, a wrong dtype or a non-contiguous in
 non-zero native status; there is no CPU fallback.
 """
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -598,8 +599,15 @@ RECURRENCE_FORMS = {"decay": 0, "sigmoid": 1}
 _I32_MAX = 2**31 - 1
 
 
+_current_device = torch.cuda.current_device
+# The handle of a device's current stream, without a Stream object around it where torch offers that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+@functools.lru_cache(maxsize=1024)
 def _strides(*values):
-    """A host array of element strides for the C ABI."""
+    """A host array of element strides for the C ABI, which only reads it."""
     return (ctypes.c_int64 * len(values))(*values)
 
 
@@ -608,18 +616,36 @@ def _needs(ctx, k):
     return k < len(ctx.needs_input_grad) and ctx.needs_input_grad[k]
 
 
-def _on_device(device):
-    """Context in which `device` is the current one (a launch goes to the current device)."""
-    return torch.cuda.device(device)
+def _run(what, fn, index, *args):
+    """A stream form on the current stream of device `index`, which is made the current device for it (a
+    launch goes to the current device)."""
+    if _current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _native.check(status, what)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def _scratch(op, nbytes, device):
     """workspace(), except that a call being captured into a CUDA graph gets scratch of its own (its
     zero-fill is captured with it): graphs may be replayed at the same time as one another and as
     calls outside them."""
-    if torch.cuda.is_current_stream_capturing():
+    index = device.index
+    if _current_device() == index:
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(index):
+            capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
         return torch.zeros(max(int(nbytes), 16), dtype=torch.uint8, device=device)
-    return workspace(op, nbytes, device)
+    buf = _WS.get((op, index, _raw_stream(index)))
+    return buf if buf is not None and buf.numel() >= nbytes else workspace(op, nbytes, device)
 
 
 def _float_tensor(t, name, device=None, dtype=None, dims=None):
@@ -637,31 +663,31 @@ def _float_tensor(t, name, device=None, dtype=None, dims=None):
         raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
     if dims is not None and t.dim() != dims:
         raise ValueError(f"{name}: expected {dims} dimensions, got {t.dim()}")
-    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
         raise ValueError(f"{name}: expected a contiguous last dimension")
-    if any(n > _I32_MAX for n in t.shape):
+    if t.numel() > _I32_MAX and any(n > _I32_MAX for n in t.shape):
         raise ValueError(f"{name}: a dimension is larger than 2^31 - 1")
     return t
 
 
 def _bth(gate, x, form):
-    """Checks gate and x [B, T, H] of a recurrence: (device, dtype code, form code, B, T, H)."""
+    """Checks gate and x [B, T, H] of a recurrence: (device, dtype code, form code, shape)."""
     if form not in RECURRENCE_FORMS:
         raise ValueError(f"form must be one of {sorted(RECURRENCE_FORMS)}, got {form!r}")
     _float_tensor(x, "x", dims=3)
-    _float_tensor(gate, "gate", x.device, x.dtype, 3)
-    if gate.shape != x.shape:
+    device, shape = x.device, x.shape
+    _float_tensor(gate, "gate", device, x.dtype, 3)
+    if gate.shape != shape:
         raise ValueError("gate and x must have the same shape (B, T, H)")
-    B, T, H = x.shape
-    return x.device, DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form], B, T, H
+    return device, DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form], shape
 
 
 def _like_bth(x):
     """An output of x's shape and dtype: dense, time first in memory when x is."""
     B, T, H = x.shape
     if B > 1 and T > 1 and x.stride(0) < x.stride(1):
-        return torch.empty((T, B, H), dtype=x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty((B, T, H), dtype=x.dtype, device=x.device)
+        return x.new_empty((T, B, H)).transpose(0, 1)
+    return x.new_empty((B, T, H))
 
 
 def _writable(t, like, name):
@@ -698,29 +724,38 @@ def _reset_arg(reset, B, T, device):
     return reset
 
 
-def _bt_strides(*tensors):
-    out = []
-    for t in tensors:
-        out += [0, 0] if t is None else [t.stride(0), t.stride(1)]
-    return _strides(*out)
+def _bt(t):
+    return (0, 0) if t is None else t.stride()[:2]
+
+
+@functools.lru_cache(maxsize=256)
+def _recurrence_sizes(B, T, H):
+    """(fp32 values of the checkpoints, bytes of the workspace)."""
+    lib = _lib()
+    return (lib.b200_linear_recurrence_checkpoint_bytes(B, T, H) // 4,
+            lib.b200_linear_recurrence_workspace_bytes(B, T, H))
+
+
+def _recurrence_scratch(nbytes, device):
+    """(workspace, its address, its bytes); sequences of one tile need none."""
+    if nbytes == 0:
+        return None, None, 0
+    ws = _scratch("linear_recurrence", nbytes, device)
+    return ws, ws.data_ptr(), ws.numel()
 
 
 def _recurrence_forward(gate, x, state, reset, form, out, train):
-    dev, dt, fm, B, T, H = _bth(gate, x, form)
+    dev, dt, fm, (B, T, H) = _bth(gate, x, form)
     state = _state_arg(state, "state", B, H, dev)
     reset = _reset_arg(reset, B, T, dev)
     h = _like_bth(x) if out is None else _writable(out, x, "out")
-    lib = _lib()
-    with _on_device(dev):
-        final = torch.empty((B, H), dtype=torch.float32, device=dev)
-        ckpt = None
-        if train:
-            n = lib.b200_linear_recurrence_checkpoint_bytes(B, T, H) // 4
-            ckpt = torch.empty(n, dtype=torch.float32, device=dev)
-        ws = _scratch("linear_recurrence", lib.b200_linear_recurrence_workspace_bytes(B, T, H), dev)
-        _native.check(lib.b200_linear_recurrence_async(
-            _ptr(gate), _ptr(x), dt, fm, _bt_strides(gate, x, h, reset), _ptr(state), _ptr(reset), B, T, H, _ptr(h),
-            _ptr(final), _ptr(ckpt), _ptr(ws), ws.numel(), _stream(dev)), "linear_recurrence")
+    n_ckpt, n_ws = _recurrence_sizes(B, T, H)
+    final = torch.empty((B, H), dtype=torch.float32, device=dev)
+    ckpt = torch.empty(n_ckpt, dtype=torch.float32, device=dev) if train else None
+    ws, ws_at, ws_bytes = _recurrence_scratch(n_ws, dev)
+    _run("linear_recurrence", _lib().b200_linear_recurrence_async, dev.index, gate.data_ptr(), x.data_ptr(), dt, fm,
+         _strides(*_bt(gate), *_bt(x), *_bt(h), *_bt(reset)), _address(state), _address(reset), B, T, H, h.data_ptr(),
+         final.data_ptr(), _address(ckpt), ws_at, ws_bytes)
     return h, final, ckpt
 
 
@@ -730,8 +765,8 @@ def linear_recurrence(gate, x, state=None, reset=None, form="decay", out=None):
 
     gate and x: fp32, bf16 or fp16 with a contiguous channel axis and any other strides (halves of one
     projection, time-first layouts).  state: fp32 [B, H] before the first step (None: 0).  reset: bool
-    [B, T], True where a step starts a new document (the state before it is dropped).  Returns (h of x's
-    dtype, the fp32 state [B, H] after the last step)."""
+    [B, T], True where a step starts a new document (the state before it is dropped).  out: x's shape and
+    dtype, in memory of its own.  Returns (h of x's dtype, the fp32 state [B, H] after the last step)."""
     h, final, _ = _recurrence_forward(gate, x, state, reset, form, out, False)
     return h, final
 
@@ -745,24 +780,23 @@ def linear_recurrence_train(gate, x, state=None, reset=None, form="decay"):
 def linear_recurrence_backward(gate, x, checkpoints, grad_h, grad_final=None, reset=None, form="decay"):
     """Gradients of linear_recurrence: (grad_gate, grad_x, grad_state) for grad_h [B, T, H] (x's dtype) and
     grad_final (fp32 [B, H] or None)."""
-    dev, dt, fm, B, T, H = _bth(gate, x, form)
+    dev, dt, fm, (B, T, H) = _bth(gate, x, form)
     _float_tensor(grad_h, "grad_h", dev, x.dtype, 3)
     if grad_h.shape != x.shape:
         raise ValueError("grad_h must have x's shape")
     grad_final = _state_arg(grad_final, "grad_final", B, H, dev)
     reset = _reset_arg(reset, B, T, dev)
-    lib = _lib()
+    n_ckpt, n_ws = _recurrence_sizes(B, T, H)
     _need(checkpoints, "checkpoints", torch.float32, dev)
-    if checkpoints.numel() * 4 != lib.b200_linear_recurrence_checkpoint_bytes(B, T, H):
+    if checkpoints.numel() != n_ckpt:
         raise ValueError("checkpoints do not belong to inputs of this shape")
-    with _on_device(dev):
-        gg, gx = _like_bth(gate), _like_bth(x)
-        gs = torch.empty((B, H), dtype=torch.float32, device=dev)
-        ws = _scratch("linear_recurrence", lib.b200_linear_recurrence_workspace_bytes(B, T, H), dev)
-        _native.check(lib.b200_linear_recurrence_backward_async(
-            _ptr(gate), _ptr(x), dt, fm, _bt_strides(gate, x, grad_h, gg, gx, reset), _ptr(checkpoints), _ptr(reset),
-            _ptr(grad_h), _ptr(grad_final), B, T, H, _ptr(gg), _ptr(gx), _ptr(gs), _ptr(ws), ws.numel(),
-            _stream(dev)), "linear_recurrence_backward")
+    gg, gx = _like_bth(gate), _like_bth(x)
+    gs = torch.empty((B, H), dtype=torch.float32, device=dev)
+    ws, ws_at, ws_bytes = _recurrence_scratch(n_ws, dev)
+    _run("linear_recurrence_backward", _lib().b200_linear_recurrence_backward_async, dev.index, gate.data_ptr(),
+         x.data_ptr(), dt, fm, _strides(*_bt(gate), *_bt(x), *_bt(grad_h), *_bt(gg), *_bt(gx), *_bt(reset)),
+         checkpoints.data_ptr(), _address(reset), grad_h.data_ptr(), _address(grad_final), B, T, H, gg.data_ptr(),
+         gx.data_ptr(), gs.data_ptr(), ws_at, ws_bytes)
     return gg, gx, gs
 
 
@@ -774,14 +808,17 @@ def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, s
     if form not in RECURRENCE_FORMS:
         raise ValueError(f"form must be one of {sorted(RECURRENCE_FORMS)}, got {form!r}")
     _float_tensor(x, "x", dims=2)
-    dev = x.device
+    dev, shape = x.device, x.shape
     _float_tensor(gate, "gate", dev, x.dtype, 2)
-    if gate.shape != x.shape:
+    if gate.shape != shape:
         raise ValueError("gate and x must have the same shape (B, H)")
-    B, H = x.shape
+    B, H = shape
     _need(state, "state", torch.float32, dev)
     if state.dim() != 2 or state.shape[1] != H:
         raise ValueError(f"state must be (slots, {H})")
+    S = state.shape[0]
+    if S > _I32_MAX:
+        raise ValueError("state has more than 2^31 - 1 rows")
     if state_out is None:
         state_out = state
     else:
@@ -789,18 +826,16 @@ def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, s
         if state_out.shape != state.shape:
             raise ValueError("state_out must have state's shape")
     if slots is None:
-        if state.shape[0] < B:
+        if S < B:
             raise ValueError("state has fewer rows than x and no slots are given")
     else:
         _need(slots, "slots", torch.int32, dev)
         if slots.shape != (B,):
             raise ValueError(f"slots must be ({B},)")
-    h = torch.empty((B, H), dtype=x.dtype, device=dev) if out is None else _writable(out, x, "out")
-    with _on_device(dev):
-        _native.check(_lib().b200_linear_recurrence_step_async(
-            _ptr(gate), _ptr(x), DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form],
-            _strides(gate.stride(0), x.stride(0), h.stride(0)), _ptr(state), _ptr(state_out), _ptr(slots),
-            state.shape[0], B, H, _ptr(h), _stream(dev)), "linear_recurrence_step")
+    h = x.new_empty((B, H)) if out is None else _writable(out, x, "out")
+    _run("linear_recurrence_step", _lib().b200_linear_recurrence_step_async, dev.index, gate.data_ptr(), x.data_ptr(),
+         DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form], _strides(gate.stride(0), x.stride(0), h.stride(0)),
+         state.data_ptr(), state_out.data_ptr(), _address(slots), S, B, H, h.data_ptr())
     return h
 
 
@@ -832,26 +867,27 @@ class LinearRecurrenceFunction(torch.autograd.Function):
 def _token_args(logits, token):
     """(device, dtype code, B, T, V, strides) of logits [..., V] and token [...] with 1 or 2 leading axes."""
     _float_tensor(logits, "logits")
-    if logits.dim() not in (2, 3):
+    shape, device = logits.shape, logits.device
+    if len(shape) not in (2, 3):
         raise ValueError("logits must be (N, V) or (B, T, V)")
     if not isinstance(token, torch.Tensor) or token.dtype != torch.int64:
         raise ValueError("token: expected an int64 tensor")
-    if token.device != logits.device:
-        raise ValueError(f"token: on {token.device}, expected {logits.device}")
-    if token.shape != logits.shape[:-1]:
+    if token.device != device:
+        raise ValueError(f"token: on {token.device}, expected {device}")
+    if token.shape != shape[:-1]:
         raise ValueError("token must have the shape of logits without the last axis")
-    V = logits.shape[-1]
+    V = shape[-1]
     if V < 1:
         raise ValueError("logits: the vocabulary is empty")
-    if logits.dim() == 2:
-        B, T = 1, logits.shape[0]
+    if len(shape) == 2:
+        B, T = 1, shape[0]
         st = _strides(0, logits.stride(0), 0, token.stride(0))
     else:
-        B, T = logits.shape[:2]
+        B, T = shape[:2]
         st = _strides(logits.stride(0), logits.stride(1), token.stride(0), token.stride(1))
     if B * T > _I32_MAX:
         raise ValueError("logits: more than 2^31 - 1 rows")
-    return logits.device, DTYPE_CODES[logits.dtype], B, T, V, st
+    return device, DTYPE_CODES[logits.dtype], B, T, V, st
 
 
 def _check_over(out, logits):
@@ -874,13 +910,11 @@ def _temperature(temperature):
 def _token_logprob(logits, token, temperature, entropy, train):
     dev, dt, B, T, V, st = _token_args(logits, token)
     temperature = _temperature(temperature)
-    with _on_device(dev):
-        lp = torch.empty(token.shape, dtype=torch.float32, device=dev)
-        ent = torch.empty(token.shape, dtype=torch.float32, device=dev) if entropy else None
-        stats = torch.empty((*token.shape, 3), dtype=torch.float32, device=dev) if train else None
-        _native.check(_lib().b200_token_logprob_async(_ptr(logits), dt, st, _ptr(token), B, T, V, temperature,
-                                                      _ptr(lp), _ptr(ent), _ptr(stats), _stream(dev)),
-                      "token_logprob")
+    lp = torch.empty(token.shape, dtype=torch.float32, device=dev)
+    ent = torch.empty(token.shape, dtype=torch.float32, device=dev) if entropy else None
+    stats = torch.empty((*token.shape, 3), dtype=torch.float32, device=dev) if train else None
+    _run("token_logprob", _lib().b200_token_logprob_async, dev.index, logits.data_ptr(), dt, st, token.data_ptr(), B, T,
+         V, temperature, lp.data_ptr(), _address(ent), _address(stats))
     return lp, ent, stats
 
 
@@ -914,17 +948,16 @@ def token_logprob_backward(logits, token, stats, grad_log_prob, grad_entropy=Non
         _need(t, nm, torch.float32, dev)
         if t.shape != shape:
             raise ValueError(f"{nm} must be {tuple(shape)}")
-    with _on_device(dev):
-        if out is None:
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        else:
-            _need(out, "out", logits.dtype, dev)
-            if out.shape != logits.shape:
-                raise ValueError("out must have logits' shape")
-            _check_over(out, logits)
-        _native.check(_lib().b200_token_logprob_backward_async(
-            _ptr(logits), dt, st, _ptr(token), _ptr(stats), _ptr(grad_log_prob), _ptr(grad_entropy), B, T, V,
-            temperature, _ptr(out), _stream(dev)), "token_logprob_backward")
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    else:
+        _need(out, "out", logits.dtype, dev)
+        if out.shape != logits.shape:
+            raise ValueError("out must have logits' shape")
+        _check_over(out, logits)
+    _run("token_logprob_backward", _lib().b200_token_logprob_backward_async, dev.index, logits.data_ptr(), dt, st,
+         token.data_ptr(), stats.data_ptr(), grad_log_prob.data_ptr(), _address(grad_entropy), B, T, V, temperature,
+         out.data_ptr())
     return out
 
 
@@ -977,26 +1010,10 @@ def _number(v, name):
     return v
 
 
-def _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy, clip_low, clip_high, dual_clip,
-                 kl_coef, kl_form, entropy_coef, reduction, scale, want_grad, want_grad_entropy):
-    _float_tensor(log_prob, "log_prob", dtype=torch.float32, dims=2)
-    dev = log_prob.device
-    B, T = log_prob.shape
-    old = log_prob if old_log_prob is None else _token_stream(old_log_prob, "old_log_prob", B, T, dev)
-    if isinstance(advantage, torch.Tensor) and advantage.dim() == 1:
-        _float_tensor(advantage.unsqueeze(1), "advantage", dev, torch.float32)
-        if advantage.shape != (B,):
-            raise ValueError(f"advantage must be ({B},) or ({B}, {T})")
-        adv_s, adv_e = advantage.stride(0), 0
-    else:
-        _token_stream(advantage, "advantage", B, T, dev)
-        adv_s, adv_e = advantage.stride(0), 1
-    if mask is not None:
-        _token_stream(mask, "mask", B, T, dev, torch.bool)
-    if ref_log_prob is not None:
-        _token_stream(ref_log_prob, "ref_log_prob", B, T, dev)
-    if entropy is not None:
-        _token_stream(entropy, "entropy", B, T, dev)
+@functools.lru_cache(maxsize=256)
+def _policy_options(clip_low, clip_high, dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale, has_ref,
+                    has_entropy):
+    """The loss's options checked, as the C ABI takes them."""
     if kl_form not in KL_FORMS:
         raise ValueError(f"kl_form must be one of {sorted(KL_FORMS)}, got {kl_form!r}")
     if reduction not in LOSS_REDUCTIONS:
@@ -1008,23 +1025,51 @@ def _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy,
     if dual_clip is not None and dual <= 1.0:
         raise ValueError("dual_clip must be larger than 1")
     kl_coef, entropy_coef = _number(kl_coef, "kl_coef"), _number(entropy_coef, "entropy_coef")
-    if kl_coef != 0.0 and ref_log_prob is None:
+    if kl_coef != 0.0 and not has_ref:
         raise ValueError("kl_coef needs ref_log_prob")
-    if entropy_coef != 0.0 and entropy is None:
+    if entropy_coef != 0.0 and not has_entropy:
         raise ValueError("entropy_coef needs entropy")
-    lib = _lib()
-    with _on_device(dev):
-        out = torch.empty(8, dtype=torch.float32, device=dev)
-        grad = torch.empty((B, T), dtype=torch.float32, device=dev) if want_grad else None
-        ge = torch.empty((B, T), dtype=torch.float32, device=dev) if want_grad_entropy else None
-        ws = _scratch("policy_loss", lib.b200_policy_loss_workspace_bytes(B, T), dev)
-        st = _strides(log_prob.stride(0), old.stride(0), adv_s, adv_e, _row_stride(ref_log_prob),
-                      _row_stride(entropy), _row_stride(mask))
-        _native.check(lib.b200_policy_loss_async(
-            _ptr(log_prob), _ptr(old), _ptr(advantage), _ptr(ref_log_prob), _ptr(entropy), _ptr(mask), st, B, T,
-            clip_low, clip_high, dual, kl_coef, KL_FORMS[kl_form], entropy_coef, LOSS_REDUCTIONS[reduction],
-            _number(scale, "scale"), _ptr(out), _ptr(grad), _ptr(ge), _ptr(ws), ws.numel(), _stream(dev)),
-            "policy_loss")
+    return (clip_low, clip_high, dual, kl_coef, KL_FORMS[kl_form], entropy_coef, LOSS_REDUCTIONS[reduction],
+            _number(scale, "scale"))
+
+
+@functools.lru_cache(maxsize=256)
+def _policy_scratch_bytes(B, T):
+    return _lib().b200_policy_loss_workspace_bytes(B, T)
+
+
+def _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy, clip_low, clip_high, dual_clip,
+                 kl_coef, kl_form, entropy_coef, reduction, scale, want_grad, want_grad_entropy):
+    _float_tensor(log_prob, "log_prob", dtype=torch.float32, dims=2)
+    dev = log_prob.device
+    B, T = log_prob.shape
+    old = log_prob if old_log_prob is None else _token_stream(old_log_prob, "old_log_prob", B, T, dev)
+    if isinstance(advantage, torch.Tensor) and advantage.dim() == 1:
+        _float_tensor(advantage.unsqueeze(1), "advantage", dev, torch.float32)
+        if advantage.shape != (B,):
+            raise ValueError(f"advantage must be ({B},) or ({B}, {T})")
+        adv_e = 0
+    else:
+        _token_stream(advantage, "advantage", B, T, dev)
+        adv_e = 1
+    if mask is not None:
+        _token_stream(mask, "mask", B, T, dev, torch.bool)
+    if ref_log_prob is not None:
+        _token_stream(ref_log_prob, "ref_log_prob", B, T, dev)
+    if entropy is not None:
+        _token_stream(entropy, "entropy", B, T, dev)
+    options = _policy_options(clip_low, clip_high, dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale,
+                              ref_log_prob is not None, entropy is not None)
+    out = torch.empty(8, dtype=torch.float32, device=dev)
+    grad = torch.empty((B, T), dtype=torch.float32, device=dev) if want_grad else None
+    ge = torch.empty((B, T), dtype=torch.float32, device=dev) if want_grad_entropy else None
+    n_ws = _policy_scratch_bytes(B, T)
+    ws = _scratch("policy_loss", n_ws, dev) if n_ws else None
+    _run("policy_loss", _lib().b200_policy_loss_async, dev.index, log_prob.data_ptr(), old.data_ptr(),
+         advantage.data_ptr(), _address(ref_log_prob), _address(entropy), _address(mask),
+         _strides(log_prob.stride(0), old.stride(0), advantage.stride(0), adv_e, _row_stride(ref_log_prob),
+                  _row_stride(entropy), _row_stride(mask)),
+         B, T, *options, out.data_ptr(), _address(grad), _address(ge), _address(ws), ws.numel() if n_ws else 0)
     return out, grad, ge
 
 
@@ -1081,6 +1126,25 @@ class PolicyLossFunction(torch.autograd.Function):
                 None, None)
 
 
+@functools.lru_cache(maxsize=256)
+def _preference_options(beta, form, label_smoothing, margin):
+    """The loss's options checked, as the C ABI takes them."""
+    if form not in PREFERENCE_FORMS:
+        raise ValueError(f"form must be one of {sorted(PREFERENCE_FORMS)}, got {form!r}")
+    beta, margin = _number(beta, "beta"), _number(margin, "margin")
+    label_smoothing = _number(label_smoothing, "label_smoothing")
+    if beta <= 0.0:
+        raise ValueError("beta must be positive")
+    if not 0.0 <= label_smoothing <= 0.5 or (label_smoothing and form != "sigmoid"):
+        raise ValueError("label_smoothing must be in [0, 0.5], and 0 unless form is 'sigmoid'")
+    return beta, PREFERENCE_FORMS[form], label_smoothing, margin
+
+
+@functools.lru_cache(maxsize=256)
+def _preference_scratch_bytes(B):
+    return _lib().b200_preference_loss_workspace_bytes(B)
+
+
 def _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, form,
                      label_smoothing, margin, average, want_chosen, want_rejected):
     _float_tensor(chosen, "chosen", dtype=torch.float32, dims=2)
@@ -1091,33 +1155,26 @@ def _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, re
         raise ValueError("chosen and rejected must have the same number of rows")
     if (ref_chosen is None) != (ref_rejected is None):
         raise ValueError("ref_chosen and ref_rejected go together")
-    for t, nm, T, ty in ((ref_chosen, "ref_chosen", Tc, torch.float32),
-                         (ref_rejected, "ref_rejected", Tr, torch.float32),
-                         (chosen_mask, "chosen_mask", Tc, torch.bool), (rejected_mask, "rejected_mask", Tr, torch.bool)):
-        if t is not None:
-            _token_stream(t, nm, B, T, dev, ty)
-    if form not in PREFERENCE_FORMS:
-        raise ValueError(f"form must be one of {sorted(PREFERENCE_FORMS)}, got {form!r}")
-    beta, margin = _number(beta, "beta"), _number(margin, "margin")
-    label_smoothing = _number(label_smoothing, "label_smoothing")
-    if beta <= 0.0:
-        raise ValueError("beta must be positive")
-    if not 0.0 <= label_smoothing <= 0.5 or (label_smoothing and form != "sigmoid"):
-        raise ValueError("label_smoothing must be in [0, 0.5], and 0 unless form is 'sigmoid'")
-    lib = _lib()
-    with _on_device(dev):
-        out = torch.empty(3, dtype=torch.float32, device=dev)
-        rc, rr = (torch.empty(B, dtype=torch.float32, device=dev) for _ in range(2))
-        gc = torch.empty((B, Tc), dtype=torch.float32, device=dev) if want_chosen else None
-        gr = torch.empty((B, Tr), dtype=torch.float32, device=dev) if want_rejected else None
-        ws = _scratch("preference_loss", lib.b200_preference_loss_workspace_bytes(B), dev)
-        st = _strides(*(_row_stride(t) for t in (chosen, rejected, ref_chosen, ref_rejected, chosen_mask,
-                                                 rejected_mask)))
-        _native.check(lib.b200_preference_loss_async(
-            _ptr(chosen), _ptr(rejected), _ptr(ref_chosen), _ptr(ref_rejected), _ptr(chosen_mask),
-            _ptr(rejected_mask), st, B, Tc, Tr, beta, PREFERENCE_FORMS[form], label_smoothing, margin,
-            int(bool(average)), _ptr(out), _ptr(rc), _ptr(rr), _ptr(gc), _ptr(gr), _ptr(ws), ws.numel(),
-            _stream(dev)), "preference_loss")
+    if ref_chosen is not None:
+        _token_stream(ref_chosen, "ref_chosen", B, Tc, dev)
+        _token_stream(ref_rejected, "ref_rejected", B, Tr, dev)
+    if chosen_mask is not None:
+        _token_stream(chosen_mask, "chosen_mask", B, Tc, dev, torch.bool)
+    if rejected_mask is not None:
+        _token_stream(rejected_mask, "rejected_mask", B, Tr, dev, torch.bool)
+    options = _preference_options(beta, form, label_smoothing, margin)
+    out = torch.empty(3, dtype=torch.float32, device=dev)
+    rc = torch.empty(B, dtype=torch.float32, device=dev)
+    rr = torch.empty(B, dtype=torch.float32, device=dev)
+    gc = torch.empty((B, Tc), dtype=torch.float32, device=dev) if want_chosen else None
+    gr = torch.empty((B, Tr), dtype=torch.float32, device=dev) if want_rejected else None
+    ws = _scratch("preference_loss", _preference_scratch_bytes(B), dev)
+    _run("preference_loss", _lib().b200_preference_loss_async, dev.index, chosen.data_ptr(), rejected.data_ptr(),
+         _address(ref_chosen), _address(ref_rejected), _address(chosen_mask), _address(rejected_mask),
+         _strides(chosen.stride(0), rejected.stride(0), _row_stride(ref_chosen), _row_stride(ref_rejected),
+                  _row_stride(chosen_mask), _row_stride(rejected_mask)),
+         B, Tc, Tr, *options, 1 if average else 0, out.data_ptr(), rc.data_ptr(), rr.data_ptr(), _address(gc),
+         _address(gr), ws.data_ptr(), ws.numel())
     return out, rc, rr, gc, gr
 
 

@@ -334,8 +334,8 @@ int b200_leaky_backward_async(const float* input_current, const float* checkpoin
  *     decay: grad_x = g, grad_gate = g * h[t-1]
  *     sigmoid: grad_x = (1 - a) * g, grad_gate = g * (h[t-1] - x) * a * (1 - a)
  *   grad_state = a[0] * g[0]
- * workspace: b200_linear_recurrence_workspace_bytes(B, T, H) bytes for either direction, 16-byte
- * aligned, zero-filled once before first use (every call leaves it ready for the next), used by one
+ * workspace: b200_linear_recurrence_workspace_bytes(B, T, H) bytes for either direction (0 for short
+ * sequences), 16-byte aligned, zero-filled once before first use (every call leaves it ready for the next), used by one
  * stream at a time.  Results are the same bits on every call.
  *
  * The step advances B rows by one token: row b reads state[slot] (fp32 [n_slots, H]) and writes
@@ -402,8 +402,9 @@ int b200_token_logprob_backward_async(const void* logits, int dtype, const int64
  * token all outputs are 0.  ref_log_prob (then kl is 0) and entropy may be NULL.
  * strides (host array, elements): rows of log_prob, old_log_prob, advantage; 1, or 0 when advantage
  * holds one value per row; rows of ref_log_prob, entropy, mask.  The token axis is contiguous.
- * workspace: b200_policy_loss_workspace_bytes(B, T) bytes, 16-byte aligned, zero-filled once before
- * first use, used by one stream at a time.
+ * workspace: b200_policy_loss_workspace_bytes(B, T) bytes (0 for few tokens), 16-byte aligned,
+ * zero-filled once before first use (every call leaves it ready for the next), used by one stream at a
+ * time.
  * ------------------------------------------------------------------------------------------- */
 #define B200_KL_K1 0
 #define B200_KL_K2 1
@@ -433,7 +434,7 @@ int b200_policy_loss_async(const float* log_prob, const float* old_log_prob, con
  * tokens, which are not looked at.  B = 0 gives 0.  strides (host array, elements): rows of chosen,
  * rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask; the token axis is contiguous.
  * workspace: b200_preference_loss_workspace_bytes(B) bytes, 16-byte aligned, zero-filled once before
- * first use, used by one stream at a time.
+ * first use (every call leaves it ready for the next), used by one stream at a time.
  * ------------------------------------------------------------------------------------------- */
 #define B200_PREFERENCE_SIGMOID 0
 #define B200_PREFERENCE_HINGE 1
