@@ -18,6 +18,7 @@
 
 #include <math.h>
 
+#include "../common/bulk.cuh"
 #include "../common/vec.cuh"
 #include "../common/workspace.cuh"
 
@@ -49,22 +50,27 @@ __device__ __forceinline__ void two_diff(float a, float b, float& s, float& e) {
 __device__ __forceinline__ bool above(float s, float e, Pair p) { return s > p.hi || (s == p.hi && e > p.lo); }
 __device__ __forceinline__ bool below(float s, float e, Pair p) { return s < p.hi || (s == p.hi && e < p.lo); }
 
-// exp(q) - 1 - q without the cancellation near 0: its Taylor series up to q^12 / 12! for |q| <= 1 (the next
-// term is below 2^-31 of the value), the difference beyond, where it costs at most some bits of expm1's.
-__device__ __forceinline__ float exp_minus_1_minus(float q) {
-  if (fabsf(q) > 1.0f) return expm1f(q) - q;
-  float p = 1.0f / 479001600.0f;
-  p = fmaf(p, q, 1.0f / 39916800.0f);
-  p = fmaf(p, q, 1.0f / 3628800.0f);
-  p = fmaf(p, q, 1.0f / 362880.0f);
-  p = fmaf(p, q, 1.0f / 40320.0f);
-  p = fmaf(p, q, 1.0f / 5040.0f);
-  p = fmaf(p, q, 1.0f / 720.0f);
-  p = fmaf(p, q, 1.0f / 120.0f);
-  p = fmaf(p, q, 1.0f / 24.0f);
-  p = fmaf(p, q, 1.0f / 6.0f);
-  p = fmaf(p, q, 0.5f);
-  return q * q * p;
+// exp(q) - 1 - q without the cancellation near 0, for two values: the Taylor series up to q^12 / 12! for
+// |q| <= 1 (the next term is below 2^-31 of the value), the difference beyond, where it costs at most
+// some bits of expm1's.
+__device__ __forceinline__ float2 exp_minus_1_minus(float2 q) {
+  float2 p = splat2(1.0f / 479001600.0f);
+  p = fma2(p, q, splat2(1.0f / 39916800.0f));
+  p = fma2(p, q, splat2(1.0f / 3628800.0f));
+  p = fma2(p, q, splat2(1.0f / 362880.0f));
+  p = fma2(p, q, splat2(1.0f / 40320.0f));
+  p = fma2(p, q, splat2(1.0f / 5040.0f));
+  p = fma2(p, q, splat2(1.0f / 720.0f));
+  p = fma2(p, q, splat2(1.0f / 120.0f));
+  p = fma2(p, q, splat2(1.0f / 24.0f));
+  p = fma2(p, q, splat2(1.0f / 6.0f));
+  p = fma2(p, q, splat2(0.5f));
+  float2 r = mul2(mul2(q, q), p);
+  if (fmaxf(fabsf(q.x), fabsf(q.y)) > 1.0f) {
+    if (fabsf(q.x) > 1.0f) r.x = expm1f(q.x) - q.x;
+    if (fabsf(q.y) > 1.0f) r.y = expm1f(q.y) - q.y;
+  }
+  return r;
 }
 
 // i / d for i < 2^31 by a multiplication (d >= 1).
@@ -93,7 +99,8 @@ struct Params {
   float high, low, dual;  // 1 + clip_high, 1 - clip_low, c (0: off)
   float kl_coef, ent_coef;
   int kl_form, reduction;
-  double scale, kl_coef_d, ent_coef_d;
+  float scale;
+  double kl_coef_d, ent_coef_d;
   float *grad, *grad_ent, *out;
 };
 
@@ -111,11 +118,12 @@ struct Ctl {
   unsigned long long tokens;
 };
 
+// The weight of a token: three roundings at most.
 __device__ __forceinline__ float token_weight(const Params& p, unsigned long long tokens, unsigned rows, int row_tokens) {
-  if (p.reduction == kTokenMean) return float(p.scale / double(tokens > 0 ? tokens : 1ull));
+  if (p.reduction == kTokenMean) return __fdiv_rn(p.scale, float(tokens > 0 ? tokens : 1ull));
   if (p.reduction == kSequenceMean)
-    return float(p.scale / (double(rows > 0 ? rows : 1u) * double(row_tokens > 0 ? row_tokens : 1)));
-  return float(p.scale);
+    return __fdiv_rn(p.scale, float(rows > 0 ? rows : 1u) * float(row_tokens > 0 ? row_tokens : 1));
+  return p.scale;
 }
 
 // The tokens of one lane as they are read: kPer consecutive ones (p.vec), or kPer a warp's width apart.  What
@@ -198,69 +206,101 @@ __device__ __forceinline__ void load_tokens(const Params& p, unsigned first, Raw
   }
 }
 
-// What a token adds: policy, kl and entropy terms weighted with w, exp(d) - 1 - d, r; and its gradient.
-struct Terms {
-  float pg, kl, ent, diff, ratio;
+// Whether a token's difference lies above log(1 + clip_high), below log(1 - clip_low), above log(dual).
+struct Side {
+  bool hi, lo, dual;
 };
 
-__device__ __forceinline__ float take_token(const Params& p, const Raw& r, int j, float w, Sums& a, Terms& k) {
-  k = Terms{0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  if (((r.on >> j) & 1u) == 0u) return 0.0f;
-  const float cur = r.cur[j], adv = r.adv[j];
-  const float s = __fsub_rn(cur, r.old[j]);
-  bool hi = s > p.log_high.hi, lo = s < p.log_low.hi;
-  bool dual = adv < 0.0f && s > p.log_dual.hi;
-  if (s == p.log_high.hi || s == p.log_low.hi || s == p.log_dual.hi) {  // the rounding decides: look at it
-    float d, e;
-    two_diff(cur, r.old[j], d, e);
-    hi = above(s, e, p.log_high);
-    lo = below(s, e, p.log_low);
-    dual = adv < 0.0f && above(s, e, p.log_dual);
+// Four tokens of one lane: their terms are added in fp32 in a tree and then to the running sums in fp64; g and ge
+// are their gradients.  w: each token's weight.
+__device__ __forceinline__ void take_tokens(const Params& p, const Raw& r, const float (&weight)[kPer], Sums& a,
+                                            float (&g)[kPer], float (&ge)[kPer]) {
+  float w[kPer], one[kPer], cur[kPer], s[kPer], A[kPer];
+  Side side[kPer];
+  bool close = false;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {  // a masked-out token becomes one with d = 0, A = 0 and weight 0
+    const bool on = (r.on >> j) & 1u;
+    w[j] = on ? weight[j] : 0.0f;
+    one[j] = on ? 1.0f : 0.0f;
+    cur[j] = on ? r.cur[j] : 0.0f;
+    A[j] = on ? r.adv[j] : 0.0f;
+    s[j] = on ? __fsub_rn(r.cur[j], r.old[j]) : 0.0f;
+    side[j] = Side{s[j] > p.log_high.hi, s[j] < p.log_low.hi, s[j] > p.log_dual.hi};
+    close |= s[j] == p.log_high.hi || s[j] == p.log_low.hi || s[j] == p.log_dual.hi;
   }
-  k.ratio = exp2_approx(s * 1.4426950408889634f);
-  k.diff = exp_minus_1_minus(s);
-  const bool clipped = (adv > 0.0f && hi) || (adv < 0.0f && lo) || dual || adv == 0.0f;
-  const float held = dual ? p.dual : hi ? p.high : p.low;
-  const float pg = adv == 0.0f ? 0.0f : (clipped ? held : k.ratio) * -adv;
-  float g = clipped ? 0.0f : pg;
-  if (p.ref != nullptr) {
-    const float q = __fsub_rn(r.ref[j], cur);
-    float dkl;
-    if (p.kl_form == kK1) {
-      k.kl = -q, dkl = 1.0f;
-    } else if (p.kl_form == kK2) {
-      k.kl = 0.5f * q * q, dkl = -q;
-    } else {
-      k.kl = exp_minus_1_minus(q), dkl = -(q + k.kl);  // 1 - exp(q)
+  if (close) {  // the rounding of a difference decides: look at it
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      float d, e;
+      two_diff(r.cur[j], r.old[j], d, e);
+      if ((r.on >> j) & 1u) side[j] = Side{above(d, e, p.log_high), below(d, e, p.log_low), above(d, e, p.log_dual)};
     }
-    g = fmaf(p.kl_coef, dkl, g);
-    k.kl *= w;
   }
-  k.pg = pg * w;
-  k.ent = r.ent[j] * w;
-  a.max_ratio = fmaxf(a.max_ratio, k.ratio);
-  a.outside += hi || lo;
-  return g * w;
-}
-
-// The tokens of one lane: their terms are added in fp32 in a tree and then to the running sums in fp64, their
-// gradients are written.  w: each token's weight.
-template <bool kVec>
-__device__ __forceinline__ void take_tokens(const Params& p, unsigned first, const Raw& r, const float (&w)[kPer],
-                                            Sums& a) {
-  Terms k[kPer];
-  float g[kPer], ge[kPer];
+  float ratio[kPer], pg[kPer], diff[kPer], slope[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; j += 2) {
+    const float2 z = mul2(make_float2(s[j], s[j + 1]), splat2(1.4426950408889634f));
+    ratio[j] = exp2_approx(z.x), ratio[j + 1] = exp2_approx(z.y);
+    const float2 d = exp_minus_1_minus(make_float2(s[j], s[j + 1]));
+    diff[j] = d.x, diff[j + 1] = d.y;
+  }
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    g[j] = take_token(p, r, j, w[j], a, k[j]);
-    ge[j] = ((r.on >> j) & 1u) != 0u ? -w[j] * p.ent_coef : 0.0f;
+    // A > 0 is held at 1 + clip_high, A < 0 at 1 - clip_low and at the dual clip; A = 0 adds nothing.
+    const bool up = A[j] > 0.0f, down = A[j] < 0.0f;
+    const bool held = (up && side[j].hi) || (down && (side[j].lo || side[j].dual));
+    const float at = up ? p.high : side[j].lo ? p.low : p.dual;
+    const float value = (held ? at : ratio[j]) * -A[j];
+    pg[j] = up || down || A[j] != A[j] ? value : 0.0f;
+    slope[j] = held ? 0.0f : pg[j];
+    a.max_ratio = fmaxf(a.max_ratio, one[j] * ratio[j]);
+    a.outside += side[j].hi || side[j].lo;
   }
   a.tokens += __popc(r.on);
-  a.pg += double((k[0].pg + k[1].pg) + (k[2].pg + k[3].pg));
-  if (p.ref != nullptr) a.kl += double((k[0].kl + k[1].kl) + (k[2].kl + k[3].kl));
-  if (p.ent != nullptr) a.ent += double((k[0].ent + k[1].ent) + (k[2].ent + k[3].ent));
-  a.diff += double((k[0].diff + k[1].diff) + (k[2].diff + k[3].diff));
-  a.ratio += double((k[0].ratio + k[1].ratio) + (k[2].ratio + k[3].ratio));
+  float kl[kPer] = {};
+  if (p.ref != nullptr) {
+    float dkl[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; j += 2) {
+      float2 q = make_float2(__fsub_rn(r.ref[j], cur[j]), __fsub_rn(r.ref[j + 1], cur[j + 1]));
+      if (!((r.on >> j) & 1u)) q.x = 0.0f;
+      if (!((r.on >> (j + 1)) & 1u)) q.y = 0.0f;
+      if (p.kl_form == kK1) {
+        kl[j] = -q.x, kl[j + 1] = -q.y;
+        dkl[j] = dkl[j + 1] = 1.0f;
+      } else if (p.kl_form == kK2) {
+        kl[j] = 0.5f * q.x * q.x, kl[j + 1] = 0.5f * q.y * q.y;
+        dkl[j] = -q.x, dkl[j + 1] = -q.y;
+      } else {
+        const float2 k = exp_minus_1_minus(q);
+        kl[j] = k.x, kl[j + 1] = k.y;
+        dkl[j] = -(q.x + k.x), dkl[j + 1] = -(q.y + k.y);  // 1 - exp(q)
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) slope[j] = fmaf(p.kl_coef, dkl[j], slope[j]);
+    a.kl += double((kl[0] * w[0] + kl[1] * w[1]) + (kl[2] * w[2] + kl[3] * w[3]));
+  }
+  if (p.ent != nullptr) {
+    float e[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) e[j] = ((r.on >> j) & 1u ? r.ent[j] : 0.0f) * w[j];
+    a.ent += double((e[0] + e[1]) + (e[2] + e[3]));
+  }
+  a.pg += double((pg[0] * w[0] + pg[1] * w[1]) + (pg[2] * w[2] + pg[3] * w[3]));
+  a.diff += double((diff[0] + diff[1]) + (diff[2] + diff[3]));
+  a.ratio += double((ratio[0] * one[0] + ratio[1] * one[1]) + (ratio[2] * one[2] + ratio[3] * one[3]));
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    g[j] = slope[j] * w[j];
+    ge[j] = -p.ent_coef * w[j];
+  }
+}
+
+template <bool kVec>
+__device__ __forceinline__ void write_tokens(const Params& p, unsigned first, const float (&g)[kPer],
+                                             const float (&ge)[kPer]) {
   if (kVec && first + kPer <= p.n) {
     if (p.grad) st_stream_f4(p.grad + first, make_float4(g[0], g[1], g[2], g[3]));
     if (p.grad_ent) st_stream_f4(p.grad_ent + first, make_float4(ge[0], ge[1], ge[2], ge[3]));
@@ -300,17 +340,16 @@ __device__ __forceinline__ void sum_block(Sums& a) {
   }
 }
 
-// tokens: fp64 holds the counts' sum of any size.
-__device__ __forceinline__ void write_outputs(const Params& p, const Sums& a, double tokens, double outside) {
-  const double n = tokens > 0 ? tokens : 1.0;
+__device__ __forceinline__ void write_outputs(const Params& p, const Sums& a) {
+  const double inv = 1.0 / double(a.tokens > 0u ? a.tokens : 1u);
   p.out[0] = float(a.pg + p.kl_coef_d * a.kl - p.ent_coef_d * a.ent);
   p.out[1] = float(a.pg);
   p.out[2] = float(a.kl);
   p.out[3] = float(a.ent);
-  p.out[4] = float(outside / n);
-  p.out[5] = float(a.diff / n);
+  p.out[4] = float(double(a.outside) * inv);
+  p.out[5] = float(a.diff * inv);
   p.out[6] = a.max_ratio;
-  p.out[7] = float(a.ratio / n);
+  p.out[7] = float(a.ratio * inv);
 }
 
 // --------------------------------------------------------------------------- few tokens: one CTA
@@ -349,9 +388,11 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_const
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
     w[j] = per_row || j == 0 ? token_weight(p, total, rows, per_row ? row_tokens[r.row[j]] : 0) : w[0];
-  take_tokens<kVec>(p, first, r, w, a);
+  float g[kPer], ge[kPer];
+  take_tokens(p, r, w, a, g, ge);
+  write_tokens<kVec>(p, first, g, ge);
   sum_block<kSmallThreads / 32>(a);
-  if (threadIdx.x == 0) write_outputs(p, a, double(a.tokens), double(a.outside));
+  if (threadIdx.x == 0) write_outputs(p, a);
 }
 
 // ------------------------------------------------------------------- many tokens: counts, then terms
@@ -404,51 +445,23 @@ __global__ void __launch_bounds__(kThreads) count_kernel(const Params p, unsigne
   }
 }
 
-// Bytes of all streams' L2 prefetch, at most: lines prefetched beyond it would be evicted before their use.
-constexpr int64_t kPrefetchBytes = 48 << 20;
+// What the counts say, for every CTA of a kernel behind count_kernel.
+struct Counts {
+  unsigned long long tokens;
+  unsigned rows;
+};
+__device__ __forceinline__ Counts read_counts(const Params& p, bool counted, Ctl* ctl) {
+  if (!counted) return Counts{(unsigned long long)(p.n), unsigned(p.B)};
+  return Counts{*reinterpret_cast<volatile unsigned long long*>(&ctl->tokens), ld_cg_u32(&ctl->rows)};
+}
 
-// A CTA takes stretches of kThreads * kPer tokens, grid-stride.  counted: count_kernel ran before; while it does,
-// this kernel brings its first stretches into L2 (their own reads wait for it).
-template <bool kVec>
-__global__ void __launch_bounds__(kThreads, 4) token_kernel(const __grid_constant__ Params p, bool counted,
-                                                            unsigned prefetch, Ctl* ctl, int* counts, Sums* sums) {
-  constexpr unsigned kUnit = kThreads * kPer;
-  const unsigned units = (p.n + kUnit - 1) / kUnit;
-  if (counted && p.dense) {
-    const float* streams[5] = {p.cur, p.old, p.adv_rows ? nullptr : p.adv, p.ref, p.ent};
-    for (unsigned u = blockIdx.x, k = 0; u < units && k < prefetch; u += gridDim.x, ++k) {
-      const unsigned at = u * kUnit + threadIdx.x * 32;  // a 128-byte line per thread
-      if (threadIdx.x < kUnit / 32 && at < p.n)
-#pragma unroll
-        for (int s = 0; s < 5; ++s)
-          if (streams[s] != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(streams[s] + at));
-    }
-  }
-  pdl_begin();
-  const bool per_row = p.reduction == kSequenceMean;
-  const unsigned rows = counted ? ld_cg_u32(&ctl->rows) : unsigned(p.B);
-  const unsigned long long tokens =
-      counted ? *reinterpret_cast<volatile unsigned long long*>(&ctl->tokens) : (unsigned long long)(p.n);
-  float w[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) w[j] = j == 0 ? token_weight(p, tokens, rows, p.T) : w[0];
-  Sums a = {};
-  for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
-    const unsigned first = first_token<kVec>(u, kThreads);
-    Raw r;
-    load_tokens<kVec>(p, first, r);
-    if (per_row && counted) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        w[j] = kVec && j > 0 && r.row[j] == r.row[j - 1] ? w[j - 1] : token_weight(p, tokens, rows, counts[r.row[j]]);
-    }
-    take_tokens<kVec>(p, first, r, w, a);
-  }
+// The end of a kernel of many CTAs: each writes its sums, the last adds them up in their order, writes the
+// outputs and leaves the workspace as it was.
+__device__ __forceinline__ void finish(const Params& p, Sums& a, bool counted, Ctl* ctl, int* counts, Sums* sums) {
   sum_block<kThreads / 32>(a);
   if (threadIdx.x == 0) sums[blockIdx.x] = a;
   if (!elect_last_cta(&ctl->done)) return;
   a = Sums{};
-  double all = 0.0, out = 0.0;
   for (unsigned i = threadIdx.x; i < gridDim.x; i += kThreads) {
     const Sums& s = sums[i];
     a.pg += __ldcg(&s.pg);
@@ -462,13 +475,141 @@ __global__ void __launch_bounds__(kThreads, 4) token_kernel(const __grid_constan
   }
   sum_block<kThreads / 32>(a);
   if (threadIdx.x == 0) {
-    all = double(a.tokens), out = double(a.outside);
-    write_outputs(p, a, all, out);
+    write_outputs(p, a);
     ctl->tokens = 0ull;
     ctl->rows = 0u;
   }
-  if (per_row && counted)
+  if (p.reduction == kSequenceMean && counted)
     for (int b = threadIdx.x; b < p.B; b += kThreads) counts[b] = 0;
+}
+
+// Any layout: a CTA takes stretches of kThreads * kPer tokens, grid-stride, through registers.
+template <bool kVec>
+__global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__ Params p, bool counted, Ctl* ctl,
+                                                         int* counts, Sums* sums) {
+  constexpr unsigned kUnit = kThreads * kPer;
+  const unsigned units = (p.n + kUnit - 1) / kUnit;
+  pdl_begin();
+  const bool per_row = p.reduction == kSequenceMean;
+  const Counts c = read_counts(p, counted, ctl);
+  float w[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) w[j] = j == 0 ? token_weight(p, c.tokens, c.rows, p.T) : w[0];
+  Sums a = {};
+  for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
+    const unsigned first = first_token<kVec>(u, kThreads);
+    Raw r;
+    load_tokens<kVec>(p, first, r);
+    if (per_row && counted) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) w[j] = token_weight(p, c.tokens, c.rows, counts[r.row[j]]);
+    }
+    float g[kPer], ge[kPer];
+    take_tokens(p, r, w, a, g, ge);
+    write_tokens<kVec>(p, first, g, ge);
+  }
+  finish(p, a, counted, ctl, counts, sums);
+}
+
+// Dense streams on 16-byte boundaries: stretches of kUnit tokens arrive in shared memory by bulk copies, kStages
+// ahead, so that loads never wait for arithmetic.  A thread has four consecutive tokens.  What is left of
+// less than a stretch goes through registers.
+// Behind count_kernel the copies start before the counts are there: every CTA of count_kernel lets this kernel
+// start only after it has itself waited for the kernels before it, so the inputs are complete.
+constexpr int kStages = 4;
+constexpr unsigned kUnit = kThreads * kPer;
+constexpr unsigned kStreamBytes = kUnit * 4u;
+
+struct Streams {
+  const float* p[5];  // cur, old, adv, ref, ent; null: not there
+  int slot[5];        // its place in a stage
+  int n;              // streams that are there
+};
+
+__global__ void __launch_bounds__(kThreads, 2) dense_kernel(const __grid_constant__ Params p,
+                                                            const __grid_constant__ Streams st, bool counted, Ctl* ctl,
+                                                            int* counts, Sums* sums) {
+  extern __shared__ __align__(128) char smem[];
+  __shared__ uint64_t full[kStages];
+  const unsigned whole = p.n / kUnit;
+  const unsigned stage_bytes = unsigned(st.n) * kStreamBytes + (p.mask != nullptr ? kUnit : 0u);
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (!counted) pdl_begin();
+  const auto fetch = [&](unsigned u, unsigned stage) {  // thread 0
+    if (u >= whole) return;
+    char* dst = smem + stage * stage_bytes;
+    mbar_arrive_expect_tx(&full[stage], stage_bytes);
+#pragma unroll
+    for (int s = 0; s < 5; ++s)
+      if (st.p[s] != nullptr)
+        bulk_g2s(dst + st.slot[s] * kStreamBytes, st.p[s] + size_t(u) * kUnit, kStreamBytes, &full[stage]);
+    if (p.mask != nullptr) bulk_g2s(dst + st.n * kStreamBytes, p.mask + size_t(u) * kUnit, kUnit, &full[stage]);
+  };
+  if (threadIdx.x == 0)
+    for (unsigned k = 0; k < unsigned(kStages); ++k) fetch(blockIdx.x + k * gridDim.x, k);
+  if (counted) pdl_begin();
+  const bool per_row = p.reduction == kSequenceMean;
+  const Counts c = read_counts(p, counted, ctl);
+  float w[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) w[j] = j == 0 ? token_weight(p, c.tokens, c.rows, p.T) : w[0];
+  Sums a = {};
+  unsigned stage = 0, parity = 0;
+  for (unsigned u = blockIdx.x; u < whole; u += gridDim.x) {
+    const unsigned first = u * kUnit + threadIdx.x * kPer;
+    Raw r;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) r.ref[j] = r.ent[j] = r.adv[j] = 0.0f;
+    if (p.need_row) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) r.row[j] = j > 0 && p.T % kPer == 0 ? r.row[0] : p.by_T.div(first + j);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (per_row && counted) w[j] = token_weight(p, c.tokens, c.rows, counts[r.row[j]]);
+        if (p.adv_rows) r.adv[j] = p.adv[int64_t(r.row[j]) * p.adv_s];
+      }
+    }
+    mbar_wait(&full[stage], parity);
+    const char* src = smem + stage * stage_bytes + threadIdx.x * (kPer * 4);
+    const auto take4 = [&](int s, float (&f)[kPer]) {
+      const float4 v = *reinterpret_cast<const float4*>(src + st.slot[s] * kStreamBytes);
+      f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    };
+    take4(0, r.cur);
+    take4(1, r.old);
+    if (!p.adv_rows) take4(2, r.adv);
+    if (p.ref != nullptr) take4(3, r.ref);
+    if (p.ent != nullptr) take4(4, r.ent);
+    uint32_t m = 0x01010101u;
+    if (p.mask != nullptr)
+      m = __vminu4(*reinterpret_cast<const uint32_t*>(smem + stage * stage_bytes + st.n * kStreamBytes +
+                                                      threadIdx.x * kPer),
+                   0x01010101u);
+    r.on = (m * 0x10204080u) >> 28;  // bit 8 j of m to bit j
+    __syncthreads();  // the stage is read
+    if (threadIdx.x == 0) fetch(u + kStages * gridDim.x, stage);
+    if (++stage == unsigned(kStages)) stage = 0, parity ^= 1u;
+    float g[kPer], ge[kPer];
+    take_tokens(p, r, w, a, g, ge);
+    write_tokens<true>(p, first, g, ge);
+  }
+  if (blockIdx.x == gridDim.x - 1 && whole * kUnit < p.n) {
+    const unsigned first = first_token<true>(whole, kThreads);
+    Raw r;
+    load_tokens<true>(p, first, r);
+    if (per_row && counted) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) w[j] = token_weight(p, c.tokens, c.rows, counts[r.row[j]]);
+    }
+    float g[kPer], ge[kPer];
+    take_tokens(p, r, w, a, g, ge);
+    write_tokens<true>(p, first, g, ge);
+  }
+  finish(p, a, counted, ctl, counts, sums);
 }
 
 // ------------------------------------------------------------------------------------ host side
@@ -514,7 +655,7 @@ inline int run(const float* cur, const float* old, const float* adv, const float
   p.log_dual = make_pair_of(dual_clip > 0.0 ? log(dual_clip) : double(NAN));  // NaN: no difference is it
   p.high = float(1.0 + clip_high), p.low = float(1.0 - clip_low), p.dual = float(dual_clip);
   p.kl_coef = float(kl_coef), p.ent_coef = float(ent_coef), p.kl_form = kl_form, p.reduction = reduction;
-  p.scale = scale, p.kl_coef_d = kl_coef, p.ent_coef_d = ent_coef;
+  p.scale = float(scale), p.kl_coef_d = kl_coef, p.ent_coef_d = ent_coef;
   p.grad = grad, p.grad_ent = grad_ent, p.out = out;
   const auto aligned = [&](const void* q, int64_t s) {
     return q == nullptr || (aligned16(q) && (p.dense || (T % kPer == 0 && s % kPer == 0)));
@@ -539,15 +680,26 @@ inline int run(const float* cur, const float* old, const float* adv, const float
                               stretches, ctl, counts);
     if (st != kOk) return st;
   }
-  const int64_t units = (n + kThreads * kPer - 1) / (kThreads * kPer);
-  int64_t ctas = int64_t(sm_count()) * resident_ctas_per_sm(token_kernel<true>, kThreads, 0);
-  if (ctas > kMaxCtas) ctas = kMaxCtas;
-  if (ctas > units) ctas = units;
-  const int streams = 2 + !p.adv_rows + (ref != nullptr) + (ent != nullptr);
-  const int64_t unit_bytes = int64_t(kThreads) * kPer * 4 * streams;
-  const unsigned prefetch = unsigned(kPrefetchBytes / (unit_bytes * ctas));
-  return launch_pdl(p.vec ? token_kernel<true> : token_kernel<false>, dim3(unsigned(ctas)), dim3(kThreads), 0, stream, p, counted, prefetch, ctl, counts,
-                    sums);
+  const int64_t units = (n + kUnit - 1) / kUnit;
+  const auto grid = [&](int per_sm) {
+    const int64_t most = int64_t(sm_count()) * per_sm;
+    return unsigned(most < units ? (most < kMaxCtas ? most : kMaxCtas) : (units < kMaxCtas ? units : kMaxCtas));
+  };
+  if (p.dense && p.vec && (mask == nullptr || aligned16(mask))) {
+    Streams st = {};
+    const float* all[5] = {cur, old, p.adv_rows ? nullptr : adv, ref, ent};
+    for (int s = 0; s < 5; ++s) {
+      st.p[s] = all[s];
+      if (all[s] != nullptr) st.slot[s] = st.n++;
+    }
+    const int smem = kStages * int(unsigned(st.n) * kStreamBytes + (mask != nullptr ? kUnit : 0u));
+    if (!ensure_dyn_smem(dense_kernel, smem)) return kCudaError;
+    return launch_pdl(dense_kernel, dim3(grid(resident_ctas_per_sm(dense_kernel, kThreads, size_t(smem)))),
+                      dim3(kThreads), size_t(smem), stream, p, st, counted, ctl, counts, sums);
+  }
+  const auto kernel = p.vec ? token_kernel<true> : token_kernel<false>;
+  return launch_pdl(kernel, dim3(grid(resident_ctas_per_sm(kernel, kThreads, 0))), dim3(kThreads), 0, stream, p, counted,
+                    ctl, counts, sums);
 }
 
 }  // namespace policy

@@ -29,25 +29,24 @@ struct Side {
   int64_t lp_s, ref_s, mask_s;  // row strides
   int T;
   float *reward, *grad;
-  bool vec_in, vec_out;  // rows of lp, ref and mask (of grad) take vectors of four tokens
 };
 
 struct Params {
   Side side[2];  // chosen, rejected
   int B;
-  double beta, smoothing, margin;
+  double beta, smoothing, margin, inv_B;
   int form;
   bool average;
   float* out;
 };
 
-__device__ __forceinline__ double softplus(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
-__device__ __forceinline__ double sigmoid(double v) { return 1.0 / (1.0 + exp(-v)); }
-
+// The loss of margin z and its derivative.
 __device__ __forceinline__ double pair_loss(const Params& p, double z, double& dz) {
   if (p.form == kSigmoid) {
-    dz = p.smoothing - sigmoid(-z);
-    return (1.0 - p.smoothing) * softplus(-z) + p.smoothing * softplus(z);
+    const double e = exp(-fabs(z)), inv = 1.0 / (1.0 + e), tail = log1p(e);  // both softplus are max + tail
+    dz = p.smoothing - (z >= 0.0 ? e * inv : inv);                           // e - sigmoid(-z)
+    if (z != z) dz = z;
+    return (1.0 - p.smoothing) * (fmax(-z, 0.0) + tail) + p.smoothing * (fmax(z, 0.0) + tail);
   }
   if (p.form == kHinge) {
     dz = z < 1.0 ? -1.0 : 0.0;
@@ -81,90 +80,122 @@ __device__ __forceinline__ double gap_of(float x, float r, bool on) {
   return on ? double(x) - double(r) : 0.0;
 }
 
-// This CTA's stretch of answer b: tokens [t0, t1), t0 a multiple of 4.  What masked-out tokens hold is read with
-// the others and not used.
+__device__ __forceinline__ unsigned ld_u8(const uint8_t* p) {
+  unsigned v;
+  asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_u32(const uint8_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+
+// One answer's row and a CTA's stretch of it.
+struct Row {
+  const float *lp, *ref;  // ref and mask may be null
+  const uint8_t* mask;
+  float* grad;
+  int t0, t1;  // the stretch
+  int v0, v1;  // of it, the part that is whole vectors of four tokens in every stream (v0 = v1: none)
+};
+
+// Rows start anywhere (every row of an odd length does), but where all streams are off their 16-byte (the mask: 4-byte)
+// boundaries by the same number of tokens, vectors begin after the same few tokens in all of them.
+__device__ __forceinline__ Row row_of(const Side& d, int64_t b, unsigned part, unsigned parts) {
+  Row r;
+  r.lp = d.lp + b * d.lp_s;
+  r.ref = d.ref == nullptr ? nullptr : d.ref + b * d.ref_s;
+  r.mask = d.mask == nullptr ? nullptr : d.mask + b * d.mask_s;
+  r.grad = d.grad == nullptr ? nullptr : d.grad + b * d.T;
+  const auto off = [](const float* p) { return unsigned(reinterpret_cast<uintptr_t>(p) >> 2) & 3u; };
+  const unsigned o = off(r.lp);
+  const bool same = (r.ref == nullptr || off(r.ref) == o) && (r.grad == nullptr || off(r.grad) == o) &&
+                    (r.mask == nullptr || (unsigned(reinterpret_cast<uintptr_t>(r.mask)) & 3u) == o);
+  const int head = min(d.T, int((4u - o) & 3u));
+  const int per = int((unsigned(d.T - head) + 4 * parts - 1) / (4 * parts)) * 4;
+  r.t0 = part == 0 ? 0 : int(min(int64_t(d.T), head + int64_t(per) * part));
+  r.t1 = int(min(int64_t(d.T), head + int64_t(per) * (part + 1)));
+  r.v0 = part == 0 ? head : r.t0;
+  r.v1 = same ? r.v0 + ((r.t1 - r.v0) & ~3) : r.v0;
+  return r;
+}
+
+// The stretch's sum and count.  What masked-out tokens hold is read with the others and not used.
 template <int kThreads>
-__device__ __forceinline__ Part sum_stretch(const Side& d, int64_t b, int t0, int t1) {
-  const float *lp = d.lp + b * d.lp_s, *ref = d.ref == nullptr ? nullptr : d.ref + b * d.ref_s;
-  const uint8_t* m = d.mask == nullptr ? nullptr : d.mask + b * d.mask_s;
+__device__ __forceinline__ Part sum_stretch(const Row& d) {
   double s = 0.0;
   unsigned n = 0;
-  if (d.vec_in) {
-    const int t1v = t1 & ~3;
-    for (int t = t0 + int(threadIdx.x) * 4; t < t1v; t += kPer * kThreads) {
-      float4 x[kVecs], r[kVecs];
-      uint32_t on[kVecs];
+  for (int t = d.v0 + int(threadIdx.x) * 4; t < d.v1; t += kPer * kThreads) {
+    float4 x[kVecs], r[kVecs];
+    uint32_t on[kVecs];
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        const int at = t + k * 4 * kThreads;
-        const bool in = at < t1v;
-        x[k] = in ? ld_stream_f4(lp + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        r[k] = in && ref != nullptr ? ld_stream_f4(ref + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        on[k] = !in ? 0u : m == nullptr ? 0x01010101u : __vminu4(*reinterpret_cast<const uint32_t*>(m + at), 0x01010101u);
-      }
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        s += (gap_of(x[k].x, r[k].x, on[k] & 0xffu) + gap_of(x[k].y, r[k].y, on[k] & 0xff00u)) +
-             (gap_of(x[k].z, r[k].z, on[k] & 0xff0000u) + gap_of(x[k].w, r[k].w, on[k] & 0xff000000u));
-        n += __popc(on[k]);
-      }
+    for (int k = 0; k < kVecs; ++k) {
+      const int at = t + k * 4 * kThreads;
+      const bool in = at < d.v1;
+      x[k] = in ? ld_stream_f4(d.lp + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      r[k] = in && d.ref != nullptr ? ld_stream_f4(d.ref + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      on[k] = !in ? 0u : d.mask == nullptr ? 0x01010101u : ld_u32(d.mask + at);
     }
-    t0 = t1v;  // at most three tokens are left
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      s += (gap_of(x[k].x, r[k].x, on[k] & 0xffu) + gap_of(x[k].y, r[k].y, on[k] & 0xff00u)) +
+           (gap_of(x[k].z, r[k].z, on[k] & 0xff0000u) + gap_of(x[k].w, r[k].w, on[k] & 0xff000000u));
+      n += __popc(__vminu4(on[k], 0x01010101u));
+    }
   }
-  for (int t = t0 + int(threadIdx.x); t < t1; t += kPer * kThreads) {
+  // The rest: the tokens before and behind the vectors, or, without vectors, all of them.
+  const int before = d.v0 - d.t0, rest = before + d.t1 - d.v1;
+  for (int i = threadIdx.x; i < rest; i += kPer * kThreads) {
     float x[kPer], r[kPer];
-    bool on[kPer];
+    unsigned on[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int at = t + k * kThreads;
-      const bool in = at < t1;
-      x[k] = in ? ld_stream_f1(lp + at) : 0.0f;
-      r[k] = in && ref != nullptr ? ld_stream_f1(ref + at) : 0.0f;
-      on[k] = in && (m == nullptr || m[at] != 0);
+      const int q = i + k * kThreads, at = q < before ? d.t0 + q : d.v1 + q - before;
+      const bool in = q < rest;
+      x[k] = in ? ld_stream_f1(d.lp + at) : 0.0f;
+      r[k] = in && d.ref != nullptr ? ld_stream_f1(d.ref + at) : 0.0f;
+      on[k] = !in ? 0u : d.mask == nullptr ? 1u : ld_u8(d.mask + at);
     }
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      s += gap_of(x[k], r[k], on[k]);
-      n += on[k];
+      s += gap_of(x[k], r[k], on[k] != 0u);
+      n += on[k] != 0u;
     }
   }
   return Part{s, n};
 }
 
 template <int kThreads>
-__device__ __forceinline__ void write_stretch(const Side& d, int64_t b, int t0, int t1, float slope) {
+__device__ __forceinline__ void write_stretch(const Row& d, float slope) {
   if (d.grad == nullptr) return;
-  const uint8_t* m = d.mask == nullptr ? nullptr : d.mask + b * d.mask_s;
-  float* g = d.grad + b * d.T;
-  if (d.vec_in && d.vec_out) {
-    for (int t = t0 + int(threadIdx.x) * 4; t < t1; t += kPer * kThreads) {  // T is a multiple of 4
-      uint32_t on[kVecs];
+  for (int t = d.v0 + int(threadIdx.x) * 4; t < d.v1; t += kPer * kThreads) {
+    uint32_t on[kVecs];
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        const int at = t + k * 4 * kThreads;
-        on[k] = at < t1 && m != nullptr ? *reinterpret_cast<const uint32_t*>(m + at) : ~0u;
-      }
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        const int at = t + k * 4 * kThreads;
-        if (at < t1)
-          st_stream_f4(g + at, make_float4(on[k] & 0xffu ? slope : 0.0f, on[k] & 0xff00u ? slope : 0.0f,
-                                           on[k] & 0xff0000u ? slope : 0.0f, on[k] & 0xff000000u ? slope : 0.0f));
-      }
+    for (int k = 0; k < kVecs; ++k) {
+      const int at = t + k * 4 * kThreads;
+      on[k] = at < d.v1 && d.mask != nullptr ? ld_u32(d.mask + at) : ~0u;
     }
-    return;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int at = t + k * 4 * kThreads;
+      if (at < d.v1)
+        st_stream_f4(d.grad + at, make_float4(on[k] & 0xffu ? slope : 0.0f, on[k] & 0xff00u ? slope : 0.0f,
+                                              on[k] & 0xff0000u ? slope : 0.0f, on[k] & 0xff000000u ? slope : 0.0f));
+    }
   }
-  for (int t = t0 + int(threadIdx.x); t < t1; t += kPer * kThreads) {
-    bool on[kPer];
+  const int before = d.v0 - d.t0, rest = before + d.t1 - d.v1;
+  for (int i = threadIdx.x; i < rest; i += kPer * kThreads) {
+    unsigned on[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int at = t + k * kThreads;
-      on[k] = at < t1 && (m == nullptr || m[at] != 0);
+      const int q = i + k * kThreads, at = q < before ? d.t0 + q : d.v1 + q - before;
+      on[k] = q >= rest ? 0u : d.mask == nullptr ? 1u : ld_u8(d.mask + at);
     }
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int at = t + k * kThreads;
-      if (at < t1) g[at] = on[k] ? slope : 0.0f;
+      const int q = i + k * kThreads, at = q < before ? d.t0 + q : d.v1 + q - before;
+      if (q < rest) d.grad[at] = on[k] != 0u ? slope : 0.0f;
     }
   }
 }
@@ -178,6 +209,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
   __shared__ Part warp_part[2][kWarps];
   __shared__ Part cta_part[2][kMaxCluster];
   __shared__ float slope[2];
+  __shared__ bool last;
   __shared__ double total[3][kWarps];
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   const unsigned part = blockIdx.x % parts;
@@ -185,13 +217,11 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
   pdl_begin();
   // Every CTA of the cluster runs before any of them writes to another (waited for below).
   if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  int t0[2], t1[2];
+  Row row[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int per = int((unsigned(p.side[k].T) + 4 * parts - 1) / (4 * parts)) * 4;
-    t0[k] = int(min(int64_t(p.side[k].T), int64_t(per) * part));
-    t1[k] = int(min(int64_t(p.side[k].T), int64_t(t0[k]) + per));
-    Part a = sum_stretch<kThreads>(p.side[k], b, t0[k], t1[k]);
+    row[k] = row_of(p.side[k], b, part, parts);
+    Part a = sum_stretch<kThreads>(row[k]);
     a.s = warp_sum(a.s);
     a.n = warp_sum_u32(a.n);
     if (lane == 0) warp_part[k][w] = a;
@@ -233,18 +263,29 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
     const double gap = p.beta * (s[0] - s[1]);
     double dz;
     const double loss = pair_loss(p, gap - p.margin, dz);
+    const double k = p.beta * dz * p.inv_B;
+    slope[0] = float(k * inv[0]);
+    slope[1] = float(-k * inv[1]);
+    last = false;
     if (part == 0) {
       pairs[b] = PairOut{loss, s[0] > s[1] ? 1.0 : 0.0, gap};
       p.side[0].reward[b] = float(p.beta * s[0]);
       p.side[1].reward[b] = float(p.beta * s[1]);
     }
-    slope[0] = float(p.beta * dz * inv[0] / p.B);
-    slope[1] = float(-p.beta * dz * inv[1] / p.B);
   }
   __syncthreads();
+  // The first CTA of a pair counts it as done while the others of its threads write gradients.
+  if (threadIdx.x == 0 && part == 0) {
+    __threadfence();
+    last = atomicAdd(&ctl->done, 1u) == unsigned(p.B) - 1u;
+  }
 #pragma unroll
-  for (int k = 0; k < 2; ++k) write_stretch<kThreads>(p.side[k], b, t0[k], t1[k], slope[k]);
-  if (!elect_last_cta(&ctl->done)) return;
+  for (int k = 0; k < 2; ++k) write_stretch<kThreads>(row[k], slope[k]);
+  if (part != 0) return;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  if (threadIdx.x == 0) ctl->done = 0u;
   double a[3] = {0.0, 0.0, 0.0};
   for (int i = threadIdx.x; i < p.B; i += kThreads) {
     a[0] += __ldcg(&pairs[i].loss);
@@ -261,7 +302,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       const double s = warp_sum(lane < kWarps ? total[k][lane] : 0.0);
-      if (lane == 0) p.out[k] = float(s / p.B);
+      if (lane == 0) p.out[k] = float(s * p.inv_B);
     }
   }
 }
@@ -306,14 +347,7 @@ inline int run(const float* chosen, const float* rejected, const float* ref_chos
   p.side[0] = Side{chosen, ref_chosen, chosen_mask, strides[0], strides[2], strides[4], Tc, reward_chosen, grad_chosen};
   p.side[1] =
       Side{rejected, ref_rejected, rejected_mask, strides[1], strides[3], strides[5], Tr, reward_rejected, grad_rejected};
-  for (Side& d : p.side) {
-    const auto rows = [](const void* q, int64_t s, int bytes) {
-      return q == nullptr || (reinterpret_cast<uintptr_t>(q) % bytes == 0 && s % 4 == 0);
-    };
-    d.vec_in = rows(d.lp, d.lp_s, 16) && rows(d.ref, d.ref_s, 16) && rows(d.mask, d.mask_s, 4);
-    d.vec_out = rows(d.grad, d.T, 16);
-  }
-  p.B = B, p.beta = beta, p.smoothing = smoothing, p.margin = margin, p.form = form, p.average = average != 0;
+  p.B = B, p.inv_B = 1.0 / B, p.beta = beta, p.smoothing = smoothing, p.margin = margin, p.form = form, p.average = average != 0;
   p.out = out;
   const unsigned parts = cluster_of(B, int64_t(Tc) + Tr);
   if (int64_t(B) * parts > 0x7fffffff) return kUnsupported;
