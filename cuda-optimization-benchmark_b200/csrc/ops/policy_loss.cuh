@@ -50,10 +50,9 @@ __device__ __forceinline__ void two_diff(float a, float b, float& s, float& e) {
 __device__ __forceinline__ bool above(float s, float e, Pair p) { return s > p.hi || (s == p.hi && e > p.lo); }
 __device__ __forceinline__ bool below(float s, float e, Pair p) { return s < p.hi || (s == p.hi && e < p.lo); }
 
-// exp(q) - 1 - q without the cancellation near 0, for two values: the Taylor series up to q^12 / 12! for
-// |q| <= 1 (the next term is below 2^-31 of the value), the difference beyond, where it costs at most
-// some bits of expm1's.
-__device__ __forceinline__ float2 exp_minus_1_minus(float2 q) {
+// exp(q) - 1 - q without the cancellation near 0: the Taylor series up to q^12 / 12!, for |q| <= 1 (the next
+// term is below 2^-31 of the value).
+__device__ __forceinline__ float2 exp_tail(float2 q) {
   float2 p = splat2(1.0f / 479001600.0f);
   p = fma2(p, q, splat2(1.0f / 39916800.0f));
   p = fma2(p, q, splat2(1.0f / 3628800.0f));
@@ -65,12 +64,17 @@ __device__ __forceinline__ float2 exp_minus_1_minus(float2 q) {
   p = fma2(p, q, splat2(1.0f / 24.0f));
   p = fma2(p, q, splat2(1.0f / 6.0f));
   p = fma2(p, q, splat2(0.5f));
-  float2 r = mul2(mul2(q, q), p);
-  if (fmaxf(fabsf(q.x), fabsf(q.y)) > 1.0f) {
-    if (fabsf(q.x) > 1.0f) r.x = expm1f(q.x) - q.x;
-    if (fabsf(q.y) > 1.0f) r.y = expm1f(q.y) - q.y;
+  return mul2(mul2(q, q), p);
+}
+// The same for kPer values of any size: beyond 1 the difference itself, which costs at most some bits of expm1's.
+__device__ __forceinline__ void exp_minus_1_minus(const float (&q)[4], float (&r)[4]) {
+  const float2 a = exp_tail(make_float2(q[0], q[1])), b = exp_tail(make_float2(q[2], q[3]));
+  r[0] = a.x, r[1] = a.y, r[2] = b.x, r[3] = b.y;
+  if (fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3]))) > 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (fabsf(q[j]) > 1.0f) r[j] = expm1f(q[j]) - q[j];
   }
-  return r;
 }
 
 // i / d for i < 2^31 by a multiplication (d >= 1).
@@ -96,7 +100,8 @@ struct Params {
   bool adv_rows;   // one advantage per row
   bool need_row;   // a token's row is needed
   Pair log_high, log_low, log_dual;
-  float high, low, dual;  // 1 + clip_high, 1 - clip_low, c (0: off)
+  float mid, half, band;  // the clip range of d is mid +- half; within band of its borders the pairs decide
+  float high, low, dual;  // 1 + clip_high, 1 - clip_low, c (infinite: off)
   float kl_coef, ent_coef;
   int kl_form, reduction;
   float scale;
@@ -104,13 +109,15 @@ struct Params {
   float *grad, *grad_ent, *out;
 };
 
-// Weighted sums of the policy, kl and entropy terms; over the masked tokens the sums of exp(d) - 1 - d and of
-// r, the largest r, and the counts of tokens and of those outside the clip range.
+// Weighted sums of the policy, kl and entropy terms; over the tokens that count the sum of exp(d) - 1 - d, the
+// largest d, their number and that of those outside the clip range; the sum of r over all tokens seen, r = 1 at
+// those that do not count, and the number of these.
 struct Sums {
   double pg, kl, ent, diff, ratio;
-  float max_ratio;
-  unsigned outside, tokens;
+  float max_d;
+  unsigned outside, tokens, skipped;
 };
+__device__ __forceinline__ Sums no_sums() { return Sums{0.0, 0.0, 0.0, 0.0, 0.0, -INFINITY, 0u, 0u, 0u}; }
 
 // The workspace's control words: zero before the first call, and again after each.
 struct Ctl {
@@ -133,8 +140,15 @@ constexpr int kPer = 4;
 struct Raw {
   float cur[kPer], old[kPer], adv[kPer], ref[kPer], ent[kPer];
   unsigned row[kPer];
-  unsigned on;  // bit j: token j counts
+  uint32_t on;  // byte j: 0xff where token j counts, else 0
 };
+__device__ __forceinline__ uint32_t count_word(uint32_t mask_bytes) { return __vminu4(mask_bytes, 0x01010101u) * 0xffu; }
+// All bits set where token j counts, else none.
+template <int j>
+__device__ __forceinline__ uint32_t bits_of(uint32_t on) {
+  return __byte_perm(on, 0u, j * 0x1111u);
+}
+__device__ __forceinline__ float keep(float v, uint32_t bits) { return __uint_as_float(__float_as_uint(v) & bits); }
 
 __device__ __forceinline__ void load4(const float* p, int64_t at, float (&f)[kPer]) {
   const float4 v = ld_stream_f4(p + at);
@@ -171,8 +185,7 @@ __device__ __forceinline__ void load_tokens(const Params& p, unsigned first, Raw
     }
     const int64_t b = r.row[0];
     const auto at = [&](int64_t stride) { return p.dense ? int64_t(first) : b * stride + t; };
-    uint32_t m = 0x01010101u;
-    if (p.mask != nullptr) m = __vminu4(*reinterpret_cast<const uint32_t*>(p.mask + at(p.mask_s)), 0x01010101u);
+    r.on = p.mask == nullptr ? ~0u : count_word(*reinterpret_cast<const uint32_t*>(p.mask + at(p.mask_s)));
     load4(p.cur, at(p.cur_s), r.cur);
     load4(p.old, at(p.old_s), r.old);
     if (p.adv_rows) {
@@ -183,7 +196,6 @@ __device__ __forceinline__ void load_tokens(const Params& p, unsigned first, Raw
     }
     if (p.ref != nullptr) load4(p.ref, at(p.ref_s), r.ref);
     if (p.ent != nullptr) load4(p.ent, at(p.ent_s), r.ent);
-    r.on = (m * 0x10204080u) >> 28;  // bit 8 j of m to bit j
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
@@ -196,7 +208,7 @@ __device__ __forceinline__ void load_tokens(const Params& p, unsigned first, Raw
       }
       const int64_t b = r.row[j];
       const auto at = [&](int64_t stride) { return p.dense ? int64_t(i) : b * stride + t; };
-      if (p.mask == nullptr || p.mask[at(p.mask_s)] != 0) r.on |= 1u << j;
+      if (p.mask == nullptr || p.mask[at(p.mask_s)] != 0) r.on |= 0xffu << (8 * j);
       r.cur[j] = ld_stream_f1(p.cur + at(p.cur_s));
       r.old[j] = ld_stream_f1(p.old + at(p.old_s));
       r.adv[j] = p.adv_rows ? p.adv[b * p.adv_s] : ld_stream_f1(p.adv + at(p.adv_s));
@@ -206,95 +218,112 @@ __device__ __forceinline__ void load_tokens(const Params& p, unsigned first, Raw
   }
 }
 
-// Whether a token's difference lies above log(1 + clip_high), below log(1 - clip_low), above log(dual).
-struct Side {
-  bool hi, lo, dual;
-};
+__device__ __forceinline__ float sum4(const float (&v)[kPer]) {
+  const float2 s = add2(make_float2(v[0], v[1]), make_float2(v[2], v[3]));
+  return s.x + s.y;
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // Four tokens of one lane: their terms are added in fp32 in a tree and then to the running sums in fp64; g and ge
-// are their gradients.  w: each token's weight.
+// are their gradients.  weight: each token's.  Instructions are what this costs, so a masked-out token is not
+// branched around: its values are cleared by bits, d = 0 and A = 0, and it adds r = 1 alone.
+//   With e = d - mid, d is outside the clip range where |e| > half, and its gradient is cut there where A e > 0
+//   (A > 0 is held at 1 + clip_high, A < 0 at 1 - clip_low).
 __device__ __forceinline__ void take_tokens(const Params& p, const Raw& r, const float (&weight)[kPer], Sums& a,
                                             float (&g)[kPer], float (&ge)[kPer]) {
-  float w[kPer], one[kPer], cur[kPer], s[kPer], A[kPer];
-  Side side[kPer];
+  const uint32_t bits[kPer] = {bits_of<0>(r.on), bits_of<1>(r.on), bits_of<2>(r.on), bits_of<3>(r.on)};
+  float s[kPer], A[kPer], e[kPer];
   bool close = false;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {  // a masked-out token becomes one with d = 0, A = 0 and weight 0
-    const bool on = (r.on >> j) & 1u;
-    w[j] = on ? weight[j] : 0.0f;
-    one[j] = on ? 1.0f : 0.0f;
-    cur[j] = on ? r.cur[j] : 0.0f;
-    A[j] = on ? r.adv[j] : 0.0f;
-    s[j] = on ? __fsub_rn(r.cur[j], r.old[j]) : 0.0f;
-    side[j] = Side{s[j] > p.log_high.hi, s[j] < p.log_low.hi, s[j] > p.log_dual.hi};
-    close |= s[j] == p.log_high.hi || s[j] == p.log_low.hi || s[j] == p.log_dual.hi;
+  for (int j = 0; j < kPer; ++j) {
+    const float d = __fsub_rn(r.cur[j], r.old[j]);
+    A[j] = keep(r.adv[j], bits[j]);
+    s[j] = keep(d, bits[j]);
+    a.max_d = fmaxf(a.max_d, __uint_as_float(__float_as_uint(d) | ~bits[j]));  // a NaN does not count
+    e[j] = s[j] - p.mid;
+    close |= fabsf(fabsf(e[j]) - p.half) <= p.band;
   }
-  if (close) {  // the rounding of a difference decides: look at it
+  if (close) {  // roundings decide: e from the exact differences
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      float d, e;
-      two_diff(r.cur[j], r.old[j], d, e);
-      if ((r.on >> j) & 1u) side[j] = Side{above(d, e, p.log_high), below(d, e, p.log_low), above(d, e, p.log_dual)};
+      float d, rest;
+      two_diff(r.cur[j], r.old[j], d, rest);
+      if (bits[j] != 0u)
+        e[j] = above(d, rest, p.log_high) ? INFINITY : below(d, rest, p.log_low) ? -INFINITY : 0.0f;
     }
   }
-  float ratio[kPer], pg[kPer], diff[kPer], slope[kPer];
+  float ratio[kPer], diff[kPer], pg[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; j += 2) {
     const float2 z = mul2(make_float2(s[j], s[j + 1]), splat2(1.4426950408889634f));
     ratio[j] = exp2_approx(z.x), ratio[j + 1] = exp2_approx(z.y);
-    const float2 d = exp_minus_1_minus(make_float2(s[j], s[j + 1]));
-    diff[j] = d.x, diff[j + 1] = d.y;
   }
+  exp_minus_1_minus(s, diff);
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    // A > 0 is held at 1 + clip_high, A < 0 at 1 - clip_low and at the dual clip; A = 0 adds nothing.
-    const bool up = A[j] > 0.0f, down = A[j] < 0.0f;
-    const bool held = (up && side[j].hi) || (down && (side[j].lo || side[j].dual));
-    const float at = up ? p.high : side[j].lo ? p.low : p.dual;
-    const float value = (held ? at : ratio[j]) * -A[j];
-    pg[j] = up || down || A[j] != A[j] ? value : 0.0f;
-    slope[j] = held ? 0.0f : pg[j];
-    a.max_ratio = fmaxf(a.max_ratio, one[j] * ratio[j]);
-    a.outside += side[j].hi || side[j].lo;
+    // (A = 0 times an infinite e is NaN and not above 0.)
+    const bool out = fabsf(e[j]) > p.half, held = out && A[j] * e[j] > 0.0f;
+    // A ratio beyond fp32 is held at its largest value, so that A = 0 adds 0.
+    const float v = held ? (A[j] > 0.0f ? p.high : p.low) : min_nan(ratio[j], 3.402823466e38f);
+    pg[j] = v * (-A[j] * weight[j]);
+    g[j] = held ? 0.0f : pg[j];
+    if (out) a.outside += 1u;
   }
-  a.tokens += __popc(r.on);
-  float kl[kPer] = {};
-  if (p.ref != nullptr) {
-    float dkl[kPer];
+  if (p.dual < INFINITY) {
 #pragma unroll
-    for (int j = 0; j < kPer; j += 2) {
-      float2 q = make_float2(__fsub_rn(r.ref[j], cur[j]), __fsub_rn(r.ref[j + 1], cur[j + 1]));
-      if (!((r.on >> j) & 1u)) q.x = 0.0f;
-      if (!((r.on >> (j + 1)) & 1u)) q.y = 0.0f;
-      if (p.kl_form == kK1) {
-        kl[j] = -q.x, kl[j + 1] = -q.y;
-        dkl[j] = dkl[j + 1] = 1.0f;
-      } else if (p.kl_form == kK2) {
-        kl[j] = 0.5f * q.x * q.x, kl[j + 1] = 0.5f * q.y * q.y;
-        dkl[j] = -q.x, dkl[j + 1] = -q.y;
-      } else {
-        const float2 k = exp_minus_1_minus(q);
-        kl[j] = k.x, kl[j + 1] = k.y;
-        dkl[j] = -(q.x + k.x), dkl[j + 1] = -(q.y + k.y);  // 1 - exp(q)
+    for (int j = 0; j < kPer; ++j) {
+      float d, rest;
+      two_diff(r.cur[j], r.old[j], d, rest);
+      if (A[j] < 0.0f && above(d, rest, p.log_dual)) {
+        pg[j] = p.dual * (-A[j] * weight[j]);
+        g[j] = 0.0f;
       }
     }
+  }
+  const unsigned n = __popc(r.on) / 8;
+  a.tokens += n;
+  a.skipped += kPer - n;
+  a.pg += double(sum4(pg));
+  a.diff += double(sum4(diff));
+  a.ratio += double(sum4(ratio));
+  if (p.ref != nullptr) {
+    float q[kPer], kl[kPer], dkl[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) slope[j] = fmaf(p.kl_coef, dkl[j], slope[j]);
-    a.kl += double((kl[0] * w[0] + kl[1] * w[1]) + (kl[2] * w[2] + kl[3] * w[3]));
+    for (int j = 0; j < kPer; ++j) q[j] = keep(__fsub_rn(r.ref[j], r.cur[j]), bits[j]);
+    if (p.kl_form == kK1) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) kl[j] = -q[j], dkl[j] = keep(1.0f, bits[j]);
+    } else if (p.kl_form == kK2) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) kl[j] = 0.5f * q[j] * q[j], dkl[j] = -q[j];
+    } else {
+      exp_minus_1_minus(q, kl);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) dkl[j] = -(q[j] + kl[j]);  // 1 - exp(q)
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      g[j] = fmaf(p.kl_coef * weight[j], dkl[j], g[j]);
+      kl[j] *= weight[j];
+    }
+    a.kl += double(sum4(kl));
   }
   if (p.ent != nullptr) {
-    float e[kPer];
+    float h[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) e[j] = ((r.on >> j) & 1u ? r.ent[j] : 0.0f) * w[j];
-    a.ent += double((e[0] + e[1]) + (e[2] + e[3]));
-  }
-  a.pg += double((pg[0] * w[0] + pg[1] * w[1]) + (pg[2] * w[2] + pg[3] * w[3]));
-  a.diff += double((diff[0] + diff[1]) + (diff[2] + diff[3]));
-  a.ratio += double((ratio[0] * one[0] + ratio[1] * one[1]) + (ratio[2] * one[2] + ratio[3] * one[3]));
+    for (int j = 0; j < kPer; ++j) {
+      h[j] = keep(r.ent[j] * weight[j], bits[j]);
+      ge[j] = keep(-p.ent_coef * weight[j], bits[j]);
+    }
+    a.ent += double(sum4(h));
+  } else {
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    g[j] = slope[j] * w[j];
-    ge[j] = -p.ent_coef * w[j];
+    for (int j = 0; j < kPer; ++j) ge[j] = 0.0f;
   }
 }
 
@@ -322,9 +351,10 @@ __device__ __forceinline__ void sum_warp(Sums& a) {
   a.ent = warp_sum(a.ent);
   a.diff = warp_sum(a.diff);
   a.ratio = warp_sum(a.ratio);
-  a.max_ratio = warp_max(a.max_ratio);
+  a.max_d = warp_max(a.max_d);
   a.outside = warp_sum_u32(a.outside);
   a.tokens = warp_sum_u32(a.tokens);
+  a.skipped = warp_sum_u32(a.skipped);
 }
 template <int kW>
 __device__ __forceinline__ void sum_block(Sums& a) {
@@ -335,7 +365,7 @@ __device__ __forceinline__ void sum_block(Sums& a) {
   if (lane == 0) part[w] = a;
   __syncthreads();
   if (w == 0) {
-    a = lane < kW ? part[lane] : Sums{};
+    a = lane < kW ? part[lane] : no_sums();
     sum_warp(a);
   }
 }
@@ -348,8 +378,8 @@ __device__ __forceinline__ void write_outputs(const Params& p, const Sums& a) {
   p.out[3] = float(a.ent);
   p.out[4] = float(double(a.outside) * inv);
   p.out[5] = float(a.diff * inv);
-  p.out[6] = a.max_ratio;
-  p.out[7] = float(a.ratio * inv);
+  p.out[6] = a.tokens > 0u ? exp2_approx(a.max_d * 1.4426950408889634f) : 0.0f;
+  p.out[7] = float((a.ratio - double(a.skipped)) * inv);
 }
 
 // --------------------------------------------------------------------------- few tokens: one CTA
@@ -370,12 +400,12 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_const
   Raw r;
   const unsigned first = first_token<kVec>(0u, kSmallThreads);
   load_tokens<kVec>(p, first, r);
-  const unsigned on = warp_sum_u32(__popc(r.on));
+  const unsigned on = warp_sum_u32(__popc(r.on) / 8);
   if (threadIdx.x % 32 == 0 && on > 0) atomicAdd(&total, on);
   if (per_row) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if ((r.on >> j) & 1u) atomicAdd(&row_tokens[r.row[j]], 1);
+      if ((r.on >> (8 * j)) & 1u) atomicAdd(&row_tokens[r.row[j]], 1);
   }
   __syncthreads();
   if (per_row) {
@@ -383,7 +413,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_const
       if (row_tokens[b] > 0) atomicAdd(&rows, 1u);
     __syncthreads();
   }
-  Sums a = {};
+  Sums a = no_sums();
   float w[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
@@ -400,12 +430,35 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_const
 // each.  Whole-number atomics, so the order does not matter.
 constexpr int kStretch = 4096;
 
-__global__ void __launch_bounds__(kThreads) count_kernel(const Params p, unsigned stretches, Ctl* ctl, int* counts) {
+__device__ __forceinline__ unsigned ones16(const uint4& x) {
+  return __popc(__vminu4(x.x, 0x01010101u)) + __popc(__vminu4(x.y, 0x01010101u)) + __popc(__vminu4(x.z, 0x01010101u)) +
+         __popc(__vminu4(x.w, 0x01010101u));
+}
+
+// Adds the CTA's numbers to the control words.
+__device__ __forceinline__ void add_counts(Ctl* ctl, unsigned tokens, unsigned rows) {
+  __shared__ unsigned part[2][kThreads / 32];
+  tokens = warp_sum_u32(tokens);
+  rows = warp_sum_u32(rows);
+  if (threadIdx.x % 32 == 0) part[0][threadIdx.x / 32] = tokens, part[1][threadIdx.x / 32] = rows;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const bool in = threadIdx.x < kThreads / 32;
+    tokens = warp_sum_u32(in ? part[0][threadIdx.x] : 0u);
+    rows = warp_sum_u32(in ? part[1][threadIdx.x] : 0u);
+    if (threadIdx.x == 0) {
+      if (tokens > 0) atomicAdd(&ctl->tokens, (unsigned long long)(tokens));
+      if (rows > 0) atomicAdd(&ctl->rows, rows);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) count_rows_kernel(const __grid_constant__ Params p, unsigned stretches,
+                                                              Ctl* ctl, int* counts) {
   pdl_begin();
   const unsigned lane = threadIdx.x % 32;
   const uint64_t warps = uint64_t(gridDim.x) * (kThreads / 32);
-  unsigned long long tokens = 0;
-  unsigned rows = 0;
+  unsigned tokens = 0, rows = 0;
   for (uint64_t u = uint64_t(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32; u < uint64_t(p.B) * stretches; u += warps) {
     const int64_t b = int64_t(u / stretches);
     const int t0 = int(u - uint64_t(b) * stretches) * kStretch;
@@ -418,11 +471,7 @@ __global__ void __launch_bounds__(kThreads) count_kernel(const Params p, unsigne
     if (tail + int(lane) < len) c += m[tail + lane] != 0;
     const uint4* v = reinterpret_cast<const uint4*>(m + head);
 #pragma unroll 4
-    for (int i = lane; i < vecs; i += 32) {
-      const uint4 x = __ldg(v + i);
-      c += __popc(__vminu4(x.x, 0x01010101u)) + __popc(__vminu4(x.y, 0x01010101u)) +
-           __popc(__vminu4(x.z, 0x01010101u)) + __popc(__vminu4(x.w, 0x01010101u));
-    }
+    for (int i = lane; i < vecs; i += 32) c += ones16(__ldg(v + i));
     c = warp_sum_u32(c);
     if (lane == 0 && c > 0) {
       if (p.reduction == kSequenceMean)
@@ -430,22 +479,28 @@ __global__ void __launch_bounds__(kThreads) count_kernel(const Params p, unsigne
       tokens += c;
     }
   }
-  __shared__ unsigned long long s_tokens;
-  __shared__ unsigned s_rows;
-  if (threadIdx.x == 0) s_tokens = 0ull, s_rows = 0u;
-  __syncthreads();
-  if (lane == 0 && tokens > 0) {
-    atomicAdd(&s_tokens, tokens);
-    atomicAdd(&s_rows, rows);
-  }
-  __syncthreads();
-  if (threadIdx.x == 0 && s_tokens > 0) {
-    atomicAdd(&ctl->tokens, s_tokens);
-    if (s_rows > 0) atomicAdd(&ctl->rows, s_rows);
-  }
+  add_counts(ctl, tokens, rows);
 }
 
-// What the counts say, for every CTA of a kernel behind count_kernel.
+// All tokens of a dense mask on a 16-byte boundary.
+__global__ void __launch_bounds__(kThreads) count_all_kernel(const uint8_t* __restrict__ mask, unsigned n, Ctl* ctl) {
+  pdl_begin();
+  const uint4* v = reinterpret_cast<const uint4*>(mask);
+  const unsigned vecs = n / 16, threads = gridDim.x * kThreads, id = blockIdx.x * kThreads + threadIdx.x;
+  unsigned c = 0;
+  for (unsigned i = id; i < vecs; i += 4 * threads) {
+    uint4 x[4];
+#pragma unroll
+    for (unsigned k = 0; k < 4; ++k)
+      x[k] = i + k * threads < vecs ? __ldg(v + i + k * threads) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c += ones16(x[k]);
+  }
+  if (id < n - vecs * 16) c += mask[vecs * 16 + id] != 0;
+  add_counts(ctl, c, 0u);
+}
+
+// What the counts say, for every CTA of a kernel behind a count kernel.
 struct Counts {
   unsigned long long tokens;
   unsigned rows;
@@ -461,7 +516,7 @@ __device__ __forceinline__ void finish(const Params& p, Sums& a, bool counted, C
   sum_block<kThreads / 32>(a);
   if (threadIdx.x == 0) sums[blockIdx.x] = a;
   if (!elect_last_cta(&ctl->done)) return;
-  a = Sums{};
+  a = no_sums();
   for (unsigned i = threadIdx.x; i < gridDim.x; i += kThreads) {
     const Sums& s = sums[i];
     a.pg += __ldcg(&s.pg);
@@ -469,9 +524,10 @@ __device__ __forceinline__ void finish(const Params& p, Sums& a, bool counted, C
     a.ent += __ldcg(&s.ent);
     a.diff += __ldcg(&s.diff);
     a.ratio += __ldcg(&s.ratio);
-    a.max_ratio = fmaxf(a.max_ratio, __ldcg(&s.max_ratio));
+    a.max_d = fmaxf(a.max_d, __ldcg(&s.max_d));
     a.outside += __ldcg(&s.outside);
     a.tokens += __ldcg(&s.tokens);
+    a.skipped += __ldcg(&s.skipped);
   }
   sum_block<kThreads / 32>(a);
   if (threadIdx.x == 0) {
@@ -487,15 +543,15 @@ __device__ __forceinline__ void finish(const Params& p, Sums& a, bool counted, C
 template <bool kVec>
 __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__ Params p, bool counted, Ctl* ctl,
                                                          int* counts, Sums* sums) {
-  constexpr unsigned kUnit = kThreads * kPer;
-  const unsigned units = (p.n + kUnit - 1) / kUnit;
+  constexpr unsigned kStretchTokens = kThreads * kPer;
+  const unsigned units = (p.n + kStretchTokens - 1) / kStretchTokens;
   pdl_begin();
   const bool per_row = p.reduction == kSequenceMean;
   const Counts c = read_counts(p, counted, ctl);
   float w[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) w[j] = j == 0 ? token_weight(p, c.tokens, c.rows, p.T) : w[0];
-  Sums a = {};
+  Sums a = no_sums();
   for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
     const unsigned first = first_token<kVec>(u, kThreads);
     Raw r;
@@ -512,12 +568,13 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__
 }
 
 // Dense streams on 16-byte boundaries: stretches of kUnit tokens arrive in shared memory by bulk copies, kStages
-// ahead, so that loads never wait for arithmetic.  A thread has four consecutive tokens.  What is left of
+// ahead, so that loads never wait for arithmetic.  A thread has kVecs times four consecutive tokens.  What is left of
 // less than a stretch goes through registers.
-// Behind count_kernel the copies start before the counts are there: every CTA of count_kernel lets this kernel
+// Behind a count kernel the copies start before the counts are there: every CTA of that lets this kernel
 // start only after it has itself waited for the kernels before it, so the inputs are complete.
-constexpr int kStages = 4;
-constexpr unsigned kUnit = kThreads * kPer;
+constexpr int kStages = 2;
+constexpr int kVecs = 2;  // vectors of kPer tokens per thread and stretch
+constexpr unsigned kUnit = kThreads * kPer * kVecs;
 constexpr unsigned kStreamBytes = kUnit * 4u;
 
 struct Streams {
@@ -526,7 +583,7 @@ struct Streams {
   int n;              // streams that are there
 };
 
-__global__ void __launch_bounds__(kThreads, 2) dense_kernel(const __grid_constant__ Params p,
+__global__ void __launch_bounds__(kThreads, 3) dense_kernel(const __grid_constant__ Params p,
                                                             const __grid_constant__ Streams st, bool counted, Ctl* ctl,
                                                             int* counts, Sums* sums) {
   extern __shared__ __align__(128) char smem[];
@@ -557,57 +614,59 @@ __global__ void __launch_bounds__(kThreads, 2) dense_kernel(const __grid_constan
   float w[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) w[j] = j == 0 ? token_weight(p, c.tokens, c.rows, p.T) : w[0];
-  Sums a = {};
+  Sums a = no_sums();
   unsigned stage = 0, parity = 0;
   for (unsigned u = blockIdx.x; u < whole; u += gridDim.x) {
-    const unsigned first = u * kUnit + threadIdx.x * kPer;
-    Raw r;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) r.ref[j] = r.ent[j] = r.adv[j] = 0.0f;
-    if (p.need_row) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) r.row[j] = j > 0 && p.T % kPer == 0 ? r.row[0] : p.by_T.div(first + j);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        if (per_row && counted) w[j] = token_weight(p, c.tokens, c.rows, counts[r.row[j]]);
-        if (p.adv_rows) r.adv[j] = p.adv[int64_t(r.row[j]) * p.adv_s];
-      }
-    }
     mbar_wait(&full[stage], parity);
-    const char* src = smem + stage * stage_bytes + threadIdx.x * (kPer * 4);
-    const auto take4 = [&](int s, float (&f)[kPer]) {
-      const float4 v = *reinterpret_cast<const float4*>(src + st.slot[s] * kStreamBytes);
-      f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-    };
-    take4(0, r.cur);
-    take4(1, r.old);
-    if (!p.adv_rows) take4(2, r.adv);
-    if (p.ref != nullptr) take4(3, r.ref);
-    if (p.ent != nullptr) take4(4, r.ent);
-    uint32_t m = 0x01010101u;
-    if (p.mask != nullptr)
-      m = __vminu4(*reinterpret_cast<const uint32_t*>(smem + stage * stage_bytes + st.n * kStreamBytes +
-                                                      threadIdx.x * kPer),
-                   0x01010101u);
-    r.on = (m * 0x10204080u) >> 28;  // bit 8 j of m to bit j
+    const char* base = smem + stage * stage_bytes;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const unsigned at = k * kThreads + threadIdx.x, first = u * kUnit + at * kPer;
+      Raw r;
+      const auto take4 = [&](int s, float (&f)[kPer]) {
+        const float4 v = *reinterpret_cast<const float4*>(base + st.slot[s] * kStreamBytes + at * (kPer * 4));
+        f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+      };
+      if (p.need_row) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const bool again = j > 0 && p.T % kPer == 0;  // the first token's row
+          const unsigned row = again ? r.row[0] : p.by_T.div(first + j);
+          r.row[j] = row;
+          if (per_row && counted) w[j] = again ? w[0] : token_weight(p, c.tokens, c.rows, counts[row]);
+          if (p.adv_rows) r.adv[j] = again ? r.adv[0] : p.adv[int64_t(row) * p.adv_s];
+        }
+      }
+      take4(0, r.cur);
+      take4(1, r.old);
+      if (!p.adv_rows) take4(2, r.adv);
+      if (p.ref != nullptr) take4(3, r.ref);
+      if (p.ent != nullptr) take4(4, r.ent);
+      r.on = p.mask == nullptr
+                 ? ~0u
+                 : count_word(*reinterpret_cast<const uint32_t*>(base + st.n * kStreamBytes + at * kPer));
+      float g[kPer], ge[kPer];
+      take_tokens(p, r, w, a, g, ge);
+      write_tokens<true>(p, first, g, ge);
+    }
     __syncthreads();  // the stage is read
     if (threadIdx.x == 0) fetch(u + kStages * gridDim.x, stage);
     if (++stage == unsigned(kStages)) stage = 0, parity ^= 1u;
-    float g[kPer], ge[kPer];
-    take_tokens(p, r, w, a, g, ge);
-    write_tokens<true>(p, first, g, ge);
   }
   if (blockIdx.x == gridDim.x - 1 && whole * kUnit < p.n) {
-    const unsigned first = first_token<true>(whole, kThreads);
-    Raw r;
-    load_tokens<true>(p, first, r);
-    if (per_row && counted) {
+#pragma unroll 1
+    for (unsigned v = 0; v < unsigned(kVecs); ++v) {
+      const unsigned first = whole * kUnit + (v * kThreads + threadIdx.x) * kPer;
+      Raw r;
+      load_tokens<true>(p, first, r);
+      if (per_row && counted) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) w[j] = token_weight(p, c.tokens, c.rows, counts[r.row[j]]);
+        for (int j = 0; j < kPer; ++j) w[j] = token_weight(p, c.tokens, c.rows, counts[r.row[j]]);
+      }
+      float g[kPer], ge[kPer];
+      take_tokens(p, r, w, a, g, ge);
+      write_tokens<true>(p, first, g, ge);
     }
-    float g[kPer], ge[kPer];
-    take_tokens(p, r, w, a, g, ge);
-    write_tokens<true>(p, first, g, ge);
   }
   finish(p, a, counted, ctl, counts, sums);
 }
@@ -627,7 +686,7 @@ inline int run(const float* cur, const float* old, const float* adv, const float
                double dual_clip, double kl_coef, int kl_form, double ent_coef, int reduction, double scale, float* out,
                float* grad, float* grad_ent, void* ws, int64_t ws_bytes, cudaStream_t stream) {
   if (B < 0 || T < 0 || out == nullptr || strides == nullptr) return kInvalidArgument;
-  if (!(clip_low >= 0.0 && clip_low < 1.0) || !(clip_high >= 0.0) || !(dual_clip == 0.0 || dual_clip > 1.0))
+  if (!(clip_low >= 0.0 && clip_low < 1.0) || !(clip_high >= 0.0 && clip_high < INFINITY) || !(dual_clip == 0.0 || dual_clip > 1.0))
     return kInvalidArgument;
   if (kl_form < kK1 || kl_form > kK3 || reduction < kTokenMean || reduction > kSum) return kInvalidArgument;
   for (int i = 0; i < 7; ++i)
@@ -653,7 +712,13 @@ inline int run(const float* cur, const float* old, const float* adv, const float
   p.need_row = !p.dense || p.adv_rows || reduction == kSequenceMean;
   p.log_high = make_pair_of(log1p(clip_high)), p.log_low = make_pair_of(log1p(-clip_low));
   p.log_dual = make_pair_of(dual_clip > 0.0 ? log(dual_clip) : double(NAN));  // NaN: no difference is it
-  p.high = float(1.0 + clip_high), p.low = float(1.0 - clip_low), p.dual = float(dual_clip);
+  {
+    // d - mid and half carry some roundings relative to the borders' sizes: band covers them.
+    const double H = log1p(clip_high), L = log1p(-clip_low);
+    p.mid = float((H + L) / 2), p.half = float((H - L) / 2);
+    p.band = float((fabs(H) + fabs(L)) * 1e-6) + 1e-30f;
+  }
+  p.high = float(1.0 + clip_high), p.low = float(1.0 - clip_low), p.dual = dual_clip > 0.0 ? float(dual_clip) : INFINITY;
   p.kl_coef = float(kl_coef), p.ent_coef = float(ent_coef), p.kl_form = kl_form, p.reduction = reduction;
   p.scale = float(scale), p.kl_coef_d = kl_coef, p.ent_coef_d = ent_coef;
   p.grad = grad, p.grad_ent = grad_ent, p.out = out;
@@ -673,15 +738,22 @@ inline int run(const float* cur, const float* old, const float* adv, const float
   int* counts = reinterpret_cast<int*>(w + 256 + kSumsBytes);
   const bool counted = mask != nullptr && reduction != kSum;
   if (counted) {
-    const unsigned stretches = unsigned((int64_t(T) + kStretch - 1) / kStretch);
-    const int64_t warps = int64_t(B) * stretches;
-    const int64_t want = (warps + kThreads / 32 - 1) / (kThreads / 32), most = int64_t(sm_count()) * 4;
-    const int st = launch_pdl(count_kernel, dim3(unsigned(want < most ? want : most)), dim3(kThreads), 0, stream, p,
-                              stretches, ctl, counts);
+    int st;
+    if (reduction == kTokenMean && (p.mask_s == T || B == 1) && aligned16(mask)) {
+      const int64_t want = (n / 16 + 4 * kThreads - 1) / (4 * kThreads), most = int64_t(sm_count()) * 2;
+      st = launch_pdl(count_all_kernel, dim3(unsigned(want < 1 ? 1 : want < most ? want : most)), dim3(kThreads), 0,
+                      stream, mask, p.n, ctl);
+    } else {
+      const unsigned stretches = unsigned((int64_t(T) + kStretch - 1) / kStretch);
+      const int64_t warps = int64_t(B) * stretches;
+      const int64_t want = (warps + kThreads / 32 - 1) / (kThreads / 32), most = int64_t(sm_count()) * 4;
+      st = launch_pdl(count_rows_kernel, dim3(unsigned(want < most ? want : most)), dim3(kThreads), 0, stream, p,
+                      stretches, ctl, counts);
+    }
     if (st != kOk) return st;
   }
-  const int64_t units = (n + kUnit - 1) / kUnit;
-  const auto grid = [&](int per_sm) {
+  const auto grid = [&](int per_sm, unsigned stretch) {
+    const int64_t units = (n + stretch - 1) / stretch;
     const int64_t most = int64_t(sm_count()) * per_sm;
     return unsigned(most < units ? (most < kMaxCtas ? most : kMaxCtas) : (units < kMaxCtas ? units : kMaxCtas));
   };
@@ -694,11 +766,11 @@ inline int run(const float* cur, const float* old, const float* adv, const float
     }
     const int smem = kStages * int(unsigned(st.n) * kStreamBytes + (mask != nullptr ? kUnit : 0u));
     if (!ensure_dyn_smem(dense_kernel, smem)) return kCudaError;
-    return launch_pdl(dense_kernel, dim3(grid(resident_ctas_per_sm(dense_kernel, kThreads, size_t(smem)))),
+    return launch_pdl(dense_kernel, dim3(grid(resident_ctas_per_sm(dense_kernel, kThreads, size_t(smem)), kUnit)),
                       dim3(kThreads), size_t(smem), stream, p, st, counted, ctl, counts, sums);
   }
   const auto kernel = p.vec ? token_kernel<true> : token_kernel<false>;
-  return launch_pdl(kernel, dim3(grid(resident_ctas_per_sm(kernel, kThreads, 0))), dim3(kThreads), 0, stream, p, counted,
+  return launch_pdl(kernel, dim3(grid(resident_ctas_per_sm(kernel, kThreads, 0), kThreads * kPer)), dim3(kThreads), 0, stream, p, counted,
                     ctl, counts, sums);
 }
 
