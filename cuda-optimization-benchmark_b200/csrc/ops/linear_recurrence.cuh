@@ -173,16 +173,28 @@ __device__ __forceinline__ void store_row(float* p, int c, int H, float2 y) {
   if (c < H) p[0] = y.x;
   if (c + 1 < H) p[1] = y.y;
 }
-// One row of an output: 4 bytes where rows are aligned to them and hold whole lanes, element by element
-// otherwise.
+// One row of an output (whole warps).  wide: rows are aligned to 4 bytes and hold whole lanes.  Otherwise 16-bit
+// rows may start between two words: each lane then writes the word of its left neighbour's second and its own
+// first channel, and the ends are written alone.
 template <typename T>
 __device__ __forceinline__ void store_out(T* p, int c, int H, bool wide, typename Lane<T>::V y) {
   const uint32_t u = Lane<T>::pack(y);
   if (wide || sizeof(T) == 4) {
     if (c < H) *reinterpret_cast<uint32_t*>(p) = u;
+    return;
+  }
+  const unsigned lane = threadIdx.x % 32;
+  uint16_t* q = reinterpret_cast<uint16_t*>(p);
+  const bool off = (reinterpret_cast<uintptr_t>(p) & 2u) != 0;  // the same in all lanes
+  const uint32_t left = __shfl_up_sync(0xffffffffu, u, 1);
+  if (off) {
+    if (lane > 0 && c < H) *reinterpret_cast<uint32_t*>(q - 1) = __byte_perm(left, u, 0x5432);
+    if (lane > 0 && c == H) q[-1] = uint16_t(left >> 16);
+    if (lane == 0 && c < H) q[0] = uint16_t(u);
+    if (lane == 31 && c + 1 < H) q[1] = uint16_t(u >> 16);
   } else {
-    if (c < H) reinterpret_cast<uint16_t*>(p)[0] = uint16_t(u);
-    if (c + 1 < H) reinterpret_cast<uint16_t*>(p)[1] = uint16_t(u >> 16);
+    if (c + 1 < H) *reinterpret_cast<uint32_t*>(q) = u;
+    else if (c < H) q[0] = uint16_t(u);
   }
 }
 
@@ -211,21 +223,46 @@ __device__ __forceinline__ void copy_rows_by(char* dst, const char* src, int64_t
 }
 
 // `rows` rows of `width` bytes (at most 128), pitch bytes apart, into a tile buffer.  `granule` bytes
-// divide the source address and the pitch; 2-byte granules (16-bit rows at odd elements) go through
-// registers, which cp.async cannot copy.
-__device__ __forceinline__ void copy_rows(char* dst, const char* src, int64_t pitch, int rows, int width,
-                                          int granule) {
-  if (granule == 16)
+// divide the source address and the pitch.  Rows of 16-bit elements off 4 bytes are copied with the 4-byte word
+// that their first element lies in, the word behind the row's 32 goes to more[r], and align_rows() shifts
+// them to their place.
+__device__ __forceinline__ void copy_rows(char* dst, uint32_t* more, const char* src, int64_t pitch, int rows,
+                                          int width, int granule) {
+  if (granule == 16) {
     copy_rows_by<16>(dst, src, pitch, rows, width);
-  else if (granule == 8)
+  } else if (granule == 8) {
     copy_rows_by<8>(dst, src, pitch, rows, width);
-  else if (granule == 4)
+  } else if (granule == 4) {
     copy_rows_by<4>(dst, src, pitch, rows, width);
-  else
-    for (int r = int(threadIdx.x) / 64, o = int(threadIdx.x % 64) * 2; r < rows; r += kThreads / 64)
-      if (o < width)
-        *reinterpret_cast<uint16_t*>(dst + r * kRowBytes + o) =
-            *reinterpret_cast<const uint16_t*>(src + r * pitch + o);
+  } else {
+    const int lane = int(threadIdx.x % 32);
+    for (int r = int(threadIdx.x) / 32; r < rows; r += kWarps) {
+      const char* s = src + r * pitch;
+      const int off = int(reinterpret_cast<uintptr_t>(s) & 2u), left = width + off - lane * 4;
+      if (left > 0) cp_async<4>(dst + r * kRowBytes + lane * 4, s - off + lane * 4, left < 4 ? left : 4);
+    }
+    const int r = int(threadIdx.x);
+    if (r < rows) {
+      const char* s = src + r * pitch;
+      const int off = int(reinterpret_cast<uintptr_t>(s) & 2u), left = width + off - kRowBytes;
+      if (left > 0) cp_async<4>(reinterpret_cast<char*>(more + r), s - off + kRowBytes, left);
+    }
+  }
+}
+
+// A warp's own rows, shifted where they were copied from an address off 4 bytes.
+__device__ __forceinline__ void align_rows(char* dst, const uint32_t* more, const char* src, int64_t pitch, int rows) {
+  const int lane = int(threadIdx.x % 32);
+  for (int r = 0; r < rows; ++r) {
+    if ((reinterpret_cast<uintptr_t>(src + r * pitch) & 2u) == 0) continue;
+    uint32_t* row = reinterpret_cast<uint32_t*>(dst + r * kRowBytes);
+    const uint32_t lo = row[lane];
+    uint32_t hi = __shfl_down_sync(0xffffffffu, lo, 1);
+    if (lane == 31) hi = more[r];
+    __syncwarp();
+    row[lane] = __funnelshift_r(lo, hi, 16);
+  }
+  __syncwarp();
 }
 
 // ------------------------------------------------------------------------------- tiles and records
@@ -261,10 +298,10 @@ struct __align__(2 * sizeof(V)) Map {
 };
 
 // Shared memory beside the tile buffers.
-template <typename V>
+template <typename V, bool kBack>
 struct Shared {
   Map<V> map[kWarps][32];        // the warps' maps (scan direction)
-  V fwd[kWarps][32];             // the warps' forward offsets (backward kernel; the factor is map.x)
+  V fwd[kBack ? kWarps - 1 : 1][32];  // the warps' forward offsets (backward kernel; the factor is map.x)
   Map<V> look[kMaxSpan][32];     // records of the tiles before this one
   unsigned look_cut[kMaxSpan];
   unsigned cut[kWarps];          // the warp's steps hold a reset: its map does not see what comes in
@@ -336,9 +373,9 @@ __device__ __forceinline__ void take_record(const ulonglong2* r, int c, int H, u
 
 // What comes into tile t from the tiles before it, for this lane's channels: y on entry is the value
 // before tile 0.  Every thread of the CTA calls it.
-template <typename V>
+template <typename V, bool kBack>
 __device__ __forceinline__ void incoming(const Grid& g, const Tile& t, int64_t B, int c, unsigned epoch,
-                                         Shared<V>& sh, V& y) {
+                                         Shared<V, kBack>& sh, V& y) {
   if (t.k == 0) return;
   const unsigned q = t.k & (g.span - 1);              // tiles of the block before this one
   const unsigned n = q + (t.k >= g.span ? 1u : 0u);   // their maps, and the state at the block's start
@@ -405,8 +442,14 @@ struct __align__(64) Input {
 };
 
 template <typename T>
-__device__ __forceinline__ void load_tile(const Input<T>& in, char* dst, const Tile& t, int64_t t0, int64_t Tn, int H,
-                                          bool tma, int granule, uint64_t* bar) {
+__device__ __forceinline__ const char* row_address(const Input<T>& in, const Tile& t, int64_t step) {
+  return reinterpret_cast<const char*>(in.p + t.b * in.s.b + step * in.s.t +
+                                       int64_t(t.group) * (kRowBytes / int(sizeof(T))));
+}
+
+template <typename T>
+__device__ __forceinline__ void load_tile(const Input<T>& in, char* dst, uint32_t* more, const Tile& t, int64_t t0,
+                                          const Grid& g, bool tma, int granule, uint64_t* bar) {
   constexpr int kGroup = kRowBytes / int(sizeof(T));
   const int c0 = int(t.group) * kGroup;
   if (tma) {  // one thread
@@ -417,10 +460,25 @@ __device__ __forceinline__ void load_tile(const Input<T>& in, char* dst, const T
         "l"(&in.map), "r"(c0), "r"(in.swap ? b : a), "r"(in.swap ? a : b), "r"(smem_addr(bar))
         : "memory");
   } else {
-    const int rows = int(Tn - t0 < kTile ? Tn - t0 : kTile);
-    copy_rows(dst, reinterpret_cast<const char*>(in.p + t.b * in.s.b + t0 * in.s.t + c0), in.s.t * int64_t(sizeof(T)),
-              rows, min(kGroup, H - c0) * int(sizeof(T)), granule);
+    copy_rows(dst, more, row_address(in, t, t0), in.s.t * int64_t(sizeof(T)), int(g.T - t0 < kTile ? g.T - t0 : kTile),
+              min(kGroup, g.H - c0) * int(sizeof(T)), granule);
   }
+}
+// Behind the copies, where they were of unaligned rows: this warp's rows (n of them, from step t0).
+template <typename T>
+__device__ __forceinline__ void align_tile(const Input<T>& in, char* rows, const uint32_t* more, const Tile& t,
+                                           int64_t t0, int n) {
+  align_rows(rows, more, row_address(in, t, t0), in.s.t * int64_t(sizeof(T)), n);
+}
+
+// Dynamic shared memory: kIn inputs in two buffers, and the words behind the rows of unaligned copies.
+template <int kIn>
+constexpr int smem_bytes(int granule) {
+  return 2 * kIn * (kBufBytes + (granule == 2 ? kTile * 4 : 0));
+}
+template <int kIn>
+__device__ __forceinline__ uint32_t* more_of(char* smem, int buf, int in) {
+  return reinterpret_cast<uint32_t*>(smem + 2 * kIn * kBufBytes) + (buf * kIn + in) * kTile;
 }
 
 // ------------------------------------------------------------------------------------- forward
@@ -439,6 +497,7 @@ struct Forward {
 };
 
 // Step 1 of the warp: a and v = u of its n steps, and their map.  kAny: fewer steps than kSteps, or resets.
+// (In the decay form a and u are the inputs themselves, which step 4 reads again instead.)
 template <typename T, int kForm, bool kAny, typename V>
 __device__ __forceinline__ void forward_map(const char* row, unsigned resets, int n, V (&a)[kSteps], V (&u)[kSteps],
                                             Map<V>& m) {
@@ -448,41 +507,55 @@ __device__ __forceinline__ void forward_map(const char* row, unsigned resets, in
     if (kAny && i >= n) break;
     const uint32_t gt = *reinterpret_cast<const uint32_t*>(row + i * kRowBytes);
     const V xv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
+    V ai, ui;
     if (kForm == kDecay) {
-      a[i] = Lane<T>::unpack(gt);
-      u[i] = xv;
+      ai = Lane<T>::unpack(gt);
+      ui = xv;
     } else {
       V na;
-      sigmoid_pair(Lane<T>::unpack_gate(gt), a[i], na);
-      u[i] = vmul(na, xv);
+      sigmoid_pair(Lane<T>::unpack_gate(gt), ai, na);
+      ui = vmul(na, xv);
+      a[i] = ai;
+      u[i] = ui;
     }
     if (kAny && ((resets >> i) & 1u)) m = Map<V>{vset(V{}, 0.0f), vset(V{}, 0.0f)};
-    m.b = vfma(a[i], m.b, u[i]);
-    m.x = vmul(m.x, a[i]);
+    m.b = vfma(ai, m.b, ui);
+    m.x = vmul(m.x, ai);
   }
 }
 
 // Step 4: the warp's steps from its incoming state y, written to out.  !kAny: kSteps steps without resets,
 // 4-byte stores.
-template <typename T, bool kAny, typename V>
-__device__ __forceinline__ void forward_steps(const V (&a)[kSteps], const V (&u)[kSteps], unsigned resets, int n,
-                                              int c, int H, bool wide, T* out, int64_t pitch, V& y) {
+template <typename T, int kForm, bool kAny, typename V>
+__device__ __forceinline__ void forward_steps(const char* row, const V (&a)[kSteps], const V (&u)[kSteps],
+                                              unsigned resets, int n, int c, int H, bool wide, T* out, int64_t pitch,
+                                              V& y) {
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     if (kAny && i >= n) break;
     if (kAny && ((resets >> i) & 1u)) y = vset(V{}, 0.0f);
-    y = vfma(a[i], y, u[i]);
+    if (kForm == kDecay)
+      y = vfma(Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + i * kRowBytes)), y,
+               Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes)));
+    else
+      y = vfma(a[i], y, u[i]);
     store_out<T>(out, c, H, !kAny || wide, y);
     out += pitch;
   }
 }
 
+// CTAs per SM: three where shared memory allows (the records' buffer of two-channel lanes does not).
+template <typename T>
+constexpr int forward_ctas() {
+  return sizeof(T) == 4 ? 3 : 2;
+}
+
 template <typename T, int kForm>
-__global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_constant__ Forward<T> p) {
+__global__ void __launch_bounds__(kThreads, forward_ctas<T>()) forward_kernel(const __grid_constant__ Forward<T> p) {
   using V = typename Lane<T>::V;
   constexpr int kVec = Lane<T>::kVec, kGroup = 32 * kVec;
   extern __shared__ __align__(128) char smem[];
-  __shared__ Shared<V> sh;
+  __shared__ Shared<V, false> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
@@ -492,8 +565,8 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
       const int64_t t0 = int64_t(t.k) * kTile;
       char* dst = smem + buf * 2 * kBufBytes;
       if (p.tma) mbar_arrive_expect_tx(&sh.full[buf], 2 * kBufBytes);
-      load_tile(p.gate, dst, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
-      load_tile(p.x, dst + kBufBytes, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
+      load_tile(p.gate, dst, more_of<2>(smem, buf, 0), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
+      load_tile(p.x, dst + kBufBytes, more_of<2>(smem, buf, 1), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
     }
     if (!p.tma) cp_commit();
   };
@@ -536,11 +609,16 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
     const int64_t t0 = int64_t(t.k) * kTile + w * kSteps;  // this warp's first step
     const int n = int(p.g.T - t0 < kSteps ? p.g.T - t0 : kSteps);  // its steps (0 or less: none)
     const int c = int(t.group) * kGroup + int(lane) * kVec;
-    const char* row = smem + buf * 2 * kBufBytes + w * kSteps * kRowBytes + lane * 4;
+    char* rows = smem + buf * 2 * kBufBytes + w * kSteps * kRowBytes;
+    if (p.granule == 2) {
+      align_tile(p.gate, rows, more_of<2>(smem, buf, 0) + w * kSteps, t, t0, n);
+      align_tile(p.x, rows + kBufBytes, more_of<2>(smem, buf, 1) + w * kSteps, t, t0, n);
+    }
+    const char* row = rows + lane * 4;
     const int64_t state_at = int64_t(t.b) * p.g.H + c;
 
     // 1. The warp's steps as one map per channel; a and v stay in registers for step 4.
-    V a[kSteps], u[kSteps];
+    V a[kSteps], u[kSteps];  // (decay: not used)
     Map<V> m;
     const bool plain = resets == 0 && n >= kSteps;
     if (plain)
@@ -580,9 +658,9 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
     // 4. The steps from there.
     T* out = p.h + t.b * p.hs.b + t0 * p.hs.t + c;
     if (plain && p.wide)
-      forward_steps<T, false>(a, u, 0u, kSteps, c, p.g.H, p.wide, out, p.hs.t, y);
+      forward_steps<T, kForm, false>(row, a, u, 0u, kSteps, c, p.g.H, p.wide, out, p.hs.t, y);
     else
-      forward_steps<T, true>(a, u, resets, n, c, p.g.H, p.wide, out, p.hs.t, y);
+      forward_steps<T, kForm, true>(row, a, u, resets, n, c, p.g.H, p.wide, out, p.hs.t, y);
     if (p.final_state != nullptr && n > 0 && t0 + n == p.g.T) store_row(p.final_state + state_at, c, p.g.H, y);
     t = next;
   }
@@ -684,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
   using V = typename Lane<T>::V;
   constexpr int kVec = Lane<T>::kVec, kGroup = 32 * kVec;
   extern __shared__ __align__(128) char smem[];
-  __shared__ Shared<V> sh;
+  __shared__ Shared<V, true> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
@@ -694,9 +772,9 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
       const int64_t t0 = int64_t(p.g.n_tiles - 1 - t.k) * kTile;
       char* dst = smem + buf * 3 * kBufBytes;
       if (p.tma) mbar_arrive_expect_tx(&sh.full[buf], 3 * kBufBytes);
-      load_tile(p.gate, dst, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
-      load_tile(p.x, dst + kBufBytes, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
-      load_tile(p.dh, dst + 2 * kBufBytes, t, t0, p.g.T, p.g.H, p.tma, p.granule, &sh.full[buf]);
+      load_tile(p.gate, dst, more_of<3>(smem, buf, 0), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
+      load_tile(p.x, dst + kBufBytes, more_of<3>(smem, buf, 1), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
+      load_tile(p.dh, dst + 2 * kBufBytes, more_of<3>(smem, buf, 2), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
     }
     if (!p.tma) cp_commit();
   };
@@ -743,7 +821,13 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
     prefetch(next, buf ^ 1);
     reset_byte = load_reset(next);
     if (threadIdx.x == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
-    const char* row = smem + buf * 3 * kBufBytes + w * kSteps * kRowBytes + lane * 4;
+    char* rows = smem + buf * 3 * kBufBytes + w * kSteps * kRowBytes;
+    if (p.granule == 2) {
+      align_tile(p.gate, rows, more_of<3>(smem, buf, 0) + w * kSteps, t, t0, n);
+      align_tile(p.x, rows + kBufBytes, more_of<3>(smem, buf, 1) + w * kSteps, t, t0, n);
+      align_tile(p.dh, rows + 2 * kBufBytes, more_of<3>(smem, buf, 2) + w * kSteps, t, t0, n);
+    }
+    const char* row = rows + lane * 4;
 
     // 1. The warp's forward and backward maps.
     V a[kSteps], na[kSteps], d[kSteps], f;
@@ -754,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
     else
       backward_map<T, kForm, true>(row, resets, n, a, na, f, m);
     sh.map[w][lane] = m;
-    sh.fwd[w][lane] = f;
+    if (w < kWarps - 1) sh.fwd[w][lane] = f;  // (no warp comes after the last)
     if (lane == 0) sh.cut[w] = resets != 0;
     __syncthreads();
 
@@ -968,11 +1052,11 @@ inline int forward(const void* gate, const void* x, int dtype, int form, const i
       p.tma = make_input_map(&p.gate, B, T, H) && make_input_map(&p.x, B, T, H);
       p.granule = in.bytes();
       p.wide = out.bytes() >= 4 && H % Lane<E>::kVec == 0;
-      constexpr int kSmem = 4 * kBufBytes;
+      const int smem = smem_bytes<2>(p.granule);
       const auto kernel = forward_kernel<E, f.value>;
       unsigned ctas = 0;
-      const int st = plan(kernel, kSmem, Lane<E>::kVec, B, T, H, ws, ws_bytes, &p.g, &ctas);
-      return st != kOk ? st : launch_pdl(kernel, dim3(ctas), dim3(kThreads), kSmem, stream, p);
+      const int st = plan(kernel, smem, Lane<E>::kVec, B, T, H, ws, ws_bytes, &p.g, &ctas);
+      return st != kOk ? st : launch_pdl(kernel, dim3(ctas), dim3(kThreads), size_t(smem), stream, p);
     });
   });
 }
@@ -1009,11 +1093,11 @@ inline int backward(const void* gate, const void* x, int dtype, int form, const 
       out.add(grad_gate, p.ggs, sizeof(E)), out.add(grad_x, p.gxs, sizeof(E));
       p.granule = in.bytes();
       p.wide = out.bytes() >= 4 && H % Lane<E>::kVec == 0;
-      constexpr int kSmem = 6 * kBufBytes;
+      const int smem = smem_bytes<3>(p.granule);
       const auto kernel = backward_kernel<E, f.value>;
       unsigned ctas = 0;
-      const int st = plan(kernel, kSmem, Lane<E>::kVec, B, T, H, ws, ws_bytes, &p.g, &ctas);
-      return st != kOk ? st : launch_pdl(kernel, dim3(ctas), dim3(kThreads), kSmem, stream, p);
+      const int st = plan(kernel, smem, Lane<E>::kVec, B, T, H, ws, ws_bytes, &p.g, &ctas);
+      return st != kOk ? st : launch_pdl(kernel, dim3(ctas), dim3(kThreads), size_t(smem), stream, p);
     });
   });
 }
