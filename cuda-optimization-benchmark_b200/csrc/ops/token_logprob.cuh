@@ -428,7 +428,8 @@ __global__ void __launch_bounds__(kThreads, kWarpRows ? 5 : 6) backward_kernel(c
 }
 
 // ------------------------------------------------------------------------------------ host side
-inline bool temperature_ok(double temperature) { return temperature > 0.0 && temperature < INFINITY; }
+// 1 / temperature, and that times log2(e), are ordinary fp32 numbers.
+inline bool temperature_ok(double temperature) { return temperature >= 1e-30 && temperature <= 1e30; }
 
 inline int check(const void* logits, int dtype, const int64_t* strides, const int64_t* token, int32_t B, int32_t T,
                  int32_t V, double temperature) {

@@ -9,6 +9,7 @@ non-zero native status; there is no CPU fallback.
 """
 import ctypes
 import functools
+import threading
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -616,14 +617,19 @@ def _needs(ctx, k):
     return k < len(ctx.needs_input_grad) and ctx.needs_input_grad[k]
 
 
+# A call may be more than one launch over the scratch of its stream, so threads take turns.
+_LAUNCH = threading.Lock()
+
+
 def _run(what, fn, index, *args):
     """A stream form on the current stream of device `index`, which is made the current device for it (a
     launch goes to the current device)."""
-    if _current_device() == index:
-        status = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
+    with _LAUNCH:
+        if _current_device() == index:
             status = fn(*args, _raw_stream(index))
+        else:
+            with torch.cuda.device(index):
+                status = fn(*args, _raw_stream(index))
     if status:
         _native.check(status, what)
 
@@ -705,6 +711,24 @@ def _writable(t, like, name):
     return t
 
 
+def _reach(t):
+    """[first, last) byte of the memory that t spans."""
+    if t.numel() == 0:
+        return 0, 0
+    n = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _apart(out, name, **inputs):
+    """Refuses an output in the memory of an input."""
+    lo, hi = _reach(out)
+    for other, t in inputs.items():
+        a, b = _reach(t)
+        if lo < b and a < hi:
+            raise ValueError(f"{name} overlaps {other}")
+    return out
+
+
 def _state_arg(state, name, B, H, device):
     if state is None:
         return None
@@ -748,7 +772,7 @@ def _recurrence_forward(gate, x, state, reset, form, out, train):
     dev, dt, fm, (B, T, H) = _bth(gate, x, form)
     state = _state_arg(state, "state", B, H, dev)
     reset = _reset_arg(reset, B, T, dev)
-    h = _like_bth(x) if out is None else _writable(out, x, "out")
+    h = _like_bth(x) if out is None else _apart(_writable(out, x, "out"), "out", gate=gate, x=x)
     n_ckpt, n_ws = _recurrence_sizes(B, T, H)
     final = torch.empty((B, H), dtype=torch.float32, device=dev)
     ckpt = torch.empty(n_ckpt, dtype=torch.float32, device=dev) if train else None
@@ -825,6 +849,8 @@ def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, s
         _need(state_out, "state_out", torch.float32, dev)
         if state_out.shape != state.shape:
             raise ValueError("state_out must have state's shape")
+        if state_out.data_ptr() != state.data_ptr():
+            _apart(state_out, "state_out", state=state)
     if slots is None:
         if S < B:
             raise ValueError("state has fewer rows than x and no slots are given")
@@ -832,7 +858,8 @@ def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, s
         _need(slots, "slots", torch.int32, dev)
         if slots.shape != (B,):
             raise ValueError(f"slots must be ({B},)")
-    h = x.new_empty((B, H)) if out is None else _writable(out, x, "out")
+    h = x.new_empty((B, H)) if out is None else _apart(_writable(out, x, "out"), "out", gate=gate, x=x, state=state,
+                                                       state_out=state_out)
     _run("linear_recurrence_step", _lib().b200_linear_recurrence_step_async, dev.index, gate.data_ptr(), x.data_ptr(),
          DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form], _strides(gate.stride(0), x.stride(0), h.stride(0)),
          state.data_ptr(), state_out.data_ptr(), _address(slots), S, B, H, h.data_ptr())
@@ -894,16 +921,13 @@ def _check_over(out, logits):
     """out is memory of its own, or exactly the logits (contiguous)."""
     if out.numel() == 0 or (out.data_ptr() == logits.data_ptr() and logits.is_contiguous()):
         return
-    reach = 1 + sum((n - 1) * s for n, s in zip(logits.shape, logits.stride()))
-    size = logits.element_size()
-    if out.data_ptr() < logits.data_ptr() + reach * size and logits.data_ptr() < out.data_ptr() + out.numel() * size:
-        raise ValueError("out overlaps the logits without being them")
+    _apart(out, "out", logits=logits)
 
 
 def _temperature(temperature):
     temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError("temperature must be positive and finite")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError("temperature must be positive (between 1e-30 and 1e30)")
     return temperature
 
 

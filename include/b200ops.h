@@ -366,7 +366,7 @@ int b200_linear_recurrence_step_async(const void* gate, const void* x, int dtype
 /* ---------------------------------------------------------------------------------------------
  * Token log-probabilities and entropies from logits (no reference counterpart: where the
  * current_log_prob and entropy streams of ppo_clip come from).  For each of B x T positions, with z
- * the V logits / temperature (temperature > 0): log_prob = z[token] - log sum exp z, entropy (may be
+ * the V logits / temperature (1e-30 to 1e30): log_prob = z[token] - log sum exp z, entropy (may be
  * NULL) of softmax(z), both fp32 [B, T].  logits are of `dtype` with a contiguous vocabulary axis;
  * `strides` (host array, elements): logits batch, logits time, token batch, token time.  A negative
  * token masks its position: outputs and gradient 0, its logits not read.  token >= V gives NaN.

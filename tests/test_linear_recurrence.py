@@ -107,7 +107,7 @@ def test_status_codes_without_a_gpu():
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("form", ["decay", "sigmoid"])
 @pytest.mark.parametrize("B,T,H", [(1, 1, 1), (2, 3, 5), (1, 127, 64), (3, 128, 66), (2, 129, 33), (1, 255, 128),
-                                   (2, 300, 70), (5, 515, 130), (1, 2049, 8)])
+                                   (2, 300, 70), (5, 515, 130), (1, 2049, 8), (2, 260, 193)])
 def test_against_oracle(ops, dtype, form, B, T, H):
     check(ops, make(B, T, H, dtype, form, seed=T * 7 + H), form)
 
@@ -172,6 +172,20 @@ def test_layouts(ops, layout, dtype):
     assert got is out and same_bits(out, h)
     big[1:-1, :, 2:-2] = 7.0
     assert torch.equal(big, torch.full_like(big, 7.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [64, 65])
+def test_strides_beyond_32_bits(ops, H):
+    """A batch stride of more than 2^31 elements, by tensor loads (H = 64) and by copies."""
+    gap = 2**31 + 64
+    s = make(2, 200, H, torch.bfloat16, "sigmoid", seed=H)
+    store = torch.empty(gap + 3 * 200 * H, dtype=torch.bfloat16, device="cuda")
+    for k, k0 in (("gate", 0), ("x", 200 * H), ("grad_h", 2 * 200 * H)):
+        v = store.as_strided((2, 200, H), (gap, H, 1), k0)
+        v.copy_(s[k])
+        s[k] = v
+    check(ops, s, "sigmoid")
 
 
 @pytest.mark.gpu
@@ -380,6 +394,8 @@ def test_refusals(ops):
                 lambda: ops.linear_recurrence(x, x, reset=torch.zeros(2, 3, device="cuda")),
                 lambda: ops.linear_recurrence(x, x, reset=torch.zeros(3, 2, device="cuda", dtype=torch.bool)),
                 lambda: ops.linear_recurrence(x, x, out=torch.zeros(1, 3, 4, device="cuda").expand(2, 3, 4)),
+                lambda: ops.linear_recurrence(x, x.clone(), out=x),
+                lambda: ops.linear_recurrence_step(x[0], x[0].clone(), torch.zeros(3, 4, device="cuda"), out=x[0]),
                 lambda: ops.linear_recurrence_backward(x, x, torch.zeros(3, device="cuda"), x),
                 lambda: ops.linear_recurrence_step(x[0], x[0], torch.zeros(2, 4, device="cuda")),
                 lambda: ops.linear_recurrence_step(x[0], x[0], torch.zeros(3, 5, device="cuda")),

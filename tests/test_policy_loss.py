@@ -252,6 +252,41 @@ def test_repeats_streams_and_captures(ops, B, T):
 
 
 @pytest.mark.gpu
+def test_threads_share_a_stream(ops):
+    """Calls of several threads on one stream, of more than one launch each, do not mix."""
+    import threading
+    sets = [make(700, 900, seed=k) for k in range(4)]
+    call = lambda s: ops.policy_loss_grad(**s, reduction="sequence_mean", **FULL)  # noqa: E731
+    want = [[t.clone() for t in call(s)] for s in sets]
+    got = [[] for _ in sets]
+
+    def work(k):
+        for _ in range(30):
+            got[k].append(call(sets[k]))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in range(4):
+        assert len(got[k]) == 30 and all(same_bits(a, b) for c in got[k] for a, b in zip(c, want[k]))
+
+
+@pytest.mark.gpu
+def test_row_strides_beyond_32_bits(ops):
+    s = make(2, 3000, seed=12)
+    gap = 2**31 + 4
+    store = torch.empty(gap + 5 * 3000, device="cuda")
+    for i, k in enumerate(("log_prob", "old_log_prob", "advantage", "ref_log_prob", "entropy")):
+        v = store.as_strided((2, 3000), (gap, 1), i * 3000)
+        v.copy_(s[k])
+        s[k] = v
+    check(ops, s, **FULL)
+
+
+@pytest.mark.gpu
 def test_autograd(ops):
     s = make(4, 50, seed=5)
     lp, ent = s["log_prob"].clone().requires_grad_(), s["entropy"].clone().requires_grad_()

@@ -60,6 +60,32 @@ def compare(got, want):
         assert (a.double() - b).abs().max() <= 1000 * 2.0 ** -24 * b.abs().max(), (a.double() - b).abs().max() / b.abs().max()
 
 
+def test_calls_go_to_the_tensors_device(monkeypatch):
+    """A call on tensors of another device than the current one makes that device current for the launch, and takes
+    that device's stream (a stand-in for the devices: no GPU here)."""
+    from conftest import pkg
+    ops = pkg().ops
+    current, seen = [0], []
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    monkeypatch.setattr(ops, "_current_device", lambda: current[0])
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 100 + index)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    call = lambda *a: seen.append((current[0], a)) or 0  # noqa: E731
+    ops._run("x", call, 1, 7)
+    ops._run("x", call, 0, 8)
+    assert seen == [(1, (7, 101)), (0, (8, 100))] and current == [0]
+
+
 @pytest.fixture(autouse=True)
 def full_precision_products():
     before = torch.backends.cuda.matmul.allow_tf32

@@ -264,7 +264,7 @@ def test_empty_and_refusals(ops):
     stats, g = torch.zeros(2, 3, 3, device="cuda"), torch.zeros(2, 3, device="cuda")
     for bad in (lambda: ops.token_logprob(x.double(), k), lambda: ops.token_logprob(x, k.int()),
                 lambda: ops.token_logprob(x, k[:, :2]), lambda: ops.token_logprob(x.transpose(1, 2), k),
-                lambda: ops.token_logprob(x, k, 0.0), lambda: ops.token_logprob(x, k, float("inf")),
+                lambda: ops.token_logprob(x, k, 0.0), lambda: ops.token_logprob(x, k, float("inf")), lambda: ops.token_logprob(x, k, 1e-40),
                 lambda: ops.token_logprob(x[..., :0], k), lambda: ops.token_logprob(x, k.cpu()),
                 lambda: ops.token_logprob(x[0, 0], k[0, 0]),
                 lambda: ops.token_logprob_backward(x, k, stats[..., :2], g),
