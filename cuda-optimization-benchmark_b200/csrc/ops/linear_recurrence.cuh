@@ -16,13 +16,14 @@
 //
 // A tile is kTile = 128 steps of one group of channels, 128 bytes wide (64 channels of 16 bits, 32 of
 // 32): each of 8 warps takes 16 steps, each lane 4 bytes of channels, so every load and store of a warp is a
-// full line.  CTAs are persistent and take tiles in time order from a ticket counter: while one tile
-// is worked on, the next one's rows arrive in the other shared-memory buffer (one tensor load per input,
-// or cp.async where rows are not on 16 bytes), so the loads never pause.  A tile is read once:
+// full line.  CTAs are persistent and take tiles in time order from a ticket counter.  A tile is read once:
 //   1. each warp composes its 16 steps into one map per channel;
 //   2. the 8 maps meet in shared memory; the tile's map goes out as a record in global memory;
 //   3. the state coming into the tile is formed from the records of the tiles before it;
 //   4. each warp runs its 16 steps again from its own incoming state and writes them.
+// Behind step 1 one warp, the clerk, finds the CTA's next tile and starts its loads into the other buffer (one
+// tensor load per input; where rows are not on 16 bytes every warp copies its own): after step 1, since a
+// tile's time is a chain of waits that all 8 warps share, and there the other warps wait anyway.
 // Records: `span` consecutive tiles form a block.  A tile that ends a block publishes the state (or
 // carried gradient) itself, the others their map; a tile takes the state at its block's start and the maps
 // of the block's tiles before it, in order.  So the association is fixed by the sizes alone and
@@ -52,6 +53,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRowBytes = 128;           // bytes of a tile's row
 constexpr int kBufBytes = kTile * kRowBytes;
 constexpr int kMaxSpan = 16;
+constexpr int kClerk = 5;                // the warp that takes the tickets (none of those with other extra work)
 constexpr size_t kCtlBytes = 256;
 
 struct Strides {  // in elements; the channel axis is contiguous
@@ -215,19 +217,23 @@ __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_grou
 template <int kBytes>
 __device__ __forceinline__ void copy_rows_by(char* dst, const char* src, int64_t pitch, int rows, int width) {
   constexpr int kPer = kRowBytes / kBytes;
-  const int off = int(threadIdx.x % kPer) * kBytes;
+  const int lane = int(threadIdx.x % 32), off = lane % kPer * kBytes;
   const int left = width - off;
   if (left <= 0) return;
-  for (int r = int(threadIdx.x) / kPer; r < rows; r += kThreads / kPer)
-    cp_async<kBytes>(dst + r * kRowBytes + off, src + r * pitch + off, left < kBytes ? left : kBytes);
+#pragma unroll
+  for (int i = 0; i < kSteps * kPer / 32; ++i) {
+    const int r = i * (32 / kPer) + lane / kPer;
+    if (r < rows) cp_async<kBytes>(dst + r * kRowBytes + off, src + r * pitch + off, left < kBytes ? left : kBytes);
+  }
 }
 
-// `rows` rows of `width` bytes (at most 128), pitch bytes apart, into a tile buffer.  `granule` bytes
-// divide the source address and the pitch.  Rows of 16-bit elements off 4 bytes are copied with the 4-byte word
-// that their first element lies in, the word behind the row's 32 goes to more[r], and align_rows() shifts
-// them to their place.
+// A warp's `rows` rows of `width` bytes (at most 128), pitch bytes apart, into its part of a tile buffer.
+// `granule` bytes divide the source address and the pitch.  Rows of 16-bit elements off 4 bytes are copied
+// with the 4-byte word that their first element lies in, the word behind the row's 32 goes to more[r], and
+// align_rows() shifts them.
 __device__ __forceinline__ void copy_rows(char* dst, uint32_t* more, const char* src, int64_t pitch, int rows,
                                           int width, int granule) {
+  const int lane = int(threadIdx.x % 32);
   if (granule == 16) {
     copy_rows_by<16>(dst, src, pitch, rows, width);
   } else if (granule == 8) {
@@ -235,24 +241,24 @@ __device__ __forceinline__ void copy_rows(char* dst, uint32_t* more, const char*
   } else if (granule == 4) {
     copy_rows_by<4>(dst, src, pitch, rows, width);
   } else {
-    const int lane = int(threadIdx.x % 32);
-    for (int r = int(threadIdx.x) / 32; r < rows; r += kWarps) {
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
       const char* s = src + r * pitch;
       const int off = int(reinterpret_cast<uintptr_t>(s) & 2u), left = width + off - lane * 4;
       if (left > 0) cp_async<4>(dst + r * kRowBytes + lane * 4, s - off + lane * 4, left < 4 ? left : 4);
     }
-    const int r = int(threadIdx.x);
-    if (r < rows) {
-      const char* s = src + r * pitch;
+    if (lane < rows) {
+      const char* s = src + lane * pitch;
       const int off = int(reinterpret_cast<uintptr_t>(s) & 2u), left = width + off - kRowBytes;
-      if (left > 0) cp_async<4>(reinterpret_cast<char*>(more + r), s - off + kRowBytes, left);
+      if (left > 0) cp_async<4>(reinterpret_cast<char*>(more + lane), s - off + kRowBytes, left);
     }
   }
 }
 
-// A warp's own rows, shifted where they were copied from an address off 4 bytes.
+// Rows copied from an address off 4 bytes, shifted to their place (the warp's own rows).
 __device__ __forceinline__ void align_rows(char* dst, const uint32_t* more, const char* src, int64_t pitch, int rows) {
   const int lane = int(threadIdx.x % 32);
+#pragma unroll 4
   for (int r = 0; r < rows; ++r) {
     if ((reinterpret_cast<uintptr_t>(src + r * pitch) & 2u) == 0) continue;
     uint32_t* row = reinterpret_cast<uint32_t*>(dst + r * kRowBytes);
@@ -273,6 +279,7 @@ struct Grid {
   unsigned span;
   Ctl* ctl;          // null when a row is one tile: no tile waits for another, CTAs take tiles in turn
   ulonglong2* recs;  // [n_tiles, B, H]
+  bool back;         // the scan runs from the last tile to the first
 };
 
 struct __align__(16) Tile {
@@ -280,6 +287,10 @@ struct __align__(16) Tile {
   unsigned b, group;
   unsigned live;  // 0: the ticket lies past the last tile
 };
+// The tile's first step.
+__device__ __forceinline__ int64_t first_step(const Grid& g, const Tile& t) {
+  return int64_t(g.back ? g.n_tiles - 1 - t.k : t.k) * kTile;
+}
 
 __device__ __forceinline__ Tile tile_of(const Grid& g, unsigned ticket) {
   Tile t;
@@ -304,8 +315,8 @@ struct Shared {
   V fwd[kBack ? kWarps - 1 : 1][32];  // the warps' forward offsets (backward kernel; the factor is map.x)
   Map<V> look[kMaxSpan][32];     // records of the tiles before this one
   unsigned look_cut[kMaxSpan];
-  unsigned cut[kWarps];          // the warp's steps hold a reset: its map does not see what comes in
-  Tile tile;                     // the next tile
+  uint64_t cut;                  // byte w: warp w's steps hold a reset, its map does not see what comes in
+  Tile tile[2];                  // of the CTA's tiles in turn
   uint64_t full[2];              // the tile buffers' loads have landed (tensor loads)
 };
 
@@ -348,56 +359,98 @@ __device__ __forceinline__ ulonglong2 wait_record(const ulonglong2* r, ulonglong
 }
 __device__ __forceinline__ float low_float(unsigned long long v) { return __uint_as_float(unsigned(v)); }
 
-// The record at r of this lane's channels; cut: its writer's steps held a reset.
-__device__ __forceinline__ void take_record(const ulonglong2* r, int c, int H, unsigned epoch, Map<float>& m,
-                                            unsigned& cut) {
+// This lane's records as they are now.
+template <int kVec>
+struct Record {
+  ulonglong2 x[kVec];
+};
+template <int kVec>
+__device__ __forceinline__ Record<kVec> peek_record(const ulonglong2* r, int c, int H) {
+  Record<kVec> q;
+#pragma unroll
+  for (int v = 0; v < kVec; ++v) q.x[v] = c + v < H ? ll_load2<LLScope::kGpu>(r + v) : make_ulonglong2(0ull, 0ull);
+  return q;
+}
+// The same once they are there; cut: their writer's steps held a reset.
+__device__ __forceinline__ void take_record(const ulonglong2* r, const Record<1>& q, int c, int H, unsigned epoch,
+                                            Map<float>& m, unsigned& cut) {
   m = Map<float>{1.0f, 0.0f};
   cut = 0;
   if (c >= H) return;
-  const ulonglong2 x = wait_record(r, ll_load2<LLScope::kGpu>(r), epoch);
+  const ulonglong2 x = wait_record(r, q.x[0], epoch);
   m = Map<float>{low_float(x.x), low_float(x.y)};
   cut = unsigned(x.x >> 32) & 1u;
 }
-__device__ __forceinline__ void take_record(const ulonglong2* r, int c, int H, unsigned epoch, Map<float2>& m,
-                                            unsigned& cut) {
+__device__ __forceinline__ void take_record(const ulonglong2* r, const Record<2>& q, int c, int H, unsigned epoch,
+                                            Map<float2>& m, unsigned& cut) {
   m = Map<float2>{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
   cut = 0;
   if (c >= H) return;
-  const ulonglong2* r1 = c + 1 < H ? r + 1 : r;
-  ulonglong2 x = ll_load2<LLScope::kGpu>(r), y = ll_load2<LLScope::kGpu>(r1);
-  x = wait_record(r, x, epoch);
-  y = wait_record(r1, y, epoch);
+  const ulonglong2 x = wait_record(r, q.x[0], epoch);
+  const ulonglong2 y = c + 1 < H ? wait_record(r + 1, q.x[1], epoch) : x;
   m = Map<float2>{make_float2(low_float(x.x), low_float(y.x)), make_float2(low_float(x.y), low_float(y.y))};
   cut = unsigned(x.x >> 32) & 1u;
 }
 
-// What comes into tile t from the tiles before it, for this lane's channels: y on entry is the value
-// before tile 0.  Every thread of the CTA calls it.
-template <typename V, bool kBack>
-__device__ __forceinline__ void incoming(const Grid& g, const Tile& t, int64_t B, int c, unsigned epoch,
-                                         Shared<V, kBack>& sh, V& y) {
-  if (t.k == 0) return;
-  const unsigned q = t.k & (g.span - 1);              // tiles of the block before this one
-  const unsigned n = q + (t.k >= g.span ? 1u : 0u);   // their maps, and the state at the block's start
+// The records of the tiles before tile t that what comes into it is formed from: n of them, the first (if the block
+// is not the row's first) the state at the block's start, then the maps of the block's tiles before t.
+struct Before {
+  const ulonglong2* first;  // of this lane's channels
+  int64_t step;
+  unsigned n;
+};
+__device__ __forceinline__ Before records_before(const Grid& g, const Tile& t, int64_t B, int c) {
+  const unsigned n = (t.k & (g.span - 1)) + (t.k >= g.span ? 1u : 0u);
+  const int64_t step = B * g.H;
+  return Before{g.recs + int64_t(t.k - n) * step + int64_t(t.b) * g.H + c, step, n};
+}
+
+// What comes into the tile, for this lane's channels: y on entry is the value before tile 0.  Warp w brings
+// records w and w + 8.  Every thread of the CTA calls it.
+template <int kVec, typename V, bool kBack>
+__device__ __forceinline__ void incoming(const Before& f, int c, int H, unsigned epoch, Shared<V, kBack>& sh, V& y) {
+  if (f.n == 0) return;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
-  const unsigned first = t.k - n;
-  for (unsigned i = w; i < n; i += kWarps) {
+  for (unsigned i = w; i < f.n; i += kWarps) {
+    const ulonglong2* r = f.first + i * f.step;
     unsigned cut;
     Map<V> m;
-    take_record(g.recs + (int64_t(first + i) * B + t.b) * g.H + c, c, g.H, epoch, m, cut);
+    take_record(r, peek_record<kVec>(r, c, H), c, H, epoch, m, cut);
     sh.look[i][lane] = m;
     cut = __any_sync(0xffffffffu, cut);
     if (lane == 0) sh.look_cut[i] = cut;
   }
   __syncthreads();
-  for (unsigned i = 0; i < n; ++i) y = apply(sh.look[i][lane], sh.look_cut[i] != 0, y);
+  for (unsigned i = 0; i < f.n; ++i) y = apply(sh.look[i][lane], sh.look_cut[i] != 0, y);
+}
+
+// The maps of the warps before warp w in the scan's direction, composed.
+template <bool kUp, typename V>
+__device__ __forceinline__ Map<V> before_warp(const Map<V> (&map)[kWarps][32], uint64_t cuts, unsigned w, bool& cut) {
+  const unsigned lane = threadIdx.x % 32;
+  Map<V> p{vset(V{}, 1.0f), vset(V{}, 0.0f)};
+  cut = false;
+#pragma unroll
+  for (int i = 0; i < kWarps - 1; ++i) {
+    const unsigned j = kUp ? i : kWarps - 1 - i;
+    if (kUp ? j >= w : j <= w) break;
+    const Map<V> m = map[j][lane];
+    if (cuts == 0) {
+      p = Map<V>{vmul(m.x, p.x), vfma(m.x, p.b, m.b)};
+    } else {
+      const bool now = ((cuts >> (8 * j)) & 1u) != 0u;
+      cut = cut || now;
+      p = Map<V>{vmul(m.x, p.x), apply(m, now, p.b)};
+    }
+  }
+  return p;
 }
 
 __device__ __forceinline__ bool ends_block(const Grid& g, unsigned k) { return (k & (g.span - 1)) == g.span - 1; }
 
-// Ends the launch's use of the workspace: the last CTA to leave makes it ready for the next launch.
+// Ends the launch's use of the workspace (the clerk, which takes no more tickets): the last CTA to leave makes it ready for the next launch.
 __device__ __forceinline__ void leave(const Grid& g, unsigned epoch) {
-  if (g.ctl == nullptr || threadIdx.x != 0) return;
+  if (g.ctl == nullptr || threadIdx.x != kClerk * 32) return;
   __threadfence();
   if (atomicAdd(&g.ctl->done, 1u) == gridDim.x - 1) {
     g.ctl->ticket = 0;
@@ -407,13 +460,9 @@ __device__ __forceinline__ void leave(const Grid& g, unsigned epoch) {
   }
 }
 
-// Thread 0's supply of tickets: after the first, taken one ahead so that no tile waits for the counter.
-struct Tickets {
-  unsigned ahead;
-  __device__ __forceinline__ unsigned take(const Grid& g, unsigned last) const {
-    return g.ctl != nullptr ? atomicAdd(&g.ctl->ticket, 1u) : last + gridDim.x;
-  }
-};
+__device__ __forceinline__ unsigned take_ticket(const Grid& g, unsigned last) {
+  return g.ctl != nullptr ? atomicAdd(&g.ctl->ticket, 1u) : last + gridDim.x;
+}
 
 // The launch's epoch: 31 bits, never 0 (a zero-filled record belongs to no launch).
 __device__ __forceinline__ unsigned launch_epoch(const Grid& g) {
@@ -441,44 +490,51 @@ struct __align__(64) Input {
   int swap;
 };
 
+// One tensor load of a tile (one thread).
 template <typename T>
-__device__ __forceinline__ const char* row_address(const Input<T>& in, const Tile& t, int64_t step) {
-  return reinterpret_cast<const char*>(in.p + t.b * in.s.b + step * in.s.t +
-                                       int64_t(t.group) * (kRowBytes / int(sizeof(T))));
+__device__ __forceinline__ void load_tile(const Input<T>& in, char* dst, const Tile& t, int64_t t0, uint64_t* bar) {
+  const int c0 = int(t.group) * (kRowBytes / int(sizeof(T))), a = int(t0), b = int(t.b);
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(smem_addr(dst)),
+      "l"(&in.map), "r"(c0), "r"(in.swap ? b : a), "r"(in.swap ? a : b), "r"(smem_addr(bar))
+      : "memory");
 }
 
+// A warp's own rows of an input, by copies (every lane).
 template <typename T>
-__device__ __forceinline__ void load_tile(const Input<T>& in, char* dst, uint32_t* more, const Tile& t, int64_t t0,
-                                          const Grid& g, bool tma, int granule, uint64_t* bar) {
-  constexpr int kGroup = kRowBytes / int(sizeof(T));
-  const int c0 = int(t.group) * kGroup;
-  if (tma) {  // one thread
-    const int a = int(t0), b = int(t.b);
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-            "r"(smem_addr(dst)),
-        "l"(&in.map), "r"(c0), "r"(in.swap ? b : a), "r"(in.swap ? a : b), "r"(smem_addr(bar))
-        : "memory");
-  } else {
-    copy_rows(dst, more, row_address(in, t, t0), in.s.t * int64_t(sizeof(T)), int(g.T - t0 < kTile ? g.T - t0 : kTile),
-              min(kGroup, g.H - c0) * int(sizeof(T)), granule);
-  }
+__device__ __forceinline__ const char* warp_rows(const Input<T>& in, const Tile& t, int64_t t0) {
+  return reinterpret_cast<const char*>(in.p + t.b * in.s.b + t0 * in.s.t + int64_t(t.group) * (kRowBytes / int(sizeof(T))));
 }
-// Behind the copies, where they were of unaligned rows: this warp's rows (n of them, from step t0).
 template <typename T>
-__device__ __forceinline__ void align_tile(const Input<T>& in, char* rows, const uint32_t* more, const Tile& t,
-                                           int64_t t0, int n) {
-  align_rows(rows, more, row_address(in, t, t0), in.s.t * int64_t(sizeof(T)), n);
+__device__ __forceinline__ void copy_tile(const Input<T>& in, char* dst, uint32_t* more, const Tile& t, int64_t t0,
+                                          const Grid& g, int granule) {
+  constexpr int kGroup = kRowBytes / int(sizeof(T));
+  const int rows = int(g.T - t0 < kSteps ? g.T - t0 : kSteps);
+  if (rows > 0)
+    copy_rows(dst, more, warp_rows(in, t, t0), in.s.t * int64_t(sizeof(T)), rows,
+              min(kGroup, g.H - int(t.group) * kGroup) * int(sizeof(T)), granule);
+}
+template <typename T>
+__device__ __forceinline__ void align_tile(const Input<T>& in, char* dst, const uint32_t* more, const Tile& t,
+                                           int64_t t0, const Grid& g) {
+  const int rows = int(g.T - t0 < kSteps ? g.T - t0 : kSteps);
+  if (rows > 0) align_rows(dst, more, warp_rows(in, t, t0), in.s.t * int64_t(sizeof(T)), rows);
 }
 
 // Dynamic shared memory: kIn inputs in two buffers, and the words behind the rows of unaligned copies.
+constexpr int kMoreWords = kTile;
 template <int kIn>
 constexpr int smem_bytes(int granule) {
-  return 2 * kIn * (kBufBytes + (granule == 2 ? kTile * 4 : 0));
+  return 2 * kIn * (kBufBytes + (granule == 2 ? kMoreWords * 4 : 0));
 }
 template <int kIn>
-__device__ __forceinline__ uint32_t* more_of(char* smem, int buf, int in) {
-  return reinterpret_cast<uint32_t*>(smem + 2 * kIn * kBufBytes) + (buf * kIn + in) * kTile;
+__device__ __forceinline__ char* buffer(char* smem, unsigned buf, int in) {
+  return smem + (buf * kIn + in) * kBufBytes;
+}
+template <int kIn>
+__device__ __forceinline__ uint32_t* more_of(char* smem, unsigned buf, int in) {
+  return reinterpret_cast<uint32_t*>(smem + 2 * kIn * kBufBytes) + (buf * kIn + in) * kMoreWords;
 }
 
 // ------------------------------------------------------------------------------------- forward
@@ -553,69 +609,71 @@ constexpr int forward_ctas() {
 template <typename T, int kForm>
 __global__ void __launch_bounds__(kThreads, forward_ctas<T>()) forward_kernel(const __grid_constant__ Forward<T> p) {
   using V = typename Lane<T>::V;
-  constexpr int kVec = Lane<T>::kVec, kGroup = 32 * kVec;
+  constexpr int kVec = Lane<T>::kVec, kIn = 2;
   extern __shared__ __align__(128) char smem[];
   __shared__ Shared<V, false> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
 
-  const auto prefetch = [&](const Tile& t, int buf) {
-    if (t.live && (!p.tma || threadIdx.x == 0)) {
-      const int64_t t0 = int64_t(t.k) * kTile;
-      char* dst = smem + buf * 2 * kBufBytes;
-      if (p.tma) mbar_arrive_expect_tx(&sh.full[buf], 2 * kBufBytes);
-      load_tile(p.gate, dst, more_of<2>(smem, buf, 0), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
-      load_tile(p.x, dst + kBufBytes, more_of<2>(smem, buf, 1), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
+  // A tile's loads: tensor loads by one thread, or this warp's own rows.
+  const auto load_all = [&](const Tile& t, unsigned buf) {
+    if (!t.live) return;
+    mbar_arrive_expect_tx(&sh.full[buf], kIn * kBufBytes);
+    load_tile(p.gate, buffer<kIn>(smem, buf, 0), t, first_step(p.g, t), &sh.full[buf]);
+    load_tile(p.x, buffer<kIn>(smem, buf, 1), t, first_step(p.g, t), &sh.full[buf]);
+  };
+  uint8_t reset_byte = 0;
+  const auto fetch_own = [&](const Tile& t, unsigned buf) {
+    if (!t.live) return;
+    const int64_t t0 = first_step(p.g, t) + w * kSteps;
+    reset_byte = p.reset.load(t.b, t0 + lane, p.g.T);
+    if (!p.tma) {
+      copy_tile(p.gate, buffer<kIn>(smem, buf, 0) + w * kSteps * kRowBytes, more_of<kIn>(smem, buf, 0) + w * kSteps, t,
+                t0, p.g, p.granule);
+      copy_tile(p.x, buffer<kIn>(smem, buf, 1) + w * kSteps * kRowBytes, more_of<kIn>(smem, buf, 1) + w * kSteps, t,
+                t0, p.g, p.granule);
+      cp_commit();
     }
-    if (!p.tma) cp_commit();
   };
-  const auto load_reset = [&](const Tile& t) {
-    return t.live ? p.reset.load(t.b, int64_t(t.k) * kTile + w * kSteps + lane, p.g.T) : uint8_t(0);
-  };
+  const bool own = !p.tma || p.reset.p != nullptr;  // every warp fetches something itself
 
-  Tickets tickets;
-  if (threadIdx.x == 0) {
+  const bool clerk = threadIdx.x == kClerk * 32;
+  unsigned ahead = 0;
+  if (clerk) {
     mbar_init(&sh.full[0], 1);
     mbar_init(&sh.full[1], 1);
     fence_barrier_init();
-    const unsigned first = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
-    sh.tile = tile_of(p.g, first);
-    tickets.ahead = first;
+    ahead = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
+    sh.tile[0] = tile_of(p.g, ahead);
+    if (p.tma) load_all(sh.tile[0], 0);
   }
   __syncthreads();
-  Tile t = sh.tile;
-  prefetch(t, 0);
-  uint8_t reset_byte = load_reset(t);
-  __syncthreads();  // sh.tile is read
-  for (unsigned it = 0; t.live; ++it) {
+  if (own) fetch_own(sh.tile[0], 0);
+  for (unsigned it = 0;; ++it) {
     const unsigned buf = it & 1u;
-    if (p.tma)
-      mbar_wait(&sh.full[buf], (it >> 1) & 1u);
-    else
-      cp_wait_all();
-    const unsigned resets = __ballot_sync(0xffffffffu, reset_byte != 0);
-    if (threadIdx.x == 0) {
-      // The second ticket waits for the first tile's rows: by then every CTA has its first.
-      if (it == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
-      sh.tile = tile_of(p.g, tickets.ahead);
-    }
-    __syncthreads();  // this tile's rows and the next tile are here; the other buffer is free
-    const Tile next = sh.tile;
-    prefetch(next, buf ^ 1);
-    reset_byte = load_reset(next);
-    if (threadIdx.x == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
-
-    const int64_t t0 = int64_t(t.k) * kTile + w * kSteps;  // this warp's first step
+    if (it > 0) __syncthreads();  // the tile before is done: its buffer and the maps are free
+    const Tile t = sh.tile[buf];
+    if (!t.live) break;
+    const int64_t t0 = first_step(p.g, t) + w * kSteps;            // this warp's first step
     const int n = int(p.g.T - t0 < kSteps ? p.g.T - t0 : kSteps);  // its steps (0 or less: none)
-    const int c = int(t.group) * kGroup + int(lane) * kVec;
-    char* rows = smem + buf * 2 * kBufBytes + w * kSteps * kRowBytes;
-    if (p.granule == 2) {
-      align_tile(p.gate, rows, more_of<2>(smem, buf, 0) + w * kSteps, t, t0, n);
-      align_tile(p.x, rows + kBufBytes, more_of<2>(smem, buf, 1) + w * kSteps, t, t0, n);
-    }
-    const char* row = rows + lane * 4;
+    const int c = (int(t.group) * 32 + int(lane)) * kVec;
     const int64_t state_at = int64_t(t.b) * p.g.H + c;
+    char* rows = buffer<kIn>(smem, buf, 0) + w * kSteps * kRowBytes;
+    if (p.tma) {
+      mbar_wait(&sh.full[buf], (it >> 1) & 1u);
+    } else {
+      cp_wait_all();
+      __syncwarp();
+      if (p.granule == 2) {
+        align_tile(p.gate, rows, more_of<kIn>(smem, buf, 0) + w * kSteps, t, t0, p.g);
+        align_tile(p.x, rows + kBufBytes, more_of<kIn>(smem, buf, 1) + w * kSteps, t, t0, p.g);
+      }
+    }
+    // The next ticket, once the rows are there: by then every CTA has its first.
+    if (clerk) ahead = take_ticket(p.g, ahead);
+    const unsigned resets = own ? __ballot_sync(0xffffffffu, reset_byte != 0) : 0u;
+    const char* row = rows + lane * 4;
 
     // 1. The warp's steps as one map per channel; a and v stay in registers for step 4.
     V a[kSteps], u[kSteps];  // (decay: not used)
@@ -626,34 +684,36 @@ __global__ void __launch_bounds__(kThreads, forward_ctas<T>()) forward_kernel(co
     else
       forward_map<T, kForm, true>(row, resets, n, a, u, m);
     sh.map[w][lane] = m;
-    if (lane == 0) sh.cut[w] = resets != 0;
+    if (lane == 0) reinterpret_cast<uint8_t*>(&sh.cut)[w] = resets != 0;
+    if (own && clerk) sh.tile[buf ^ 1] = tile_of(p.g, ahead);  // all warps need it at once
     __syncthreads();
+    if (own) {
+      fetch_own(sh.tile[buf ^ 1], buf ^ 1);
+      if (p.tma && clerk) load_all(sh.tile[buf ^ 1], buf ^ 1);
+    } else if (clerk) {
+      sh.tile[buf ^ 1] = tile_of(p.g, ahead);
+      load_all(sh.tile[buf ^ 1], buf ^ 1);
+    }
+    const uint64_t cuts = sh.cut;
+    bool pre_cut;
+    const Map<V> pre = before_warp<true>(sh.map, cuts, w, pre_cut);
 
     // 2. The tile's map, by the last warp; a tile that ends a block publishes its state in step 3.
     const bool ends = ends_block(p.g, t.k), more = t.k + 1 < p.g.n_tiles;
-    bool tile_cut = false;
     if (w == kWarps - 1 && more) {
-      m = sh.map[0][lane];
-      tile_cut = sh.cut[0] != 0;
-#pragma unroll
-      for (int j = 1; j < kWarps; ++j) {
-        const bool cut = sh.cut[j] != 0;
-        const Map<V> s = sh.map[j][lane];
-        tile_cut |= cut;
-        m = Map<V>{vmul(s.x, m.x), apply(s, cut, m.b)};
-      }
-      if (!ends) publish(p.g, t, p.B, c, m, epoch * 2u + (tile_cut ? 1u : 0u));
+      m = Map<V>{vmul(m.x, pre.x), apply(m, resets != 0, pre.b)};
+      if (!ends) publish(p.g, t, p.B, c, m, epoch * 2u + (cuts != 0 ? 1u : 0u));
     }
 
     // 3. The state that comes in.
     V y = vset(V{}, 0.0f);
     if (p.state != nullptr && t.k < p.g.span) load_row(p.state + state_at, c, p.g.H, y);
-    incoming(p.g, t, p.B, c, epoch, sh, y);
+    incoming<kVec>(records_before(p.g, t, p.B, c), c, p.g.H, epoch, sh, y);
     if (w == kWarps - 1 && more && ends)
-      publish(p.g, t, p.B, c, Map<V>{vset(V{}, 0.0f), apply(m, tile_cut, y)}, epoch * 2u + 1u);
+      publish(p.g, t, p.B, c, Map<V>{vset(V{}, 0.0f), apply(m, cuts != 0, y)}, epoch * 2u + 1u);
     if (w == 0 && p.ckpt != nullptr)
       store_row(p.ckpt + (int64_t(t.b) * p.g.n_tiles + t.k) * p.g.H + c, c, p.g.H, y);
-    for (unsigned j = 0; j < w; ++j) y = apply(sh.map[j][lane], sh.cut[j] != 0, y);
+    y = apply(pre, pre_cut, y);
 
     // 4. The steps from there.
     T* out = p.h + t.b * p.hs.b + t0 * p.hs.t + c;
@@ -662,7 +722,6 @@ __global__ void __launch_bounds__(kThreads, forward_ctas<T>()) forward_kernel(co
     else
       forward_steps<T, kForm, true>(row, a, u, resets, n, c, p.g.H, p.wide, out, p.hs.t, y);
     if (p.final_state != nullptr && n > 0 && t0 + n == p.g.T) store_row(p.final_state + state_at, c, p.g.H, y);
-    t = next;
   }
   leave(p.g, epoch);
 }
@@ -682,14 +741,23 @@ struct Backward {
   bool tma, wide;
 };
 
-// Step 1 of the warp: a and 1 - a of its steps (decay: a alone), its forward map f and its backward map.  In the
-// order of time the backward map of steps 0 .. i is c -> P_i c + sum_j P_j grad_h[j], P_i the product of a
-// up to step i, so it needs no second pass and its factor is the forward map's.
+constexpr int kHalf = kSteps / 2;
+
+// What step 1 leaves of a warp's steps: a and 1 - a (decay: a alone), the state after the first half as a map of
+// the state before it, and the forward offset and the backward map of them all.
+template <typename V>
+struct Steps {
+  V a[kSteps], na[kSteps];
+  Map<V> half, m;
+  V f;
+};
+
+// In the order of time the backward map of steps 0 .. i is c -> P_i c + sum_j P_j grad_h[j], P_i the product of
+// a up to step i, so it needs no second pass and its factor is the forward map's.
 template <typename T, int kForm, bool kAny, typename V>
-__device__ __forceinline__ void backward_map(const char* row, unsigned resets, int n, V (&a)[kSteps],
-                                             V (&na)[kSteps], V& f, Map<V>& m) {
-  f = vset(V{}, 0.0f);
-  m = Map<V>{vset(V{}, 1.0f), vset(V{}, 0.0f)};
+__device__ __forceinline__ void backward_map(const char* row, unsigned resets, int n, Steps<V>& q) {
+  q.f = vset(V{}, 0.0f);
+  q.m = q.half = Map<V>{vset(V{}, 1.0f), vset(V{}, 0.0f)};
   bool cut = false;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
@@ -698,56 +766,54 @@ __device__ __forceinline__ void backward_map(const char* row, unsigned resets, i
     V u = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
     const V dv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + 2 * kBufBytes + i * kRowBytes));
     if (kForm == kDecay) {
-      a[i] = Lane<T>::unpack(gt);
+      q.a[i] = Lane<T>::unpack(gt);
     } else {
-      sigmoid_pair(Lane<T>::unpack_gate(gt), a[i], na[i]);
-      u = vmul(na[i], u);
+      sigmoid_pair(Lane<T>::unpack_gate(gt), q.a[i], q.na[i]);
+      u = vmul(q.na[i], u);
     }
     if (kAny && ((resets >> i) & 1u)) {
-      f = vset(V{}, 0.0f);
+      q.f = vset(V{}, 0.0f);
       cut = true;  // what lies behind a reset reaches no step before it
     }
-    f = vfma(a[i], f, u);
-    m.x = vmul(m.x, a[i]);
-    if (!kAny || !cut) m.b = vfma(m.x, dv, m.b);
+    q.f = vfma(q.a[i], q.f, u);
+    q.m.x = vmul(q.m.x, q.a[i]);
+    if (!kAny || !cut) q.m.b = vfma(q.m.x, dv, q.m.b);
+    if (i == kHalf - 1) q.half = Map<V>{q.m.x, q.f};
   }
 }
 
-// The states before the warp's steps from the state s before its first, turned into what multiplies g in
-// grad_gate: h[t-1], or (h[t-1] - x) a (1 - a).
-template <typename T, int kForm, bool kAny, typename V>
-__device__ __forceinline__ void backward_states(const char* row, unsigned resets, int n, const V (&a)[kSteps],
-                                                const V (&na)[kSteps], V s, V (&d)[kSteps]) {
+// Step 4 for half the warp's steps, kFrom .. kFrom + kHalf - 1: the states before them, from the state s before the
+// first, turned into what multiplies g in grad_gate (h[t-1], or (h[t-1] - x) a (1 - a)), then the steps
+// backwards from the gradient y that comes in.  Half at a time keeps these factors in few registers.
+template <typename T, int kForm, bool kAny, int kFrom, typename V>
+__device__ __forceinline__ void backward_steps(const char* row, unsigned resets, int n, const Steps<V>& q, V s, int c,
+                                               int H, bool wide, T* og, int64_t gpitch, T* ox, int64_t xpitch, V& y) {
+  V d[kHalf];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
+  for (int k = 0; k < kHalf; ++k) {
+    const int i = kFrom + k;
     if (kAny && i >= n) break;
     const V xv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + kBufBytes + i * kRowBytes));
     if (kAny && ((resets >> i) & 1u)) s = vset(V{}, 0.0f);
     if (kForm == kDecay) {
-      d[i] = s;
-      s = vfma(a[i], s, xv);
+      d[k] = s;
+      s = vfma(q.a[i], s, xv);
     } else {
-      d[i] = vmul(vsub(s, xv), vmul(a[i], na[i]));
-      s = vfma(a[i], s, vmul(na[i], xv));
+      d[k] = vmul(vsub(s, xv), vmul(q.a[i], q.na[i]));
+      s = vfma(q.a[i], s, vmul(q.na[i], xv));
     }
   }
-}
-
-// The warp's steps backwards from the gradient y that comes in.
-template <typename T, int kForm, bool kAny, typename V>
-__device__ __forceinline__ void backward_steps(const char* row, unsigned resets, int n, const V (&a)[kSteps],
-                                               const V (&na)[kSteps], const V (&d)[kSteps], int c, int H, bool wide,
-                                               T* og, int64_t gpitch, T* ox, int64_t xpitch, V& y) {
-  og += (kSteps - 1) * gpitch;
-  ox += (kSteps - 1) * xpitch;
+  og += (kFrom + kHalf - 1) * gpitch;
+  ox += (kFrom + kHalf - 1) * xpitch;
 #pragma unroll
-  for (int i = kSteps - 1; i >= 0; --i) {
+  for (int k = kHalf - 1; k >= 0; --k) {
+    const int i = kFrom + k;
     if (!kAny || i < n) {
       const V dv = Lane<T>::unpack(*reinterpret_cast<const uint32_t*>(row + 2 * kBufBytes + i * kRowBytes));
       const V g = vadd(dv, y);
-      store_out<T>(og, c, H, !kAny || wide, vmul(g, d[i]));
-      store_out<T>(ox, c, H, !kAny || wide, kForm == kDecay ? g : vmul(na[i], g));
-      y = vmul(a[i], g);
+      store_out<T>(og, c, H, !kAny || wide, vmul(g, d[k]));
+      store_out<T>(ox, c, H, !kAny || wide, kForm == kDecay ? g : vmul(q.na[i], g));
+      y = vmul(q.a[i], g);
       if (kAny && ((resets >> i) & 1u)) y = vset(V{}, 0.0f);
     }
     og -= gpitch;
@@ -760,128 +826,138 @@ __device__ __forceinline__ void backward_steps(const char* row, unsigned resets,
 template <typename T, int kForm>
 __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_constant__ Backward<T> p) {
   using V = typename Lane<T>::V;
-  constexpr int kVec = Lane<T>::kVec, kGroup = 32 * kVec;
+  constexpr int kVec = Lane<T>::kVec, kIn = 3;
   extern __shared__ __align__(128) char smem[];
   __shared__ Shared<V, true> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
 
-  const auto prefetch = [&](const Tile& t, int buf) {
-    if (t.live && (!p.tma || threadIdx.x == 0)) {
-      const int64_t t0 = int64_t(p.g.n_tiles - 1 - t.k) * kTile;
-      char* dst = smem + buf * 3 * kBufBytes;
-      if (p.tma) mbar_arrive_expect_tx(&sh.full[buf], 3 * kBufBytes);
-      load_tile(p.gate, dst, more_of<3>(smem, buf, 0), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
-      load_tile(p.x, dst + kBufBytes, more_of<3>(smem, buf, 1), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
-      load_tile(p.dh, dst + 2 * kBufBytes, more_of<3>(smem, buf, 2), t, t0, p.g, p.tma, p.granule, &sh.full[buf]);
+  // A tile's loads: tensor loads by one thread, or this warp's own rows.
+  const auto load_all = [&](const Tile& t, unsigned buf) {
+    if (!t.live) return;
+    mbar_arrive_expect_tx(&sh.full[buf], kIn * kBufBytes);
+    load_tile(p.gate, buffer<kIn>(smem, buf, 0), t, first_step(p.g, t), &sh.full[buf]);
+    load_tile(p.x, buffer<kIn>(smem, buf, 1), t, first_step(p.g, t), &sh.full[buf]);
+    load_tile(p.dh, buffer<kIn>(smem, buf, 2), t, first_step(p.g, t), &sh.full[buf]);
+  };
+  uint8_t reset_byte = 0;
+  const auto fetch_own = [&](const Tile& t, unsigned buf) {
+    if (!t.live) return;
+    const int64_t t0 = first_step(p.g, t) + w * kSteps;
+    reset_byte = p.reset.load(t.b, t0 + lane, p.g.T);
+    if (!p.tma) {
+      copy_tile(p.gate, buffer<kIn>(smem, buf, 0) + w * kSteps * kRowBytes, more_of<kIn>(smem, buf, 0) + w * kSteps, t,
+                t0, p.g, p.granule);
+      copy_tile(p.x, buffer<kIn>(smem, buf, 1) + w * kSteps * kRowBytes, more_of<kIn>(smem, buf, 1) + w * kSteps, t,
+                t0, p.g, p.granule);
+      copy_tile(p.dh, buffer<kIn>(smem, buf, 2) + w * kSteps * kRowBytes, more_of<kIn>(smem, buf, 2) + w * kSteps, t,
+                t0, p.g, p.granule);
+      cp_commit();
     }
-    if (!p.tma) cp_commit();
   };
-  const auto load_reset = [&](const Tile& t) {
-    return t.live ? p.reset.load(t.b, int64_t(p.g.n_tiles - 1 - t.k) * kTile + w * kSteps + lane, p.g.T)
-                  : uint8_t(0);
-  };
+  const bool own = !p.tma || p.reset.p != nullptr;  // every warp fetches something itself
 
-  Tickets tickets;
-  if (threadIdx.x == 0) {
+  const bool clerk = threadIdx.x == kClerk * 32;
+  unsigned ahead = 0;
+  if (clerk) {
     mbar_init(&sh.full[0], 1);
     mbar_init(&sh.full[1], 1);
     fence_barrier_init();
-    const unsigned first = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
-    sh.tile = tile_of(p.g, first);
-    tickets.ahead = first;
+    ahead = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
+    sh.tile[0] = tile_of(p.g, ahead);
+    if (p.tma) load_all(sh.tile[0], 0);
   }
   __syncthreads();
-  Tile t = sh.tile;
-  prefetch(t, 0);
-  uint8_t reset_byte = load_reset(t);
-  __syncthreads();  // sh.tile is read
-  for (unsigned it = 0; t.live; ++it) {
+  if (own) fetch_own(sh.tile[0], 0);
+  for (unsigned it = 0;; ++it) {
     const unsigned buf = it & 1u;
+    if (it > 0) __syncthreads();  // the tile before is done: its buffer and the maps are free
+    const Tile t = sh.tile[buf];
+    if (!t.live) break;
     const unsigned kt = p.g.n_tiles - 1 - t.k;  // the time tile
-    const int64_t t0 = int64_t(kt) * kTile + w * kSteps;
+    const int64_t t0 = first_step(p.g, t) + w * kSteps;
     const int n = int(p.g.T - t0 < kSteps ? p.g.T - t0 : kSteps);
-    const int c = int(t.group) * kGroup + int(lane) * kVec;
+    const int c = (int(t.group) * 32 + int(lane)) * kVec;
     const int64_t state_at = int64_t(t.b) * p.g.H + c;
     V s;  // the state before the tile
     load_row(p.ckpt + (int64_t(t.b) * p.g.n_tiles + kt) * p.g.H + c, c, p.g.H, s);
-    if (p.tma)
+    char* rows = buffer<kIn>(smem, buf, 0) + w * kSteps * kRowBytes;
+    if (p.tma) {
       mbar_wait(&sh.full[buf], (it >> 1) & 1u);
-    else
+    } else {
       cp_wait_all();
-    const unsigned resets = __ballot_sync(0xffffffffu, reset_byte != 0);
-    if (threadIdx.x == 0) {
-      // The second ticket waits for the first tile's rows: by then every CTA has its first.
-      if (it == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
-      sh.tile = tile_of(p.g, tickets.ahead);
+      __syncwarp();
+      if (p.granule == 2) {
+        align_tile(p.gate, rows, more_of<kIn>(smem, buf, 0) + w * kSteps, t, t0, p.g);
+        align_tile(p.x, rows + kBufBytes, more_of<kIn>(smem, buf, 1) + w * kSteps, t, t0, p.g);
+        align_tile(p.dh, rows + 2 * kBufBytes, more_of<kIn>(smem, buf, 2) + w * kSteps, t, t0, p.g);
+      }
     }
-    __syncthreads();  // this tile's rows and the next tile are here; the other buffer is free
-    const Tile next = sh.tile;
-    prefetch(next, buf ^ 1);
-    reset_byte = load_reset(next);
-    if (threadIdx.x == 0) tickets.ahead = tickets.take(p.g, tickets.ahead);
-    char* rows = smem + buf * 3 * kBufBytes + w * kSteps * kRowBytes;
-    if (p.granule == 2) {
-      align_tile(p.gate, rows, more_of<3>(smem, buf, 0) + w * kSteps, t, t0, n);
-      align_tile(p.x, rows + kBufBytes, more_of<3>(smem, buf, 1) + w * kSteps, t, t0, n);
-      align_tile(p.dh, rows + 2 * kBufBytes, more_of<3>(smem, buf, 2) + w * kSteps, t, t0, n);
-    }
+    // The next ticket, once the rows are there: by then every CTA has its first.
+    if (clerk) ahead = take_ticket(p.g, ahead);
+    const unsigned resets = own ? __ballot_sync(0xffffffffu, reset_byte != 0) : 0u;
     const char* row = rows + lane * 4;
 
     // 1. The warp's forward and backward maps.
-    V a[kSteps], na[kSteps], d[kSteps], f;
-    Map<V> m;
+    Steps<V> q;
     const bool plain = resets == 0 && n >= kSteps;
     if (plain)
-      backward_map<T, kForm, false>(row, 0u, kSteps, a, na, f, m);
+      backward_map<T, kForm, false>(row, 0u, kSteps, q);
     else
-      backward_map<T, kForm, true>(row, resets, n, a, na, f, m);
-    sh.map[w][lane] = m;
-    if (w < kWarps - 1) sh.fwd[w][lane] = f;  // (no warp comes after the last)
-    if (lane == 0) sh.cut[w] = resets != 0;
+      backward_map<T, kForm, true>(row, resets, n, q);
+    sh.map[w][lane] = q.m;
+    if (w < kWarps - 1) sh.fwd[w][lane] = q.f;  // (no warp comes after the last)
+    if (lane == 0) reinterpret_cast<uint8_t*>(&sh.cut)[w] = resets != 0;
+    if (own && clerk) sh.tile[buf ^ 1] = tile_of(p.g, ahead);  // all warps need it at once
     __syncthreads();
+    if (own) {
+      fetch_own(sh.tile[buf ^ 1], buf ^ 1);
+      if (p.tma && clerk) load_all(sh.tile[buf ^ 1], buf ^ 1);
+    } else if (clerk) {
+      sh.tile[buf ^ 1] = tile_of(p.g, ahead);
+      load_all(sh.tile[buf ^ 1], buf ^ 1);
+    }
+    const uint64_t cuts = sh.cut;
+    bool pre_cut;
+    const Map<V> pre = before_warp<false>(sh.map, cuts, w, pre_cut);
 
     // 2. The tile's map (from its last warp back), by warp 0, which holds the last of it.
     const bool ends = ends_block(p.g, t.k), more = t.k + 1 < p.g.n_tiles;
-    bool tile_cut = false;
+    Map<V> m;
     if (w == 0 && more) {
-      m = sh.map[kWarps - 1][lane];
-      tile_cut = sh.cut[kWarps - 1] != 0;
-#pragma unroll
-      for (int j = kWarps - 2; j >= 0; --j) {
-        const bool cut = sh.cut[j] != 0;
-        const Map<V> q = sh.map[j][lane];
-        tile_cut |= cut;
-        m = Map<V>{vmul(q.x, m.x), apply(q, cut, m.b)};
-      }
-      if (!ends) publish(p.g, t, p.B, c, m, epoch * 2u + (tile_cut ? 1u : 0u));
+      m = Map<V>{vmul(q.m.x, pre.x), apply(q.m, resets != 0, pre.b)};
+      if (!ends) publish(p.g, t, p.B, c, m, epoch * 2u + (cuts != 0 ? 1u : 0u));
     }
 
-    // The states before each step, from the checkpoint.
-    for (unsigned j = 0; j < w; ++j) s = apply(Map<V>{sh.map[j][lane].x, sh.fwd[j][lane]}, sh.cut[j] != 0, s);
-    if (plain)
-      backward_states<T, kForm, false>(row, 0u, kSteps, a, na, s, d);
-    else
-      backward_states<T, kForm, true>(row, resets, n, a, na, s, d);
+    // The state before the warp's steps, from the checkpoint, and in their middle.
+#pragma unroll
+    for (int j = 0; j < kWarps - 1; ++j) {
+      if (j >= int(w)) break;
+      const V x = sh.map[j][lane].x, f = sh.fwd[j][lane];
+      s = cuts == 0 ? vfma(x, s, f) : apply(Map<V>{x, f}, ((cuts >> (8 * j)) & 1u) != 0u, s);
+    }
+    const V mid = apply(q.half, (resets & ((1u << kHalf) - 1u)) != 0u, s);
 
     // 3. The gradient that comes in.
     V y = vset(V{}, 0.0f);
     if (p.grad_final != nullptr && t.k < p.g.span) load_row(p.grad_final + state_at, c, p.g.H, y);
-    incoming(p.g, t, p.B, c, epoch, sh, y);
+    incoming<kVec>(records_before(p.g, t, p.B, c), c, p.g.H, epoch, sh, y);
     if (w == 0 && more && ends)
-      publish(p.g, t, p.B, c, Map<V>{vset(V{}, 0.0f), apply(m, tile_cut, y)}, epoch * 2u + 1u);
-    for (int j = kWarps - 1; j > int(w); --j) y = apply(sh.map[j][lane], sh.cut[j] != 0, y);
+      publish(p.g, t, p.B, c, Map<V>{vset(V{}, 0.0f), apply(m, cuts != 0, y)}, epoch * 2u + 1u);
+    y = apply(pre, pre_cut, y);
 
     // 4. The steps from there, backwards.
     T* og = p.grad_gate + t.b * p.ggs.b + t0 * p.ggs.t + c;
     T* ox = p.grad_x + t.b * p.gxs.b + t0 * p.gxs.t + c;
-    if (plain && p.wide)
-      backward_steps<T, kForm, false>(row, 0u, kSteps, a, na, d, c, p.g.H, p.wide, og, p.ggs.t, ox, p.gxs.t, y);
-    else
-      backward_steps<T, kForm, true>(row, resets, n, a, na, d, c, p.g.H, p.wide, og, p.ggs.t, ox, p.gxs.t, y);
+    if (plain && p.wide) {
+      backward_steps<T, kForm, false, kHalf>(row, 0u, kSteps, q, mid, c, p.g.H, true, og, p.ggs.t, ox, p.gxs.t, y);
+      backward_steps<T, kForm, false, 0>(row, 0u, kSteps, q, s, c, p.g.H, true, og, p.ggs.t, ox, p.gxs.t, y);
+    } else {
+      backward_steps<T, kForm, true, kHalf>(row, resets, n, q, mid, c, p.g.H, p.wide, og, p.ggs.t, ox, p.gxs.t, y);
+      backward_steps<T, kForm, true, 0>(row, resets, n, q, s, c, p.g.H, p.wide, og, p.ggs.t, ox, p.gxs.t, y);
+    }
     if (p.grad_state != nullptr && t0 == 0) store_row(p.grad_state + state_at, c, p.g.H, y);
-    t = next;
   }
   leave(p.g, epoch);
 }
@@ -1053,6 +1129,7 @@ inline int forward(const void* gate, const void* x, int dtype, int form, const i
       p.granule = in.bytes();
       p.wide = out.bytes() >= 4 && H % Lane<E>::kVec == 0;
       const int smem = smem_bytes<2>(p.granule);
+      p.g.back = false;
       const auto kernel = forward_kernel<E, f.value>;
       unsigned ctas = 0;
       const int st = plan(kernel, smem, Lane<E>::kVec, B, T, H, ws, ws_bytes, &p.g, &ctas);
@@ -1094,6 +1171,7 @@ inline int backward(const void* gate, const void* x, int dtype, int form, const 
       p.granule = in.bytes();
       p.wide = out.bytes() >= 4 && H % Lane<E>::kVec == 0;
       const int smem = smem_bytes<3>(p.granule);
+      p.g.back = true;
       const auto kernel = backward_kernel<E, f.value>;
       unsigned ctas = 0;
       const int st = plan(kernel, smem, Lane<E>::kVec, B, T, H, ws, ws_bytes, &p.g, &ctas);
