@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_const
 // ------------------------------------------------------------------- many tokens: counts, then terms
 // Counts of the masked tokens, in all (token mean) or per row (sequence mean): rows cut into stretches, a warp
 // each.  Whole-number atomics, so the order does not matter.
-constexpr int kStretch = 4096;
+constexpr int kStretch = 1024;
 
 __device__ __forceinline__ unsigned ones16(const uint4& x) {
   return __popc(__vminu4(x.x, 0x01010101u)) + __popc(__vminu4(x.y, 0x01010101u)) + __popc(__vminu4(x.z, 0x01010101u)) +

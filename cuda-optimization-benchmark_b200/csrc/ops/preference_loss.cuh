@@ -34,26 +34,30 @@ struct Side {
 struct Params {
   Side side[2];  // chosen, rejected
   int B;
-  double beta, smoothing, margin, inv_B;
+  double beta, smoothing, margin, inv_B, inv_beta;
   int form;
   bool average;
   float* out;
 };
 
-// The loss of margin z and its derivative.
-__device__ __forceinline__ double pair_loss(const Params& p, double z, double& dz) {
+// The derivative of the loss of margin z.
+__device__ __forceinline__ double pair_slope(const Params& p, double z) {
   if (p.form == kSigmoid) {
-    const double e = exp(-fabs(z)), inv = 1.0 / (1.0 + e), tail = log1p(e);  // both softplus are max + tail
-    dz = p.smoothing - (z >= 0.0 ? e * inv : inv);                           // e - sigmoid(-z)
-    if (z != z) dz = z;
+    const double e = exp(-fabs(z)), inv = 1.0 / (1.0 + e);
+    return z != z ? z : p.smoothing - (z >= 0.0 ? e * inv : inv);  // e - sigmoid(-z)
+  }
+  if (p.form == kHinge) return z < 1.0 ? -1.0 : 0.0;
+  return 2.0 * (z - 0.5) * p.inv_beta * p.inv_beta;
+}
+
+// The loss of margin z.
+__device__ __forceinline__ double pair_loss(const Params& p, double z) {
+  if (p.form == kSigmoid) {
+    const double tail = log1p(exp(-fabs(z)));  // softplus(z) = max(z, 0) + tail
     return (1.0 - p.smoothing) * (fmax(-z, 0.0) + tail) + p.smoothing * (fmax(z, 0.0) + tail);
   }
-  if (p.form == kHinge) {
-    dz = z < 1.0 ? -1.0 : 0.0;
-    return z >= 1.0 ? 0.0 : 1.0 - z;  // NaN stays NaN
-  }
-  const double u = (z - 0.5) / p.beta;
-  dz = 2.0 * u / p.beta;
+  if (p.form == kHinge) return z >= 1.0 ? 0.0 : 1.0 - z;  // NaN stays NaN
+  const double u = (z - 0.5) * p.inv_beta;
   return u * u;
 }
 
@@ -208,7 +212,6 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
   constexpr int kWarps = kThreads / 32;
   __shared__ Part warp_part[2][kWarps];
   __shared__ Part cta_part[2][kMaxCluster];
-  __shared__ float slope[2];
   __shared__ bool last;
   __shared__ double total[3][kWarps];
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
@@ -251,36 +254,26 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
   } else {
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    double s[2], inv[2];
+  // Every thread forms the pair's slopes, so that no one waits for another to; one of them goes on to the loss while
+  // the rest write gradients.
+  double s[2], inv[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      Part a = cta_part[k][0];
-      for (unsigned i = 1; i < parts; ++i) a.s += cta_part[k][i].s, a.n += cta_part[k][i].n;
-      inv[k] = p.average ? 1.0 / double(a.n > 0 ? a.n : 1u) : 1.0;
-      s[k] = a.s * inv[k];
-    }
-    const double gap = p.beta * (s[0] - s[1]);
-    double dz;
-    const double loss = pair_loss(p, gap - p.margin, dz);
-    const double k = p.beta * dz * p.inv_B;
-    slope[0] = float(k * inv[0]);
-    slope[1] = float(-k * inv[1]);
-    last = false;
-    if (part == 0) {
-      pairs[b] = PairOut{loss, s[0] > s[1] ? 1.0 : 0.0, gap};
-      p.side[0].reward[b] = float(p.beta * s[0]);
-      p.side[1].reward[b] = float(p.beta * s[1]);
-    }
+  for (int k = 0; k < 2; ++k) {
+    Part a = cta_part[k][0];
+    for (unsigned i = 1; i < parts; ++i) a.s += cta_part[k][i].s, a.n += cta_part[k][i].n;
+    inv[k] = p.average ? 1.0 / double(a.n > 0 ? a.n : 1u) : 1.0;
+    s[k] = a.s * inv[k];
   }
-  __syncthreads();
-  // The first CTA of a pair counts it as done while the others of its threads write gradients.
-  if (threadIdx.x == 0 && part == 0) {
+  const double gap = p.beta * (s[0] - s[1]), slope = p.beta * pair_slope(p, gap - p.margin) * p.inv_B;
+  if (part == 0 && threadIdx.x == kThreads - 1) {
+    pairs[b] = PairOut{pair_loss(p, gap - p.margin), s[0] > s[1] ? 1.0 : 0.0, gap};
+    p.side[0].reward[b] = float(p.beta * s[0]);
+    p.side[1].reward[b] = float(p.beta * s[1]);
     __threadfence();
     last = atomicAdd(&ctl->done, 1u) == unsigned(p.B) - 1u;
   }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) write_stretch<kThreads>(row[k], slope[k]);
+  write_stretch<kThreads>(row[0], float(slope * inv[0]));
+  write_stretch<kThreads>(row[1], float(-slope * inv[1]));
   if (part != 0) return;
   __syncthreads();
   if (!last) return;
@@ -347,7 +340,7 @@ inline int run(const float* chosen, const float* rejected, const float* ref_chos
   p.side[0] = Side{chosen, ref_chosen, chosen_mask, strides[0], strides[2], strides[4], Tc, reward_chosen, grad_chosen};
   p.side[1] =
       Side{rejected, ref_rejected, rejected_mask, strides[1], strides[3], strides[5], Tr, reward_rejected, grad_rejected};
-  p.B = B, p.inv_B = 1.0 / B, p.beta = beta, p.smoothing = smoothing, p.margin = margin, p.form = form, p.average = average != 0;
+  p.B = B, p.inv_B = 1.0 / B, p.inv_beta = 1.0 / beta, p.beta = beta, p.smoothing = smoothing, p.margin = margin, p.form = form, p.average = average != 0;
   p.out = out;
   const unsigned parts = cluster_of(B, int64_t(Tc) + Tr);
   if (int64_t(B) * parts > 0x7fffffff) return kUnsupported;
