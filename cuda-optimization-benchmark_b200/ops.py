@@ -688,12 +688,17 @@ def _bth(gate, x, form):
     return device, DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form], shape
 
 
+def _dense_like(t):
+    """A contiguous output of t's shape and dtype."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _like_bth(x):
     """An output of x's shape and dtype: dense, time first in memory when x is."""
     B, T, H = x.shape
     if B > 1 and T > 1 and x.stride(0) < x.stride(1):
         return x.new_empty((T, B, H)).transpose(0, 1)
-    return x.new_empty((B, T, H))
+    return _dense_like(x)
 
 
 def _writable(t, like, name):
@@ -858,7 +863,7 @@ def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, s
         _need(slots, "slots", torch.int32, dev)
         if slots.shape != (B,):
             raise ValueError(f"slots must be ({B},)")
-    h = x.new_empty((B, H)) if out is None else _apart(_writable(out, x, "out"), "out", gate=gate, x=x, state=state,
+    h = _dense_like(x) if out is None else _apart(_writable(out, x, "out"), "out", gate=gate, x=x, state=state,
                                                        state_out=state_out)
     _run("linear_recurrence_step", _lib().b200_linear_recurrence_step_async, dev.index, gate.data_ptr(), x.data_ptr(),
          DTYPE_CODES[x.dtype], RECURRENCE_FORMS[form], _strides(gate.stride(0), x.stride(0), h.stride(0)),
@@ -935,7 +940,7 @@ def _token_logprob(logits, token, temperature, entropy, train):
     dev, dt, B, T, V, st = _token_args(logits, token)
     temperature = _temperature(temperature)
     lp = torch.empty(token.shape, dtype=torch.float32, device=dev)
-    ent = torch.empty(token.shape, dtype=torch.float32, device=dev) if entropy else None
+    ent = _dense_like(lp) if entropy else None
     stats = torch.empty((*token.shape, 3), dtype=torch.float32, device=dev) if train else None
     _run("token_logprob", _lib().b200_token_logprob_async, dev.index, logits.data_ptr(), dt, st, token.data_ptr(), B, T,
          V, temperature, lp.data_ptr(), _address(ent), _address(stats))
@@ -973,7 +978,7 @@ def token_logprob_backward(logits, token, stats, grad_log_prob, grad_entropy=Non
         if t.shape != shape:
             raise ValueError(f"{nm} must be {tuple(shape)}")
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        out = _dense_like(logits)
     else:
         _need(out, "out", logits.dtype, dev)
         if out.shape != logits.shape:
@@ -1017,6 +1022,9 @@ PREFERENCE_OUTPUTS = ("loss", "accuracy", "margin")
 
 def _token_stream(t, name, B, T, device, dtype=torch.float32):
     """A [B, T] per-token tensor with a contiguous token axis."""
+    if isinstance(t, torch.Tensor) and t.shape == (B, T) and t.dtype == dtype and t.stride(1) == 1 \
+            and t.device == device:
+        return t
     _float_tensor(t, name, device, dtype, 2)
     if t.shape != (B, T):
         raise ValueError(f"{name} must be ({B}, {T}), got {tuple(t.shape)}")
@@ -1085,8 +1093,8 @@ def _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy,
     options = _policy_options(clip_low, clip_high, dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale,
                               ref_log_prob is not None, entropy is not None)
     out = torch.empty(8, dtype=torch.float32, device=dev)
-    grad = torch.empty((B, T), dtype=torch.float32, device=dev) if want_grad else None
-    ge = torch.empty((B, T), dtype=torch.float32, device=dev) if want_grad_entropy else None
+    grad = _dense_like(log_prob) if want_grad else None
+    ge = _dense_like(log_prob) if want_grad_entropy else None
     n_ws = _policy_scratch_bytes(B, T)
     ws = _scratch("policy_loss", n_ws, dev) if n_ws else None
     _run("policy_loss", _lib().b200_policy_loss_async, dev.index, log_prob.data_ptr(), old.data_ptr(),
@@ -1190,8 +1198,8 @@ def _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, re
     out = torch.empty(3, dtype=torch.float32, device=dev)
     rc = torch.empty(B, dtype=torch.float32, device=dev)
     rr = torch.empty(B, dtype=torch.float32, device=dev)
-    gc = torch.empty((B, Tc), dtype=torch.float32, device=dev) if want_chosen else None
-    gr = torch.empty((B, Tr), dtype=torch.float32, device=dev) if want_rejected else None
+    gc = _dense_like(chosen) if want_chosen else None
+    gr = _dense_like(rejected) if want_rejected else None
     ws = _scratch("preference_loss", _preference_scratch_bytes(B), dev)
     _run("preference_loss", _lib().b200_preference_loss_async, dev.index, chosen.data_ptr(), rejected.data_ptr(),
          _address(ref_chosen), _address(ref_rejected), _address(chosen_mask), _address(rejected_mask),
