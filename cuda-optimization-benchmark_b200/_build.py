@@ -6,6 +6,9 @@ Everything is compiled in-tree with nvcc for sm_100a only:
          -o <package>/libb200ops.so <package>/csrc/capi.cu
 
 The build is skipped when the library is newer than every source under csrc/ and include/.
+
+The package's CPython module over torch's C++ API (_calls, host code alone: csrc/python/calls.cpp) is compiled with
+the host compiler by build_calls().
 """
 import os
 import subprocess
@@ -16,6 +19,8 @@ PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libb200ops.so"
+CALLS_SOURCE = CSRC / "python" / "calls.cpp"
+CALLS = PKG / "_calls.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3"]
 
@@ -58,6 +63,32 @@ def build_library(force=False, verbose=False):
     return LIB
 
 
+def build_calls(force=False, verbose=False):
+    """Compile _calls.so in-tree against the installed torch; returns its path.  Raises on a compile error."""
+    newest = max(CALLS_SOURCE.stat().st_mtime, *(p.stat().st_mtime for p in (REPO / "include").glob("*.h")))
+    if not force and CALLS.exists() and CALLS.stat().st_mtime >= newest:
+        return CALLS
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    cuda = Path(nvcc()).resolve().parent.parent
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(cuda / "include")]
+    libs = cpp_extension.library_paths()
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{p}" for p in includes),
+           str(CALLS_SOURCE), *(f"-L{p}" for p in libs), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+           "-ltorch_python", "-ldl", "-o", str(CALLS) + ".tmp"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"the host compiler failed building {CALLS.name} (exit {r.returncode})")
+    os.replace(str(CALLS) + ".tmp", CALLS)
+    return CALLS
+
+
 def build_grader_libs(verbose=False):
     """Build every abi/<task>/solution.cu the way the reference grader does (in parallel)."""
     import importlib.util
@@ -77,3 +108,4 @@ def build_grader_libs(verbose=False):
 
 if __name__ == "__main__":
     print(build_library(force="--force" in sys.argv, verbose=True))
+    print(build_calls(force="--force" in sys.argv, verbose=True))

@@ -5,6 +5,7 @@ There is no fallback: if the library is missing or fails to load, every op raise
 `__graft_entry__.build()` (or `python -m` on `_build.py`) first.
 """
 import ctypes
+import functools
 from pathlib import Path
 
 from . import _build
@@ -153,6 +154,19 @@ def load():
         fn.argtypes = args
     _LIB = lib
     return lib
+
+
+@functools.cache
+def calls():
+    """The module _calls over the library (the short way for the sequence-policy operators), None where it is not built
+    or was built for another torch: ctypes serves their calls then."""
+    load()
+    try:
+        from . import _calls
+    except ImportError:
+        return None
+    _calls.init(str(library_path()), OpError)
+    return _calls
 
 
 def check(status, what):

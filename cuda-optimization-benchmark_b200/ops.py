@@ -634,6 +634,16 @@ def _run(what, fn, index, *args):
         _native.check(status, what)
 
 
+def _call(name, *args):
+    """An operator's outputs by the short way (csrc/python/calls.cpp), which takes its ordinary calls; None where the
+    call has to go the long way, through the checks below and ctypes."""
+    calls = _native.calls()
+    if calls is None:
+        return None
+    with _LAUNCH:
+        return getattr(calls, name)(*args)
+
+
 def _address(t):
     return None if t is None else t.data_ptr()
 
@@ -773,7 +783,16 @@ def _recurrence_scratch(nbytes, device):
     return ws, ws.data_ptr(), ws.numel()
 
 
+def _form_code(forms, form):
+    """The C ABI's number of a form, -1 for none."""
+    return forms.get(form, -1) if isinstance(form, str) else -1
+
+
 def _recurrence_forward(gate, x, state, reset, form, out, train):
+    if out is None:
+        r = _call("recurrence", gate, x, state, reset, _form_code(RECURRENCE_FORMS, form), train)
+        if r is not None:
+            return r
     dev, dt, fm, (B, T, H) = _bth(gate, x, form)
     state = _state_arg(state, "state", B, H, dev)
     reset = _reset_arg(reset, B, T, dev)
@@ -809,6 +828,10 @@ def linear_recurrence_train(gate, x, state=None, reset=None, form="decay"):
 def linear_recurrence_backward(gate, x, checkpoints, grad_h, grad_final=None, reset=None, form="decay"):
     """Gradients of linear_recurrence: (grad_gate, grad_x, grad_state) for grad_h [B, T, H] (x's dtype) and
     grad_final (fp32 [B, H] or None)."""
+    r = _call("recurrence_backward", gate, x, checkpoints, grad_h, grad_final, reset,
+              _form_code(RECURRENCE_FORMS, form))
+    if r is not None:
+        return r
     dev, dt, fm, (B, T, H) = _bth(gate, x, form)
     _float_tensor(grad_h, "grad_h", dev, x.dtype, 3)
     if grad_h.shape != x.shape:
@@ -834,6 +857,10 @@ def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, s
     (or written to state_out).  slots (int32 [B]) names each row's state, row b its own without it.  Rows
     with the same slot are consecutive tokens of one sequence, in row order; a row whose slot is outside
     [0, S) is skipped (its h row is left as it was, so pass `out` to know what it holds)."""
+    if out is None:
+        r = _call("recurrence_step", gate, x, state, slots, _form_code(RECURRENCE_FORMS, form), state_out)
+        if r is not None:
+            return r[0]
     if form not in RECURRENCE_FORMS:
         raise ValueError(f"form must be one of {sorted(RECURRENCE_FORMS)}, got {form!r}")
     _float_tensor(x, "x", dims=2)
@@ -937,6 +964,9 @@ def _temperature(temperature):
 
 
 def _token_logprob(logits, token, temperature, entropy, train):
+    r = _call("logprob", logits, token, temperature, bool(entropy), train)
+    if r is not None:
+        return r
     dev, dt, B, T, V, st = _token_args(logits, token)
     temperature = _temperature(temperature)
     lp = torch.empty(token.shape, dtype=torch.float32, device=dev)
@@ -968,6 +998,10 @@ def token_logprob_train(logits, token, temperature=1.0, entropy=True):
 def token_logprob_backward(logits, token, stats, grad_log_prob, grad_entropy=None, temperature=1.0, out=None):
     """grad_logits (contiguous, of logits' dtype) for the gradients of token_logprob's outputs (fp32).  out may
     be the logits themselves when these are contiguous (they are overwritten)."""
+    if out is None:
+        r = _call("logprob_backward", logits, token, stats, grad_log_prob, grad_entropy, temperature)
+        if r is not None:
+            return r[0]
     dev, dt, B, T, V, st = _token_args(logits, token)
     temperature = _temperature(temperature)
     for t, nm, shape in ((stats, "stats", (*token.shape, 3)), (grad_log_prob, "grad_log_prob", token.shape),
@@ -1042,10 +1076,18 @@ def _number(v, name):
     return v
 
 
-@functools.lru_cache(maxsize=256)
 def _policy_options(clip_low, clip_high, dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale, has_ref,
                     has_entropy):
-    """The loss's options checked, as the C ABI takes them."""
+    """The loss's options checked, as the C ABI takes them.  They are made Python's numbers first, so that a tensor is
+    read in every call."""
+    return _checked_policy_options(float(clip_low), float(clip_high), None if dual_clip is None else float(dual_clip),
+                                   float(kl_coef), kl_form, float(entropy_coef), reduction, float(scale), has_ref,
+                                   has_entropy)
+
+
+@functools.lru_cache(maxsize=256)
+def _checked_policy_options(clip_low, clip_high, dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale, has_ref,
+                            has_entropy):
     if kl_form not in KL_FORMS:
         raise ValueError(f"kl_form must be one of {sorted(KL_FORMS)}, got {kl_form!r}")
     if reduction not in LOSS_REDUCTIONS:
@@ -1072,6 +1114,12 @@ def _policy_scratch_bytes(B, T):
 
 def _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy, clip_low, clip_high, dual_clip,
                  kl_coef, kl_form, entropy_coef, reduction, scale, want_grad, want_grad_entropy):
+    options = _policy_options(clip_low, clip_high, dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale,
+                              ref_log_prob is not None, entropy is not None)
+    r = _call("policy", log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy, options, want_grad,
+              want_grad_entropy)
+    if r is not None:
+        return r
     _float_tensor(log_prob, "log_prob", dtype=torch.float32, dims=2)
     dev = log_prob.device
     B, T = log_prob.shape
@@ -1090,8 +1138,6 @@ def _policy_loss(log_prob, old_log_prob, advantage, mask, ref_log_prob, entropy,
         _token_stream(ref_log_prob, "ref_log_prob", B, T, dev)
     if entropy is not None:
         _token_stream(entropy, "entropy", B, T, dev)
-    options = _policy_options(clip_low, clip_high, dual_clip, kl_coef, kl_form, entropy_coef, reduction, scale,
-                              ref_log_prob is not None, entropy is not None)
     out = torch.empty(8, dtype=torch.float32, device=dev)
     grad = _dense_like(log_prob) if want_grad else None
     ge = _dense_like(log_prob) if want_grad_entropy else None
@@ -1158,9 +1204,13 @@ class PolicyLossFunction(torch.autograd.Function):
                 None, None)
 
 
-@functools.lru_cache(maxsize=256)
 def _preference_options(beta, form, label_smoothing, margin):
-    """The loss's options checked, as the C ABI takes them."""
+    """The loss's options checked, as the C ABI takes them (as in _policy_options)."""
+    return _checked_preference_options(float(beta), form, float(label_smoothing), float(margin))
+
+
+@functools.lru_cache(maxsize=256)
+def _checked_preference_options(beta, form, label_smoothing, margin):
     if form not in PREFERENCE_FORMS:
         raise ValueError(f"form must be one of {sorted(PREFERENCE_FORMS)}, got {form!r}")
     beta, margin = _number(beta, "beta"), _number(margin, "margin")
@@ -1179,6 +1229,11 @@ def _preference_scratch_bytes(B):
 
 def _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, form,
                      label_smoothing, margin, average, want_chosen, want_rejected):
+    options = _preference_options(beta, form, label_smoothing, margin)
+    r = _call("preference", chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, options,
+              bool(average), want_chosen, want_rejected)
+    if r is not None:
+        return r
     _float_tensor(chosen, "chosen", dtype=torch.float32, dims=2)
     dev = chosen.device
     _float_tensor(rejected, "rejected", dev, torch.float32, 2)
@@ -1194,7 +1249,6 @@ def _preference_loss(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, re
         _token_stream(chosen_mask, "chosen_mask", B, Tc, dev, torch.bool)
     if rejected_mask is not None:
         _token_stream(rejected_mask, "rejected_mask", B, Tr, dev, torch.bool)
-    options = _preference_options(beta, form, label_smoothing, margin)
     out = torch.empty(3, dtype=torch.float32, device=dev)
     rc = torch.empty(B, dtype=torch.float32, device=dev)
     rr = torch.empty(B, dtype=torch.float32, device=dev)

@@ -5,7 +5,8 @@ The whole step is held against the same step in fp64 (torch autograd over elemen
 import pytest
 import torch
 
-from sequence_policy import load_ops
+from conftest import pkg
+from sequence_policy import captured, load_ops, same_bits
 
 
 @pytest.fixture(scope="module")
@@ -178,3 +179,74 @@ def test_captured_training_step(ops):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.allclose(a, b, rtol=1e-4, atol=1e-6)
+
+
+def test_options_held_in_tensors_are_read_every_call():
+    ops = pkg().ops
+    v = torch.tensor(0.5)
+    policy = lambda: ops._policy_options(0.2, 0.2, None, v, "k3", 0.0, "sum", 1.0, True, False)[3]
+    preference = lambda: ops._preference_options(v, "sigmoid", 0.0, 0.0)[0]
+    assert (policy(), preference()) == (0.5, 0.5)
+    v.fill_(0.25)
+    assert (policy(), preference()) == (0.25, 0.25)
+
+
+def everything(ops, s, dtype):
+    """Every operator once: all outputs."""
+    x, gate, reset = s["x"].to(dtype), s["gate"].to(dtype), s["reset"]
+    h, final, ckpt = ops.linear_recurrence_train(gate, x, s["state"], reset, "sigmoid")
+    out = [h, final, ckpt, *ops.linear_recurrence(gate.transpose(0, 1).contiguous().transpose(0, 1), x, form="sigmoid")]
+    out += ops.linear_recurrence_backward(gate, x, ckpt, h, final, reset, "sigmoid")
+    pool, after = s["state"].clone(), torch.zeros_like(s["state"])
+    out += [ops.linear_recurrence_step(gate[:, 0], x[:, 0], pool, s["slots"]), pool,
+            ops.linear_recurrence_step(gate[:, 1], x[:, 1], pool, None, "sigmoid", state_out=after), after]
+    lp, ent, stats = ops.token_logprob_train(h, s["token"], 0.7)
+    out += [lp, ent, stats, *ops.token_logprob(h[:, 1:], s["token"][:, 1:]), ops.token_logprob(h[0], s["token"][0], 2.0, False)[0],
+            ops.token_logprob_backward(h, s["token"], stats, lp, ent, 0.7)]
+    out += ops.policy_loss_grad(lp, s["old"], s["adv"], s["mask"], s["old"], ent, kl_coef=0.1, entropy_coef=0.01)
+    out += [ops.policy_loss(lp, None, lp, reduction="sum", dual_clip=3.0)]
+    out += ops.preference_loss_grad(lp, lp[:, 5:], s["old"], s["old"][:, 5:], s["mask"], None, average=True)
+    out += ops.preference_loss(lp, s["old"], form="hinge", margin=0.5)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_both_ways_of_a_call_agree(ops, monkeypatch, dtype):
+    """What the module _calls returns has the bits of the call through ctypes, also while it is captured."""
+    B, T, H = 3, 300, 200
+    g = torch.Generator().manual_seed(5)
+    s = {"x": torch.randn(B, T, H, generator=g).cuda(), "gate": torch.rand(B, T, H, generator=g).cuda(),
+         "reset": (torch.rand(B, T, generator=g) < 0.02).cuda(), "state": torch.randn(B, H, generator=g).cuda(),
+         "slots": torch.tensor([2, 0, 2], dtype=torch.int32).cuda(), "token": torch.randint(-1, H, (B, T), generator=g).cuda(),
+         "old": -torch.rand(B, T, generator=g).cuda() * 8, "adv": torch.randn(B, generator=g).cuda(),
+         "mask": (torch.rand(B, T, generator=g) < 0.8).cuda()}
+    native = pkg()._native
+    assert native.calls() is not None
+    short = everything(ops, s, dtype)
+    graph, during = captured(lambda: everything(ops, s, dtype))
+    graph.replay()
+    monkeypatch.setattr(native, "calls", lambda: None)
+    long = everything(ops, s, dtype)
+    assert len(short) == len(long) == len(during)
+    for a, b, c in zip(short, long, during):
+        assert a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
+        assert same_bits(a, b) and same_bits(c, b)
+
+
+@pytest.mark.gpu
+def test_calls_leave_what_they_cannot_take(ops):
+    """The short way returns None for wrong arguments, and the checks in front of the long way say what is wrong."""
+    calls = pkg()._native.calls()
+    x = torch.zeros(2, 3, 4).cuda()
+    for bad in (x.double(), x.cpu(), x[0], x.transpose(1, 2), torch.zeros(0, 3, 4).cuda(), None, 3, x.to_sparse()):
+        assert calls.recurrence(x, bad, None, None, 0, False) is None
+        assert calls.recurrence(bad, x, None, None, 0, False) is None
+        assert calls.recurrence(x, x, bad, None, 0, False) is None or bad is None
+        assert calls.recurrence(x, x, None, bad, 0, False) is None or bad is None
+    for form in (-1, "decay", None, 1.0, 2 ** 70):
+        assert calls.recurrence(x, x, None, None, form, False) is None
+    with pytest.raises(ValueError, match="form"):
+        ops.linear_recurrence(x, x, form="other")
+    with pytest.raises(ValueError, match="last dimension"):
+        ops.linear_recurrence(x.transpose(1, 2), x.transpose(1, 2))
