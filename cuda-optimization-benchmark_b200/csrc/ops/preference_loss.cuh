@@ -10,6 +10,11 @@
 // reward_rejected.  Every masked token of an answer has the gradient +-beta dloss/dz / B (/ its
 // answer's tokens when `average`).  An answer without tokens has s = 0.
 // The sums are in fp64: their difference, a small part of them, is what the loss sees.
+//
+// What bounds it: memory for many tokens, and for few the latency of a launch with its reductions.  One kernel does it
+// all: the pair's slope is known as soon as its CTAs have met, and the gradients, constant along an answer, are
+// written then.  Measured: 4 pairs of 700 and 523 tokens 6.7 us; 512 pairs of 8192 tokens with references and masks 20.1 us
+// (5.4 TB/s); 2 pairs of 131072 tokens 17 us.
 #pragma once
 
 #include "../common/bulk.cuh"
@@ -76,6 +81,8 @@ struct Ctl {
   unsigned done;
 };
 
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kVecs = 2;      // vectors of four tokens of a lane in flight, log-probs and references
 constexpr int kPer = 4 * kVecs;
@@ -126,7 +133,6 @@ __device__ __forceinline__ Row row_of(const Side& d, int64_t b, unsigned part, u
 }
 
 // The stretch's sum and count.  What masked-out tokens hold is read with the others and not used.
-template <int kThreads>
 __device__ __forceinline__ Part sum_stretch(const Row& d) {
   double s = 0.0;
   unsigned n = 0;
@@ -170,7 +176,6 @@ __device__ __forceinline__ Part sum_stretch(const Row& d) {
   return Part{s, n};
 }
 
-template <int kThreads>
 __device__ __forceinline__ void write_stretch(const Row& d, float slope) {
   if (d.grad == nullptr) return;
   for (int t = d.v0 + int(threadIdx.x) * 4; t < d.v1; t += kPer * kThreads) {
@@ -207,9 +212,8 @@ __device__ __forceinline__ void write_stretch(const Row& d, float slope) {
 // A cluster of `parts` CTAs per pair, each on a stretch of both answers: the CTAs exchange their sums through
 // shared memory, every one forms the pair's slope from all of them in the same order and writes its
 // stretch of the gradients.  The last CTA of the grid adds up the pairs in their order.
-template <int kThreads>
-__global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ Params p, unsigned parts, Ctl* ctl, PairOut* pairs) {
-  constexpr int kWarps = kThreads / 32;
+__global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ Params p, unsigned parts, Ctl* ctl,
+                                                        PairOut* pairs) {
   __shared__ Part warp_part[2][kWarps];
   __shared__ Part cta_part[2][kMaxCluster];
   __shared__ bool last;
@@ -224,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     row[k] = row_of(p.side[k], b, part, parts);
-    Part a = sum_stretch<kThreads>(row[k]);
+    Part a = sum_stretch(row[k]);
     a.s = warp_sum(a.s);
     a.n = warp_sum_u32(a.n);
     if (lane == 0) warp_part[k][w] = a;
@@ -272,8 +276,8 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
     __threadfence();
     last = atomicAdd(&ctl->done, 1u) == unsigned(p.B) - 1u;
   }
-  write_stretch<kThreads>(row[0], float(slope * inv[0]));
-  write_stretch<kThreads>(row[1], float(-slope * inv[1]));
+  write_stretch(row[0], float(slope * inv[0]));
+  write_stretch(row[1], float(-slope * inv[1]));
   if (part != 0) return;
   __syncthreads();
   if (!last) return;
@@ -300,18 +304,16 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
   }
 }
 
-// Threads of a CTA: with few pairs (the largest cluster each) a CTA has an SM for itself, and only more threads
-// keep more of its stretch in flight.
-constexpr int kPairThreads = 256;
-constexpr int kLongThreads = 1024;
-
 inline int64_t workspace_bytes(int32_t B) { return int64_t(256 + align256(size_t(B) * sizeof(PairOut))); }
 
-// CTAs per pair: 1 once two CTAs per SM have a pair each, else enough for that, but no CTA with fewer than
-// 2048 tokens.
+// CTAs per pair: doubled while two CTAs per SM hold them all and none has fewer than 4096 tokens.  Measured with 1, 2, 4 and
+// 8 CTAs per pair: 16 pairs of 2 x 16384 tokens 16.0, 12.0, 9.7 and 9.1 us, 64 of 2 x 4096 9.2, 8.9, 9.1 and 10.2, 256
+// of 2 x 2048 8.3, 11.1, 14.0 and 20.6; a pair of 2 x 512 takes 6.4 us with one and 6.8 with two.  CTAs of 1024 threads
+// took 1 to 3 us more than these of 256 up to 2 pairs of 2 x 32768 tokens, and twice the time for many pairs (2 pairs of 2 x
+// 131072, 14 us against 17, are what they were good for).
 inline unsigned cluster_of(int64_t pairs, int64_t tokens) {
   unsigned c = 1;
-  while (c < unsigned(kMaxCluster) && pairs * c < 2 * sm_count() && tokens / (2 * c) >= 2048) c *= 2;
+  while (c < unsigned(kMaxCluster) && pairs * 2 * c <= 2 * sm_count() && tokens / (2 * c) >= 4096) c *= 2;
   return c;
 }
 
@@ -333,7 +335,7 @@ inline int run(const float* chosen, const float* rejected, const float* ref_chos
       reward_rejected == nullptr)
     return kInvalidArgument;
   // Token indexes run in ints, up to a round of the CTA past the end.
-  if (Tc > 0x7fffffff - 2 * kPer * kLongThreads || Tr > 0x7fffffff - 2 * kPer * kLongThreads) return kUnsupported;
+  if (Tc > 0x7fffffff - 2 * kPer * kThreads || Tr > 0x7fffffff - 2 * kPer * kThreads) return kUnsupported;
   if (ws == nullptr || ws_bytes < workspace_bytes(B)) return kWorkspaceTooSmall;
   if (!aligned16(ws)) return kInvalidArgument;
   Params p;
@@ -346,8 +348,7 @@ inline int run(const float* chosen, const float* rejected, const float* ref_chos
   if (int64_t(B) * parts > 0x7fffffff) return kUnsupported;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(B) * parts);
-  const bool wide = parts == unsigned(kMaxCluster);
-  cfg.blockDim = dim3(wide ? kLongThreads : kPairThreads);
+  cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -357,7 +358,7 @@ inline int run(const float* chosen, const float* rejected, const float* ref_chos
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = parts > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, wide ? pair_kernel<kLongThreads> : pair_kernel<kPairThreads>, p, parts, static_cast<Ctl*>(ws),
+  return cudaLaunchKernelEx(&cfg, pair_kernel, p, parts, static_cast<Ctl*>(ws),
                             reinterpret_cast<PairOut*>(static_cast<char*>(ws) + 256)) == cudaSuccess
              ? kOk
              : kCudaError;

@@ -17,9 +17,17 @@
 // to both limits), everything else is packed two to an instruction.  The backward reads the logits once
 // more and writes the gradient.
 //
-// Split (the numbers are measured, bf16): a warp per row up to kWarpRowV logits; above, a CTA per row when
-// rows fill the GPU, and with few rows a cluster of up to 8 CTAs per row, each on a stretch of it, whose partial results meet
-// in the first CTA's shared memory.
+// Split: a warp per row where there are many rows for their length (warps_take), else a CTA per row (the backward: per
+// piece of one), and in the forward, with few long rows, a cluster of up to 8 CTAs per row, each on a stretch of it, whose
+// partial results meet in the first CTA's shared memory.
+//
+// Measured, bf16, forward and backward (a plain copy runs at 6.56 TB/s on the same GPU):
+//   16 rows of 32768 (forward): 3.0 us, of which an empty launch is 2;
+//   4096 rows of 131072: 150 us and 335 us (6.4 TB/s, counting the rows that are masked, which only the backward
+//   writes);
+//   2044 rows of 50001: 36 us (5.7 TB/s) and 78 us (5.2 TB/s; 63 us at 50000, where rows are on 16 bytes);
+//   37888 rows of 512: 19 us each (2 and 4 TB/s): a warp's row is then two vectors a lane, and the reductions over
+//   the warp take longer than its loads.
 #pragma once
 
 #include <math.h>
@@ -34,7 +42,6 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;          // vectors in flight per thread
 constexpr int kMaxCluster = 8;
-constexpr int64_t kWarpRowV = 8192;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Below this, 2^z is 0 in fp32: z is held above it so that 0 * z stays 0 (z = -inf at masked logits).
@@ -452,6 +459,18 @@ inline int with_flag(bool flag, F&& f) {
   return flag ? f(std::true_type{}) : f(std::false_type{});
 }
 
+// Whether a warp takes a row alone: the time of one row grows with its length then, while many warps share the GPU, and a
+// CTA has its reductions to pay for, so it takes the more rows the longer they are.  The factor is where both are alike;
+// measured, us, warp and CTA per row, bf16:
+//   forward  V 512: 256 rows 2.5 and 3.0, 9472 rows 6.2 and 24;  V 2048: 256 rows 3.2 and 3.2, 9472 rows 9.8 and 28;
+//            V 6000: 592 rows 6.4 and 4.9, 2368 rows 8.2 and 10.1, 37888 rows 87 and 136;
+//            V 12000: 1184 rows 9.6 and 8.2, 37888 rows 141 and 188;  V 24000: 2368 rows 28 and 23, 37888 rows 266 and 293
+//   backward V 512: 256 rows 2.2 and 2.7;  V 2048: 256 rows 3.7 and 2.5, 9472 rows 12.5 and 30;
+//            V 6000: 2368 rows 11.5 and 11.6, 37888 rows 150 and 162;  V 12000: 9472 rows 81 and 78, 37888 rows 298 and 345
+constexpr int64_t kForwardRows = 32768, kBackwardRows = 8192;
+constexpr int64_t kWarpRowV = 32768;  // the longest row that was measured
+inline bool warps_take(int64_t rows, int64_t V, int64_t factor) { return V <= kWarpRowV && rows * factor >= V * V; }
+
 // CTAs per row: 1 once two CTAs per SM have a row each, else enough for that, but no CTA with fewer than
 // 8192 logits: joining a cluster costs more than it saves there (64 rows of 50001 bf16 logits: 5.2 us with
 // 4 CTAs a row, 6.2 us with 8; 2044 rows: 37 us with one, 42 us with 2, 56 us with 4).
@@ -469,7 +488,7 @@ inline int forward(const void* logits, int dtype, const int64_t* strides, const 
   if (st >= 0) return st;
   if (log_prob == nullptr) return kInvalidArgument;
   const Rows q = rows_of(strides, B, T, V);
-  const bool warp_rows = V <= kWarpRowV;
+  const bool warp_rows = warps_take(q.rows, V, kForwardRows);
   const unsigned parts = warp_rows ? 1u : cluster_of(q.rows, V);
   const int64_t grid = warp_rows ? (int64_t(q.rows) + kWarps - 1) / kWarps : int64_t(q.rows) * parts;
   if (grid > 0x7fffffff) return kInvalidArgument;
@@ -509,7 +528,7 @@ inline int backward(const void* logits, int dtype, const int64_t* strides, const
   if (st >= 0) return st;
   if (stats == nullptr || grad_log_prob == nullptr || grad_logits == nullptr) return kInvalidArgument;
   const Rows q = rows_of(strides, B, T, V);
-  const bool warp_rows = V <= kWarpRowV;
+  const bool warp_rows = warps_take(q.rows, V, kBackwardRows);
   const int64_t vecs = (int64_t(V) * dtype_size(dtype) + 15) / 16;
   const unsigned pieces = warp_rows ? 1u : unsigned((vecs + kPieceVecs - 1) / kPieceVecs);
   const int64_t grid = warp_rows ? (int64_t(q.rows) + kWarps - 1) / kWarps : int64_t(q.rows) * pieces;
