@@ -15,6 +15,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <dlfcn.h>
@@ -112,8 +113,9 @@ T* ptr(const Tensor* t) {
   return static_cast<T*>(at_(t));
 }
 
+// A new tensor, without the way through torch's dispatcher.
 Tensor make(at::IntArrayRef shape, at::ScalarType type, const Place& p) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(p.device));
+  return at::detail::empty_cuda(shape, type, p.device, std::nullopt);
 }
 
 enum Op { kRecurrence, kPolicy, kPreference };
