@@ -22,7 +22,7 @@
 // partial results meet in the first CTA's shared memory.
 //
 // Measured, bf16, forward and backward (a plain copy runs at 6.56 TB/s on the same GPU):
-//   16 rows of 32768 (forward): 3.0 us, of which an empty launch is 2;
+//   16 rows of 32768 (forward): 3.0 us (the smallest calls take 1.9);
 //   4096 rows of 131072: 150 us and 335 us (6.4 TB/s, counting the rows that are masked, which only the backward
 //   writes);
 //   2044 rows of 50001: 36 us (5.7 TB/s) and 78 us (5.2 TB/s; 63 us at 50000, where rows are on 16 bytes);
