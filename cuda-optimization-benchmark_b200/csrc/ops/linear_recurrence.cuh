@@ -35,7 +35,7 @@
 // 1024 channels of 16 bits: 196 us with spans up to 4, 162 up to 8, 150 up to 16).
 //
 // Measured, forward and backward (a plain copy runs at 6.56 TB/s on the same GPU), B = 8, T = 4096, H = 2048:
-//   bf16 sigmoid 86 us (4.7 TB/s) and 130 us (5.2 TB/s), bf16 decay 77 and 115 us;
+//   bf16 sigmoid 86 us (4.7 TB/s) and 130 us (5.2 TB/s), bf16 decay 74 and 116 us;
 //   fp32 sigmoid 127 us (6.3 TB/s) and 211 us (6.4 TB/s).
 // So fp32 is bound by memory.  With 16 bits the same bytes carry twice the elements: 21 and 37 instructions an element
 // leave a warp of the 16 on an SM issuing in 45 to 50 % of the cycles, and what it waits for is its own arithmetic
@@ -320,13 +320,13 @@ struct __align__(2 * sizeof(V)) Map {
   V x, b;
 };
 
-// Shared memory beside the tile buffers.
-template <typename V, bool kBack>
+// Shared memory beside the tile buffers; kLook: records that it holds at once.
+template <typename V, bool kBack, int kLook>
 struct Shared {
   Map<V> map[kWarps][32];        // the warps' maps (scan direction)
   V fwd[kBack ? kWarps - 1 : 1][32];  // the warps' forward offsets (backward kernel; the factor is map.x)
-  Map<V> look[kMaxSpan][32];     // records of the tiles before this one
-  unsigned look_cut[kMaxSpan];
+  Map<V> look[kLook][32];        // records of the tiles before this one
+  unsigned look_cut[kLook];
   uint64_t cut;                  // byte w: warp w's steps hold a reset, its map does not see what comes in
   Tile tile[2];                  // of the CTA's tiles in turn
   uint64_t full[2];              // the tile buffers' loads have landed (tensor loads)
@@ -418,22 +418,29 @@ __device__ __forceinline__ Before records_before(const Grid& g, const Tile& t, i
 }
 
 // What comes into the tile, for this lane's channels: y on entry is the value before tile 0.  Warp w brings
-// records w and w + 8.  Every thread of the CTA calls it.
-template <int kVec, typename V, bool kBack>
-__device__ __forceinline__ void incoming(const Before& f, int c, int H, unsigned epoch, Shared<V, kBack>& sh, V& y) {
+// record w of every kWarps, kLook of them at a time.  Every thread of the CTA calls it.
+template <int kVec, typename V, bool kBack, int kLook>
+__device__ __forceinline__ void incoming(const Before& f, int c, int H, unsigned epoch, Shared<V, kBack, kLook>& sh,
+                                         V& y) {
+  static_assert(kLook % kWarps == 0 && kMaxSpan % kLook == 0, "");
   if (f.n == 0) return;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
-  for (unsigned i = w; i < f.n; i += kWarps) {
-    const ulonglong2* r = f.first + i * f.step;
-    unsigned cut;
-    Map<V> m;
-    take_record(r, peek_record<kVec>(r, c, H), c, H, epoch, m, cut);
-    sh.look[i][lane] = m;
-    cut = __any_sync(0xffffffffu, cut);
-    if (lane == 0) sh.look_cut[i] = cut;
+#pragma unroll 1
+  for (unsigned from = 0; from < (kLook < kMaxSpan ? f.n : 1u); from += kLook) {
+    if (from != 0) __syncthreads();  // the records before are used
+    const unsigned n = kLook < kMaxSpan && f.n - from > kLook ? kLook : f.n - from;
+    for (unsigned i = w; i < n; i += kWarps) {
+      const ulonglong2* r = f.first + (from + i) * f.step;
+      unsigned cut;
+      Map<V> m;
+      take_record(r, peek_record<kVec>(r, c, H), c, H, epoch, m, cut);
+      sh.look[i][lane] = m;
+      cut = __any_sync(0xffffffffu, cut);
+      if (lane == 0) sh.look_cut[i] = cut;
+    }
+    __syncthreads();
+    for (unsigned i = 0; i < n; ++i) y = apply(sh.look[i][lane], sh.look_cut[i] != 0, y);
   }
-  __syncthreads();
-  for (unsigned i = 0; i < f.n; ++i) y = apply(sh.look[i][lane], sh.look_cut[i] != 0, y);
 }
 
 // The maps of the warps before warp w in the scan's direction, composed.
@@ -613,19 +620,20 @@ __device__ __forceinline__ void forward_steps(const char* row, const V (&a)[kSte
   }
 }
 
-// CTAs per SM: three for fp32 (80 registers a thread are enough for one channel a lane: 154 us against 177 with two
-// for 1 x 65539 x 1024); two-channel lanes need 128.
-template <typename T>
-constexpr int forward_ctas() {
-  return sizeof(T) == 4 ? 3 : 2;
-}
+// CTAs per SM: three, except in the sigmoid form of 16 bits, whose a and v of two channels take 128 registers a thread.
+// Measured with two and with three: 1 x 65539 x 1024 fp32 177 and 154 us; decay, bf16: B = 8, T = 4096, H = 2048 76.3 and
+// 73.7 us, B = 1, T = 65536, H = 1024 150 and 122 us (three need the records' buffer of two-channel lanes halved).  Sigmoid,
+// bf16, three with a and v formed again in step 4: 93.8 us instead of 85.6, and 141 instead of 157 for the long
+// sequence; with 6 of the 16 kept in registers 88.5 and 142.
+template <typename T, int kForm>
+constexpr bool kThreeCtas = sizeof(T) == 4 || kForm == kDecay;
 
 template <typename T, int kForm>
-__global__ void __launch_bounds__(kThreads, forward_ctas<T>()) forward_kernel(const __grid_constant__ Forward<T> p) {
+__global__ void __launch_bounds__(kThreads, (kThreeCtas<T, kForm> ? 3 : 2)) forward_kernel(const __grid_constant__ Forward<T> p) {
   using V = typename Lane<T>::V;
   constexpr int kVec = Lane<T>::kVec, kIn = 2;
   extern __shared__ __align__(128) char smem[];
-  __shared__ Shared<V, false> sh;
+  __shared__ Shared<V, false, kThreeCtas<T, kForm> && kVec == 2 ? kWarps : kMaxSpan> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);
@@ -842,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
   using V = typename Lane<T>::V;
   constexpr int kVec = Lane<T>::kVec, kIn = 3;
   extern __shared__ __align__(128) char smem[];
-  __shared__ Shared<V, true> sh;
+  __shared__ Shared<V, true, kMaxSpan> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
   const unsigned epoch = launch_epoch(p.g);

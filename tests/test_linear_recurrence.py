@@ -133,6 +133,14 @@ def test_long_narrow(ops, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("form", ["decay", "sigmoid"])
+def test_long_narrow_16_bits(ops, dtype, form):
+    """Several blocks of records, each brought in more than one round where a lane has two channels, with resets."""
+    check(ops, make(2, 6011, 72, dtype, form, seed=77, reset_p=1e-3), form)
+
+
+@pytest.mark.gpu
 def test_many_channels(ops):
     check(ops, make(16, 260, 1030, torch.bfloat16, "sigmoid", seed=6, reset_p=0.01), "sigmoid")
 
