@@ -162,10 +162,12 @@ def calls():
     or was built for another torch: ctypes serves their calls then."""
     load()
     try:
+        import torch
+
         from . import _calls
+        _calls.init(str(library_path()), OpError, torch.__version__)
     except ImportError:
         return None
-    _calls.init(str(library_path()), OpError)
     return _calls
 
 

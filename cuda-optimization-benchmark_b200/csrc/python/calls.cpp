@@ -20,7 +20,9 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
+#include <cstring>
 #include <map>
 #include <optional>
 #include <tuple>
@@ -48,6 +50,16 @@ ENTRY(b200_policy_loss_workspace_bytes);
 ENTRY(b200_policy_loss_async);
 ENTRY(b200_preference_loss_workspace_bytes);
 ENTRY(b200_preference_loss_async);
+
+// Other threads run Python while a call allocates and launches (a launch waits when the GPU's queue is full).
+template <typename F>
+int unlocked(F&& f) {
+  struct NoGil {
+    PyThreadState* state = PyEval_SaveThread();
+    ~NoGil() { PyEval_RestoreThread(state); }
+  } no_gil;
+  return f();
+}
 
 // What a call works on: the current device and its current stream.
 struct Place {
@@ -107,7 +119,7 @@ bool stream_ok(const Tensor* t, const Place& p, at::ScalarType type, int64_t B, 
   return t == nullptr || (rows(*t, p, type, 2) && t->size(0) == B && t->size(1) == T);
 }
 int64_t row_stride(const Tensor* t) { return t == nullptr ? 0 : t->stride(0); }
-void* at_(const Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }
+void* at_(const Tensor* t) { return t == nullptr || !t->defined() ? nullptr : t->data_ptr(); }
 template <typename T>
 T* ptr(const Tensor* t) {
   return static_cast<T*>(at_(t));
@@ -214,15 +226,17 @@ PyObject* recurrence(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t bytes = b200_linear_recurrence_workspace_bytes_(int(B), int(T), int(H));
   const Tensor* ws = nullptr;
   ORDINARY(bytes == 0 || (ws = scratch(kRecurrence, bytes, *p)) != nullptr);
-  Tensor h = like_bth(*x, *p), final_state = make({B, H}, at::kFloat, *p), ckpt;
-  if (a[5] == Py_True)
-    ckpt = make({b200_linear_recurrence_checkpoint_bytes_(int(B), int(T), int(H)) / 4}, at::kFloat, *p);
-  const int64_t st[8] = {gate->stride(0), gate->stride(1), x->stride(0), x->stride(1), h.stride(0), h.stride(1),
-                         reset ? reset->stride(0) : 0, reset ? reset->stride(1) : 0};
-  const int status = b200_linear_recurrence_async_(
-      gate->data_ptr(), x->data_ptr(), dtype, form, st, ptr<float>(state), ptr<uint8_t>(reset), int(B), int(T), int(H),
-      h.data_ptr(), final_state.data_ptr<float>(), ckpt.defined() ? ckpt.data_ptr<float>() : nullptr, at_(ws),
-      ws ? ws->numel() : 0, p->stream);
+  Tensor h, final_state, ckpt;
+  const bool train = a[5] == Py_True;
+  const int status = unlocked([&] {
+    h = like_bth(*x, *p), final_state = make({B, H}, at::kFloat, *p);
+    if (train) ckpt = make({b200_linear_recurrence_checkpoint_bytes_(int(B), int(T), int(H)) / 4}, at::kFloat, *p);
+    const int64_t st[8] = {gate->stride(0), gate->stride(1), x->stride(0), x->stride(1), h.stride(0), h.stride(1),
+                           reset ? reset->stride(0) : 0, reset ? reset->stride(1) : 0};
+    return b200_linear_recurrence_async_(
+        gate->data_ptr(), x->data_ptr(), dtype, form, st, ptr<float>(state), ptr<uint8_t>(reset), int(B), int(T), int(H),
+        h.data_ptr(), ptr<float>(&final_state), ptr<float>(&ckpt), at_(ws), ws ? ws->numel() : 0, p->stream);
+  });
   return done(status, "linear_recurrence", h, final_state, ckpt);
   END
 }
@@ -243,14 +257,18 @@ PyObject* recurrence_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t bytes = b200_linear_recurrence_workspace_bytes_(int(B), int(T), int(H));
   const Tensor* ws = nullptr;
   ORDINARY(bytes == 0 || (ws = scratch(kRecurrence, bytes, *p)) != nullptr);
-  Tensor gg = like_bth(*gate, *p), gx = like_bth(*x, *p), gs = make({B, H}, at::kFloat, *p);
-  const int64_t st[12] = {gate->stride(0), gate->stride(1), x->stride(0),  x->stride(1),
-                          dh->stride(0),   dh->stride(1),   gg.stride(0),  gg.stride(1),
-                          gx.stride(0),    gx.stride(1),    reset ? reset->stride(0) : 0, reset ? reset->stride(1) : 0};
-  const int status = b200_linear_recurrence_backward_async_(
-      gate->data_ptr(), x->data_ptr(), dtype, form, st, ptr<float>(ckpt), ptr<uint8_t>(reset), dh->data_ptr(),
-      ptr<float>(df), int(B), int(T), int(H), gg.data_ptr(), gx.data_ptr(), gs.data_ptr<float>(), at_(ws),
-      ws ? ws->numel() : 0, p->stream);
+  Tensor gg, gx, gs;
+  const int status = unlocked([&] {
+    gg = like_bth(*gate, *p), gx = like_bth(*x, *p), gs = make({B, H}, at::kFloat, *p);
+    const int64_t st[12] = {gate->stride(0), gate->stride(1), x->stride(0), x->stride(1),
+                            dh->stride(0),   dh->stride(1),   gg.stride(0), gg.stride(1),
+                            gx.stride(0),    gx.stride(1),    reset ? reset->stride(0) : 0,
+                            reset ? reset->stride(1) : 0};
+    return b200_linear_recurrence_backward_async_(
+        gate->data_ptr(), x->data_ptr(), dtype, form, st, ptr<float>(ckpt), ptr<uint8_t>(reset), dh->data_ptr(),
+        ptr<float>(df), int(B), int(T), int(H), gg.data_ptr(), gx.data_ptr(), ptr<float>(&gs), at_(ws),
+        ws ? ws->numel() : 0, p->stream);
+  });
   return done(status, "linear_recurrence_backward", gg, gx, gs);
   END
 }
@@ -276,11 +294,14 @@ PyObject* recurrence_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t bytes = S * H * 4;
     ORDINARY(s == o || s + bytes <= o || o + bytes <= s);
   }
-  Tensor h = make({B, H}, x->scalar_type(), *p);
-  const int64_t st[3] = {gate->stride(0), x->stride(0), H};
-  const int status = b200_linear_recurrence_step_async_(gate->data_ptr(), x->data_ptr(), dtype, form, st, ptr<float>(state),
-                                                        ptr<float>(next ? next : state), ptr<int32_t>(slots), int(S),
-                                                        int(B), int(H), h.data_ptr(), p->stream);
+  Tensor h;
+  const int status = unlocked([&] {
+    h = make({B, H}, x->scalar_type(), *p);
+    const int64_t st[3] = {gate->stride(0), x->stride(0), H};
+    return b200_linear_recurrence_step_async_(gate->data_ptr(), x->data_ptr(), dtype, form, st, ptr<float>(state),
+                                              ptr<float>(next ? next : state), ptr<int32_t>(slots), int(S), int(B),
+                                              int(H), h.data_ptr(), p->stream);
+  });
   return done(status, "linear_recurrence_step", h);
   END
 }
@@ -312,17 +333,19 @@ PyObject* logprob(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int dtype = code_of(*x);
   const double temperature = PyFloat_AS_DOUBLE(a[2]);
   ORDINARY(dtype >= 0 && temperature >= 1e-30 && temperature <= 1e30 && place_of(*x, &p) && logits_ok(*x, *token, *p, &q));
-  Tensor lp = make(token->sizes(), at::kFloat, *p), ent, stats;
-  if (a[3] == Py_True) ent = make(token->sizes(), at::kFloat, *p);
-  if (a[4] == Py_True) {
-    at::DimVector shape(token->sizes().begin(), token->sizes().end());
-    shape.push_back(3);
-    stats = make(shape, at::kFloat, *p);
-  }
-  const int status = b200_token_logprob_async_(x->data_ptr(), dtype, q.st, token->data_ptr<int64_t>(), int(q.B), int(q.T),
-                                               int(q.V), temperature, lp.data_ptr<float>(),
-                                               ent.defined() ? ent.data_ptr<float>() : nullptr,
-                                               stats.defined() ? stats.data_ptr<float>() : nullptr, p->stream);
+  Tensor lp, ent, stats;
+  const bool entropy = a[3] == Py_True, train = a[4] == Py_True;
+  const int status = unlocked([&] {
+    lp = make(token->sizes(), at::kFloat, *p);
+    if (entropy) ent = make(token->sizes(), at::kFloat, *p);
+    if (train) {
+      at::DimVector shape(token->sizes().begin(), token->sizes().end());
+      shape.push_back(3);
+      stats = make(shape, at::kFloat, *p);
+    }
+    return b200_token_logprob_async_(x->data_ptr(), dtype, q.st, ptr<int64_t>(token), int(q.B), int(q.T), int(q.V),
+                                     temperature, ptr<float>(&lp), ptr<float>(&ent), ptr<float>(&stats), p->stream);
+  });
   return done(status, "token_logprob", lp, ent, stats);
   END
 }
@@ -342,10 +365,13 @@ PyObject* logprob_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   shape.push_back(3);
   ORDINARY(dense(*stats, *p, at::kFloat, shape) && dense(*gl, *p, at::kFloat, token->sizes()) &&
            (ge == nullptr || dense(*ge, *p, at::kFloat, token->sizes())));
-  Tensor out = make(x->sizes(), x->scalar_type(), *p);
-  const int status = b200_token_logprob_backward_async_(x->data_ptr(), dtype, q.st, token->data_ptr<int64_t>(),
-                                                        ptr<float>(stats), ptr<float>(gl), ptr<float>(ge), int(q.B),
-                                                        int(q.T), int(q.V), temperature, out.data_ptr(), p->stream);
+  Tensor out;
+  const int status = unlocked([&] {
+    out = make(x->sizes(), x->scalar_type(), *p);
+    return b200_token_logprob_backward_async_(x->data_ptr(), dtype, q.st, ptr<int64_t>(token), ptr<float>(stats),
+                                              ptr<float>(gl), ptr<float>(ge), int(q.B), int(q.T), int(q.V), temperature,
+                                              out.data_ptr(), p->stream);
+  });
   return done(status, "token_logprob_backward", out);
   END
 }
@@ -379,16 +405,19 @@ PyObject* policy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor* ws = nullptr;
   ORDINARY(bytes == 0 || (ws = scratch(kPolicy, bytes, *p)) != nullptr);
   if (old == nullptr) old = lp;
-  Tensor out = make({8}, at::kFloat, *p), grad, ge;
-  if (a[7] == Py_True) grad = make({B, T}, at::kFloat, *p);
-  if (a[8] == Py_True) ge = make({B, T}, at::kFloat, *p);
-  const int64_t st[7] = {lp->stride(0), old->stride(0), adv->stride(0), per_row ? 0 : 1,
-                         row_stride(ref), row_stride(ent), row_stride(mask)};
-  const int status = b200_policy_loss_async_(
-      ptr<float>(lp), ptr<float>(old), ptr<float>(adv), ptr<float>(ref), ptr<float>(ent), ptr<uint8_t>(mask), st, int(B),
-      int(T), o[0], o[1], o[2], o[3], int(o[4]), o[5], int(o[6]), o[7], out.data_ptr<float>(),
-      grad.defined() ? grad.data_ptr<float>() : nullptr, ge.defined() ? ge.data_ptr<float>() : nullptr, at_(ws),
-      ws ? ws->numel() : 0, p->stream);
+  Tensor out, grad, ge;
+  const bool want_grad = a[7] == Py_True, want_grad_entropy = a[8] == Py_True;
+  const int status = unlocked([&] {
+    out = make({8}, at::kFloat, *p);
+    if (want_grad) grad = make({B, T}, at::kFloat, *p);
+    if (want_grad_entropy) ge = make({B, T}, at::kFloat, *p);
+    const int64_t st[7] = {lp->stride(0),   old->stride(0),  adv->stride(0), per_row ? 0 : 1,
+                           row_stride(ref), row_stride(ent), row_stride(mask)};
+    return b200_policy_loss_async_(ptr<float>(lp), ptr<float>(old), ptr<float>(adv), ptr<float>(ref), ptr<float>(ent),
+                                   ptr<uint8_t>(mask), st, int(B), int(T), o[0], o[1], o[2], o[3], int(o[4]), o[5],
+                                   int(o[6]), o[7], ptr<float>(&out), ptr<float>(&grad), ptr<float>(&ge), at_(ws),
+                                   ws ? ws->numel() : 0, p->stream);
+  });
   return done(status, "policy_loss", out, grad, ge);
   END
 }
@@ -410,24 +439,33 @@ PyObject* preference(PyObject*, PyObject* const* a, Py_ssize_t n) {
            stream_ok(mr, *p, at::kBool, B, Tr));
   const Tensor* ws = scratch(kPreference, b200_preference_loss_workspace_bytes_(int(B)), *p);
   ORDINARY(ws != nullptr);
-  Tensor out = make({3}, at::kFloat, *p), rc = make({B}, at::kFloat, *p), rr = make({B}, at::kFloat, *p), gc, gr;
-  if (a[8] == Py_True) gc = make({B, Tc}, at::kFloat, *p);
-  if (a[9] == Py_True) gr = make({B, Tr}, at::kFloat, *p);
-  const int64_t st[6] = {c->stride(0), r->stride(0), row_stride(fc), row_stride(fr), row_stride(mc), row_stride(mr)};
-  const int status = b200_preference_loss_async_(
-      ptr<float>(c), ptr<float>(r), ptr<float>(fc), ptr<float>(fr), ptr<uint8_t>(mc), ptr<uint8_t>(mr), st, int(B),
-      int(Tc), int(Tr), o[0], int(o[1]), o[2], o[3], a[7] == Py_True, out.data_ptr<float>(), rc.data_ptr<float>(),
-      rr.data_ptr<float>(), gc.defined() ? gc.data_ptr<float>() : nullptr, gr.defined() ? gr.data_ptr<float>() : nullptr,
-      at_(ws), ws->numel(), p->stream);
+  Tensor out, rc, rr, gc, gr;
+  const bool average = a[7] == Py_True, want_chosen = a[8] == Py_True, want_rejected = a[9] == Py_True;
+  const int status = unlocked([&] {
+    out = make({3}, at::kFloat, *p), rc = make({B}, at::kFloat, *p), rr = make({B}, at::kFloat, *p);
+    if (want_chosen) gc = make({B, Tc}, at::kFloat, *p);
+    if (want_rejected) gr = make({B, Tr}, at::kFloat, *p);
+    const int64_t st[6] = {c->stride(0),   r->stride(0),   row_stride(fc),
+                           row_stride(fr), row_stride(mc), row_stride(mr)};
+    return b200_preference_loss_async_(ptr<float>(c), ptr<float>(r), ptr<float>(fc), ptr<float>(fr), ptr<uint8_t>(mc),
+                                       ptr<uint8_t>(mr), st, int(B), int(Tc), int(Tr), o[0], int(o[1]), o[2], o[3],
+                                       average, ptr<float>(&out), ptr<float>(&rc), ptr<float>(&rr), ptr<float>(&gc),
+                                       ptr<float>(&gr), at_(ws), ws->numel(), p->stream);
+  });
   return done(status, "preference_loss", out, rc, rr, gc, gr);
   END
 }
 
-// init(path of the library, OpError)
+// init(path of the library, OpError, torch's version): ImportError for another torch than the one built for.
 PyObject* init(PyObject*, PyObject* args) {
-  const char* path;
+  const char *path, *version;
   PyObject* error;
-  if (!PyArg_ParseTuple(args, "sO", &path, &error)) return nullptr;
+  if (!PyArg_ParseTuple(args, "sOs", &path, &error, &version)) return nullptr;
+  const size_t n = strlen(TORCH_VERSION);
+  if (strncmp(version, TORCH_VERSION, n) != 0 || (version[n] != '\0' && version[n] != '+')) {
+    PyErr_Format(PyExc_ImportError, "_calls was built for torch %s, not %s", TORCH_VERSION, version);
+    return nullptr;
+  }
   void* lib = dlopen(path, RTLD_NOW | RTLD_LOCAL);
   if (lib == nullptr) {
     PyErr_Format(PyExc_OSError, "%s", dlerror());

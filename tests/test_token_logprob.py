@@ -276,3 +276,11 @@ def test_empty_and_refusals(ops):
                                                    out=x.flatten()[1:26].view(5, 5))):
         with pytest.raises((ValueError, TypeError)):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,V", [(127, 2048), (128, 2048), (511, 2048), (513, 2048), (2469, 8995), (2600, 8995)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_both_sides_of_a_warp_per_row(ops, dtype, rows, V):
+    """Row numbers on either side of where a warp takes a row alone, forward and backward."""
+    check(ops, make(1, rows, V, dtype, seed=rows), 0.9)
