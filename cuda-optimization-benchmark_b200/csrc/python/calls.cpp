@@ -125,6 +125,16 @@ T* ptr(const Tensor* t) {
   return static_cast<T*>(at_(t));
 }
 
+// Whether two tensors span different memory.
+bool apart(const Tensor& a, const Tensor& b) {
+  const auto last = [](const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+    return static_cast<const char*>(t.data_ptr()) + n * int64_t(t.element_size());
+  };
+  return last(a) <= static_cast<const char*>(b.data_ptr()) || last(b) <= static_cast<const char*>(a.data_ptr());
+}
+
 // A new tensor, without the way through torch's dispatcher.
 Tensor make(at::IntArrayRef shape, at::ScalarType type, const Place& p) {
   return at::detail::empty_cuda(shape, type, p.device, std::nullopt);
@@ -288,12 +298,10 @@ PyObject* recurrence_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
            dense(*state, *p, at::kFloat, {state->size(0), H}));
   const int64_t S = state->size(0);
   ORDINARY(slots ? dense(*slots, *p, at::kInt, {B}) : S >= B);
-  if (next != nullptr) {
-    ORDINARY(dense(*next, *p, at::kFloat, {S, H}));
-    const char *s = ptr<char>(state), *o = ptr<char>(next);
-    const int64_t bytes = S * H * 4;
-    ORDINARY(s == o || s + bytes <= o || o + bytes <= s);
-  }
+  ORDINARY(next == nullptr || (dense(*next, *p, at::kFloat, {S, H}) &&
+                               (at_(next) == at_(state) || apart(*next, *state))));
+  const Tensor& written = next ? *next : *state;
+  ORDINARY(apart(written, *gate) && apart(written, *x) && (slots == nullptr || apart(written, *slots)));
   Tensor h;
   const int status = unlocked([&] {
     h = make({B, H}, x->scalar_type(), *p);

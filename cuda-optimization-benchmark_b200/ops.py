@@ -738,6 +738,8 @@ def _apart(out, name, **inputs):
     """Refuses an output in the memory of an input."""
     lo, hi = _reach(out)
     for other, t in inputs.items():
+        if t is None:
+            continue
         a, b = _reach(t)
         if lo < b and a < hi:
             raise ValueError(f"{name} overlaps {other}")
@@ -796,7 +798,8 @@ def _recurrence_forward(gate, x, state, reset, form, out, train):
     dev, dt, fm, (B, T, H) = _bth(gate, x, form)
     state = _state_arg(state, "state", B, H, dev)
     reset = _reset_arg(reset, B, T, dev)
-    h = _like_bth(x) if out is None else _apart(_writable(out, x, "out"), "out", gate=gate, x=x)
+    h = _like_bth(x) if out is None else _apart(_writable(out, x, "out"), "out", gate=gate, x=x, state=state,
+                                                        reset=reset)
     n_ckpt, n_ws = _recurrence_sizes(B, T, H)
     final = torch.empty((B, H), dtype=torch.float32, device=dev)
     ckpt = torch.empty(n_ckpt, dtype=torch.float32, device=dev) if train else None
@@ -854,7 +857,7 @@ def linear_recurrence_backward(gate, x, checkpoints, grad_h, grad_final=None, re
 
 def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, state_out=None):
     """One token per row: h [B, H] from gate and x [B, H] and a pool of states fp32 [S, H], updated in place
-    (or written to state_out).  slots (int32 [B]) names each row's state, row b its own without it.  Rows
+    (or written to state_out, whose other rows stay as they are).  slots (int32 [B]) names each row's state, row b its own without it.  Rows
     with the same slot are consecutive tokens of one sequence, in row order; a row whose slot is outside
     [0, S) is skipped (its h row is left as it was, so pass `out` to know what it holds)."""
     if out is None:
@@ -890,6 +893,7 @@ def linear_recurrence_step(gate, x, state, slots=None, form="decay", out=None, s
         _need(slots, "slots", torch.int32, dev)
         if slots.shape != (B,):
             raise ValueError(f"slots must be ({B},)")
+    _apart(state_out, "the written state", gate=gate, x=x, slots=slots)
     h = _dense_like(x) if out is None else _apart(_writable(out, x, "out"), "out", gate=gate, x=x, state=state,
                                                        state_out=state_out)
     _run("linear_recurrence_step", _lib().b200_linear_recurrence_step_async, dev.index, gate.data_ptr(), x.data_ptr(),
@@ -1018,6 +1022,7 @@ def token_logprob_backward(logits, token, stats, grad_log_prob, grad_entropy=Non
         if out.shape != logits.shape:
             raise ValueError("out must have logits' shape")
         _check_over(out, logits)
+        _apart(out, "out", token=token, stats=stats, grad_log_prob=grad_log_prob, grad_entropy=grad_entropy)
     _run("token_logprob_backward", _lib().b200_token_logprob_backward_async, dev.index, logits.data_ptr(), dt, st,
          token.data_ptr(), stats.data_ptr(), grad_log_prob.data_ptr(), _address(grad_entropy), B, T, V, temperature,
          out.data_ptr())

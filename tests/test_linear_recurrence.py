@@ -418,3 +418,21 @@ def test_refusals(ops):
         p = x.data_ptr()
         assert lib.b200_linear_recurrence_async(p, p, 0, 0, st, None, None, 2, 300, 4, p, None, None, p, need - 1,
                                                 None) == 4
+
+
+@pytest.mark.gpu
+def test_refuses_inputs_in_the_written_state(ops):
+    pool = torch.randn(8, 40, device="cuda")
+    gate, x = torch.rand(2, 40, device="cuda"), torch.randn(2, 40, device="cuda")
+    slots = torch.tensor([7, 6], dtype=torch.int32, device="cuda")
+    before = pool.clone()
+    for kw in (dict(gate=pool[:2], x=x), dict(gate=gate, x=pool[1:5:2])):
+        with pytest.raises(ValueError, match="written state overlaps"):
+            ops.linear_recurrence_step(state=pool, slots=slots, **kw)
+        with pytest.raises(ValueError, match="written state overlaps"):
+            ops.linear_recurrence_step(state=before, slots=slots, state_out=pool, **kw)
+    assert torch.equal(pool, before)
+    ops.linear_recurrence_step(gate, before[:2], pool, slots)          # reading another pool is fine
+    state = torch.randn(2, 40, device="cuda")
+    with pytest.raises(ValueError, match="out overlaps state"):
+        ops.linear_recurrence(gate[:, None], x[:, None], state, out=state[:, None])

@@ -284,3 +284,16 @@ def test_empty_and_refusals(ops):
 def test_both_sides_of_a_warp_per_row(ops, dtype, rows, V):
     """Row numbers on either side of where a warp takes a row alone, forward and backward."""
     check(ops, make(1, rows, V, dtype, seed=rows), 0.9)
+
+
+@pytest.mark.gpu
+def test_backward_refuses_an_output_over_its_inputs(ops):
+    s = make(1, 6, 50, torch.float32, seed=2)
+    lp, ent, stats = ops.token_logprob_train(s["logits"], s["token"])
+    whole = torch.zeros(300 + 18, device="cuda")
+    inside = whole[300:].view(1, 6, 3).copy_(stats)
+    ops.token_logprob_backward(s["logits"], s["token"], inside, s["gl"], out=whole[:300].view(1, 6, 50))
+    with pytest.raises(ValueError, match="out overlaps stats"):
+        ops.token_logprob_backward(s["logits"], s["token"], inside, s["gl"], out=whole[18:].view(1, 6, 50))
+    with pytest.raises(ValueError, match="out overlaps grad_log_prob"):
+        ops.token_logprob_backward(s["logits"], s["token"], stats, whole[:6].view(1, 6), out=whole[:300].view(1, 6, 50))
