@@ -74,7 +74,7 @@ struct Strides {  // in elements; the channel axis is contiguous
 
 // Control words of the workspace: zero before the first launch, and ready for the next after each.
 struct Ctl {
-  unsigned ticket, done, epoch;
+  unsigned ticket, epoch;  // tickets taken in this launch, epoch of the one before
 };
 
 __host__ __device__ inline int64_t tiles(int64_t T) { return (T + kTile - 1) / kTile; }
@@ -289,6 +289,7 @@ struct Grid {
   int H;
   unsigned groups, chains, n_tiles, total;  // chains = B * groups; total = chains * n_tiles
   unsigned span;
+  bool one;          // every CTA takes one ticket: there are as many as tiles
   Ctl* ctl;          // null when a row is one tile: no tile waits for another, CTAs take tiles in turn
   ulonglong2* recs;  // [n_tiles, B, H]
   bool back;         // the scan runs from the last tile to the first
@@ -330,6 +331,7 @@ struct Shared {
   uint64_t cut;                  // byte w: warp w's steps hold a reset, its map does not see what comes in
   Tile tile[2];                  // of the CTA's tiles in turn
   uint64_t full[2];              // the tile buffers' loads have landed (tensor loads)
+  unsigned epoch;                // the launch's
 };
 
 // The map applied to y; a map with a cut drops y, whatever it holds.
@@ -467,28 +469,30 @@ __device__ __forceinline__ Map<V> before_warp(const Map<V> (&map)[kWarps][32], u
 
 __device__ __forceinline__ bool ends_block(const Grid& g, unsigned k) { return (k & (g.span - 1)) == g.span - 1; }
 
-// Ends the launch's use of the workspace (the clerk, which takes no more tickets): the last CTA to leave makes it
-// ready for the next launch.
-__device__ __forceinline__ void leave(const Grid& g, unsigned epoch) {
-  if (g.ctl == nullptr || threadIdx.x != kClerk * 32) return;
-  __threadfence();
-  if (atomicAdd(&g.ctl->done, 1u) == gridDim.x - 1) {
-    g.ctl->ticket = 0;
-    g.ctl->done = 0;
-    g.ctl->epoch = epoch;
+// Tickets, by the clerk.  The first comes with the launch's epoch: 31 bits, never 0 (a zero-filled record belongs to no
+// launch).
+__device__ __forceinline__ unsigned first_ticket(const Grid& g, unsigned& epoch) {
+  epoch = 1u;
+  if (g.ctl == nullptr) return blockIdx.x;
+  unsigned before;  // read before this CTA's ticket is counted
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(before) : "l"(&g.ctl->epoch) : "memory");
+  const unsigned e = (before + 1u) & 0x7fffffffu;
+  epoch = e == 0u ? 1u : e;
+  return atomicAdd(&g.ctl->ticket, 1u);
+}
+// The next one; where every CTA takes one only, a ticket past the last tile.
+__device__ __forceinline__ unsigned next_ticket(const Grid& g, unsigned last) {
+  if (g.ctl == nullptr) return last + gridDim.x;
+  return g.one ? g.total : atomicAdd(&g.ctl->ticket, 1u);
+}
+// A CTA stops at its first ticket past the last tile, so every launch takes the same number of them, and who has the last
+// leaves the workspace ready for the next launch.
+__device__ __forceinline__ void settle(const Grid& g, unsigned ticket, unsigned epoch) {
+  if (g.ctl != nullptr && ticket == (g.one ? g.total : g.total + gridDim.x) - 1u) {
     __threadfence();
+    g.ctl->ticket = 0;
+    g.ctl->epoch = epoch;
   }
-}
-
-__device__ __forceinline__ unsigned take_ticket(const Grid& g, unsigned last) {
-  return g.ctl != nullptr ? atomicAdd(&g.ctl->ticket, 1u) : last + gridDim.x;
-}
-
-// The launch's epoch: 31 bits, never 0 (a zero-filled record belongs to no launch).
-__device__ __forceinline__ unsigned launch_epoch(const Grid& g) {
-  if (g.ctl == nullptr) return 1u;
-  const unsigned e = (ld_cg_u32(&g.ctl->epoch) + 1u) & 0x7fffffffu;
-  return e == 0u ? 1u : e;
 }
 
 // The resets of one warp's steps as bits (bit i: step i of the warp).
@@ -636,8 +640,6 @@ __global__ void __launch_bounds__(kThreads, (kThreeCtas<T, kForm> ? 3 : 2)) forw
   __shared__ Shared<V, false, kThreeCtas<T, kForm> && kVec == 2 ? kWarps : kMaxSpan> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
-  const unsigned epoch = launch_epoch(p.g);
-
   // A tile's loads: tensor loads by one thread, or this warp's own rows.
   const auto load_all = [&](const Tile& t, unsigned buf) {
     if (!t.live) return;
@@ -666,11 +668,15 @@ __global__ void __launch_bounds__(kThreads, (kThreeCtas<T, kForm> ? 3 : 2)) forw
     mbar_init(&sh.full[0], 1);
     mbar_init(&sh.full[1], 1);
     fence_barrier_init();
-    ahead = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
+    unsigned e;
+    ahead = first_ticket(p.g, e);
     sh.tile[0] = tile_of(p.g, ahead);
     if (p.tma) load_all(sh.tile[0], 0);
+    sh.epoch = e;
+    settle(p.g, ahead, e);
   }
   __syncthreads();
+  const unsigned epoch = sh.epoch;
   if (own) fetch_own(sh.tile[0], 0);
   for (unsigned it = 0;; ++it) {
     const unsigned buf = it & 1u;
@@ -693,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, (kThreeCtas<T, kForm> ? 3 : 2)) forw
       }
     }
     // The next ticket, once the rows are there: by then every CTA has its first.
-    if (clerk) ahead = take_ticket(p.g, ahead);
+    if (clerk) ahead = next_ticket(p.g, ahead);
     const unsigned resets = own ? __ballot_sync(0xffffffffu, reset_byte != 0) : 0u;
     const char* row = rows + lane * 4;
 
@@ -745,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, (kThreeCtas<T, kForm> ? 3 : 2)) forw
       forward_steps<T, kForm, true>(row, a, u, resets, n, c, p.g.H, p.wide, out, p.hs.t, y);
     if (p.final_state != nullptr && n > 0 && t0 + n == p.g.T) store_row(p.final_state + state_at, c, p.g.H, y);
   }
-  leave(p.g, epoch);
+  if (clerk) settle(p.g, ahead, epoch);
 }
 
 // ------------------------------------------------------------------------------------ backward
@@ -853,8 +859,6 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
   __shared__ Shared<V, true, kMaxSpan> sh;
   const unsigned lane = threadIdx.x % 32, w = threadIdx.x / 32;
   pdl_begin();
-  const unsigned epoch = launch_epoch(p.g);
-
   // A tile's loads: tensor loads by one thread, or this warp's own rows.
   const auto load_all = [&](const Tile& t, unsigned buf) {
     if (!t.live) return;
@@ -886,11 +890,15 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
     mbar_init(&sh.full[0], 1);
     mbar_init(&sh.full[1], 1);
     fence_barrier_init();
-    ahead = p.g.ctl != nullptr ? atomicAdd(&p.g.ctl->ticket, 1u) : blockIdx.x;
+    unsigned e;
+    ahead = first_ticket(p.g, e);
     sh.tile[0] = tile_of(p.g, ahead);
     if (p.tma) load_all(sh.tile[0], 0);
+    sh.epoch = e;
+    settle(p.g, ahead, e);
   }
   __syncthreads();
+  const unsigned epoch = sh.epoch;
   if (own) fetch_own(sh.tile[0], 0);
   for (unsigned it = 0;; ++it) {
     const unsigned buf = it & 1u;
@@ -917,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
       }
     }
     // The next ticket, once the rows are there: by then every CTA has its first.
-    if (clerk) ahead = take_ticket(p.g, ahead);
+    if (clerk) ahead = next_ticket(p.g, ahead);
     const unsigned resets = own ? __ballot_sync(0xffffffffu, reset_byte != 0) : 0u;
     const char* row = rows + lane * 4;
 
@@ -981,7 +989,7 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
     }
     if (p.grad_state != nullptr && t0 == 0) store_row(p.grad_state + state_at, c, p.g.H, y);
   }
-  leave(p.g, epoch);
+  if (clerk) settle(p.g, ahead, epoch);
 }
 
 // T = 0: what comes in goes out.
@@ -1086,6 +1094,7 @@ inline int plan(Kernel kernel, int smem, int vec, int64_t B, int64_t T, int64_t 
   if (!ensure_dyn_smem(kernel, smem)) return kCudaError;
   const unsigned resident = unsigned(sm_count() * resident_ctas_per_sm(kernel, kThreads, size_t(smem)));
   *ctas = resident < g->total ? resident : g->total;
+  g->one = *ctas == g->total;
   // Tiles of one chain that are worked on at once, rounded up to a power of two.
   unsigned span = 1;
   while (span < kMaxSpan && span * g->chains < resident) span *= 2;
