@@ -15,9 +15,9 @@
 // What bounds it: memory for many tokens (25 bytes a token with all streams), a launch's latency for few.  The weights
 // of the means need the number of tokens first, so a small kernel counts the mask (a byte a token) and the main one,
 // whose loads run ahead meanwhile, follows it; up to kSmallTokens tokens and kSmallRows rows one CTA does both in one
-// launch.  Measured: 16 x 256 tokens 4.7 us; 61 x 4099 12.1 us; 4096 x 1000 with an entropy 23.4 us (4.4 TB/s), 20.2
-// us (5.1 TB/s) without the counting (sum).  Loads through registers, without the bulk copies, took 30 us, and counts
-// by a warp per row 26 us.
+// launch.  Measured: 16 x 256 tokens 4.6 us; 61 x 4099 11.3 us; 4096 x 1000 with an entropy 21.9 us (4.7 TB/s), 19.2
+// us (5.3 TB/s) without the counting (sum).  Loads through registers, without the bulk copies, took 30 us.  With a
+// reference and k3 instructions are the bound (25 us).
 //
 // A token is clipped or not by a step in its gradient, so the comparison is exact: cur - old as an
 // unrounded pair of floats (s, e) against log(1 + clip_high) and log(1 - clip_low) as pairs.
@@ -575,13 +575,15 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__
 }
 
 // Dense streams on 16-byte boundaries: stretches of kUnit tokens arrive in shared memory by bulk copies, kStages
-// ahead, so that loads never wait for arithmetic.  A thread has kVecs times four consecutive tokens.  What is left of
+// ahead, so that loads never wait for arithmetic.  A thread has four consecutive tokens of a stretch.  What is left of
 // less than a stretch goes through registers.
+// Measured with inputs and outputs out of L2, 4096 x 1000 tokens with an entropy (the same with reduction sum, and 16384 x
+// 1000 of that): 24.9 us (22.4, 67.0: 6.1 TB/s); with three stages 24.5 (23.4, 75.4), with two of 2048 tokens 26.6 (24.4,
+// 76.7), with four CTAs per SM, whose 64 registers spill, 29.3 (25.9, 73.4).
 // Behind a count kernel the copies start before the counts are there: every CTA of that lets this kernel
 // start only after it has itself waited for the kernels before it, so the inputs are complete.
 constexpr int kStages = 2;
-constexpr int kVecs = 2;  // vectors of kPer tokens per thread and stretch
-constexpr unsigned kUnit = kThreads * kPer * kVecs;
+constexpr unsigned kUnit = kThreads * kPer;
 constexpr unsigned kStreamBytes = kUnit * 4u;
 
 struct Streams {
@@ -626,54 +628,48 @@ __global__ void __launch_bounds__(kThreads, 3) dense_kernel(const __grid_constan
   for (unsigned u = blockIdx.x; u < whole; u += gridDim.x) {
     mbar_wait(&full[stage], parity);
     const char* base = smem + stage * stage_bytes;
+    const unsigned at = threadIdx.x, first = u * kUnit + at * kPer;
+    Raw r;
+    const auto take4 = [&](int s, float (&f)[kPer]) {
+      const float4 v = *reinterpret_cast<const float4*>(base + st.slot[s] * kStreamBytes + at * (kPer * 4));
+      f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    };
+    if (p.need_row) {
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-      const unsigned at = k * kThreads + threadIdx.x, first = u * kUnit + at * kPer;
-      Raw r;
-      const auto take4 = [&](int s, float (&f)[kPer]) {
-        const float4 v = *reinterpret_cast<const float4*>(base + st.slot[s] * kStreamBytes + at * (kPer * 4));
-        f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-      };
-      if (p.need_row) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const bool again = j > 0 && p.T % kPer == 0;  // the first token's row
-          const unsigned row = again ? r.row[0] : p.by_T.div(first + j);
-          r.row[j] = row;
-          if (per_row && counted) w[j] = again ? w[0] : token_weight(p, c.tokens, c.rows, counts[row]);
-          if (p.adv_rows) r.adv[j] = again ? r.adv[0] : p.adv[int64_t(row) * p.adv_s];
-        }
+      for (int j = 0; j < kPer; ++j) {
+        const bool again = j > 0 && p.T % kPer == 0;  // the first token's row
+        const unsigned row = again ? r.row[0] : p.by_T.div(first + j);
+        r.row[j] = row;
+        if (per_row && counted) w[j] = again ? w[0] : token_weight(p, c.tokens, c.rows, counts[row]);
+        if (p.adv_rows) r.adv[j] = again ? r.adv[0] : p.adv[int64_t(row) * p.adv_s];
       }
-      take4(0, r.cur);
-      take4(1, r.old);
-      if (!p.adv_rows) take4(2, r.adv);
-      if (p.ref != nullptr) take4(3, r.ref);
-      if (p.ent != nullptr) take4(4, r.ent);
-      r.on = p.mask == nullptr
-                 ? ~0u
-                 : count_word(*reinterpret_cast<const uint32_t*>(base + st.n * kStreamBytes + at * kPer));
-      float g[kPer], ge[kPer];
-      take_tokens(p, r, w, a, g, ge);
-      write_tokens<true>(p, first, g, ge);
     }
+    take4(0, r.cur);
+    take4(1, r.old);
+    if (!p.adv_rows) take4(2, r.adv);
+    if (p.ref != nullptr) take4(3, r.ref);
+    if (p.ent != nullptr) take4(4, r.ent);
+    r.on = p.mask == nullptr
+               ? ~0u
+               : count_word(*reinterpret_cast<const uint32_t*>(base + st.n * kStreamBytes + at * kPer));
+    float g[kPer], ge[kPer];
+    take_tokens(p, r, w, a, g, ge);
+    write_tokens<true>(p, first, g, ge);
     __syncthreads();  // the stage is read
     if (threadIdx.x == 0) fetch(u + kStages * gridDim.x, stage);
     if (++stage == unsigned(kStages)) stage = 0, parity ^= 1u;
   }
   if (blockIdx.x == gridDim.x - 1 && whole * kUnit < p.n) {
-#pragma unroll 1
-    for (unsigned v = 0; v < unsigned(kVecs); ++v) {
-      const unsigned first = whole * kUnit + (v * kThreads + threadIdx.x) * kPer;
-      Raw r;
-      load_tokens<true>(p, first, r);
-      if (per_row && counted) {
+    const unsigned first = whole * kUnit + threadIdx.x * kPer;
+    Raw r;
+    load_tokens<true>(p, first, r);
+    if (per_row && counted) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) w[j] = token_weight(p, c.tokens, c.rows, counts[r.row[j]]);
-      }
-      float g[kPer], ge[kPer];
-      take_tokens(p, r, w, a, g, ge);
-      write_tokens<true>(p, first, g, ge);
+      for (int j = 0; j < kPer; ++j) w[j] = token_weight(p, c.tokens, c.rows, counts[r.row[j]]);
     }
+    float g[kPer], ge[kPer];
+    take_tokens(p, r, w, a, g, ge);
+    write_tokens<true>(p, first, g, ge);
   }
   finish(p, a, counted, ctl, counts, sums);
 }
